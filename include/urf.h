@@ -584,6 +584,47 @@ int urf_search_by_projection_slot(const urf_sbp_config *cfg, const void *d_slot,
 int urf_cv_find_fundamental(const float *pts0, const float *pts1, int n, double thresh, double confidence, uint8_t *mask,
                             double *F9, int *iterations, int device);
 
+/* ------------------------------------------- operators for adapting a matcher ---- */
+/* What lies between a matcher's activations and a gradient, on device tensors the caller owns: attention with its backward pass
+ * (the 18 multi-head attentions of SuperGlue, src/super_glue.cpp:243-300, in any size), log probabilities of given candidates, and
+ * distillation from a teacher's top alternatives.  The upstream fine-tunes its networks outside the C++ path
+ * (superpoint/train.py:11-43); these calls let a training program use the GPU the matcher runs on.
+ * Asynchronous on `stream` (hipStream_t of `device`; NULL = its null stream).  No call allocates, synchronises or keeps anything:
+ * scratch is the caller's d_work (16-byte aligned, at least the bytes its workspace query names, one per call in flight), so that a
+ * call may be captured into a graph as it is.  The calling thread's current device is left as it was.  Outputs may not overlap
+ * inputs.  Every output is the same bits in every run: no atomics, fixed orders of summation. */
+#define URF_F32 0
+#define URF_F16 1
+#define URF_BF16 2
+
+typedef struct {
+  int dtype;                  /* URF_F32, URF_F16, URF_BF16: of q, k, v, o and their gradients */
+  int batch, q_heads, kv_heads, head_dim;   /* q_heads a multiple of kv_heads (query head h reads key head h / (q_heads / kv_heads));
+                               * head_dim a multiple of 8, 8 .. 128 */
+  int q_len, k_len;           /* rows of the tensors per sequence; k_len may be 0 */
+  int causal;                 /* non-zero: row i of a sequence sees key j iff j <= i + (its keys - its rows), the last row the last key */
+  float scale;                /* of q . k; 0 -> 1 / sqrt(head_dim) */
+  int device;
+} urf_attn_config;
+/* element (b, row, head, d) at data[b * batch_stride + row * row_stride + head * head_stride + d], strides in elements, any order
+ * of the dimensions; data and strides multiples of 16 bytes.  Inputs may be broadcast (stride 0). */
+typedef struct { void *data; long long batch_stride, row_stride, head_stride; } urf_attn_tensor;
+/* bytes of d_work for urf_attn_forward (backward = 0) / urf_attn_backward (1) */
+int urf_attn_workspace(const urf_attn_config *cfg, int backward, size_t *bytes);
+/* o = softmax(scale q k^T) v per head, lse[b][head][row] = log of the row's sum of exponentials (f32, contiguous).
+ * d_q_lens / d_k_lens: device ints, rows / keys in use per sequence (NULL = all; values are clamped to the tensors).  What lies
+ * behind them is never used, whatever it holds; o is 0 and lse -infinity in rows behind q_lens and in rows that see no key.
+ * Scores, maxima, sums and accumulators are fp32; 16-bit types round the probabilities once, for the second product. */
+int urf_attn_forward(const urf_attn_config *cfg, const urf_attn_tensor *q, const urf_attn_tensor *k, const urf_attn_tensor *v,
+                     const int *d_q_lens, const int *d_k_lens, const urf_attn_tensor *o, float *d_lse, void *d_work,
+                     size_t work_bytes, void *stream);
+/* gradients of sum(o * d_o) with respect to q, k and v; o and d_lse are the forward call's, the probabilities are recomputed from
+ * them.  Heads that share a key head are summed into its dk and dv.  Rows behind q_lens / k_lens get 0. */
+int urf_attn_backward(const urf_attn_config *cfg, const urf_attn_tensor *q, const urf_attn_tensor *k, const urf_attn_tensor *v,
+                      const urf_attn_tensor *o, const float *d_lse, const urf_attn_tensor *d_o, const int *d_q_lens,
+                      const int *d_k_lens, const urf_attn_tensor *dq, const urf_attn_tensor *dk, const urf_attn_tensor *dv,
+                      void *d_work, size_t work_bytes, void *stream);
+
 /* arithmetic taps of the GPU parity tests: pure functions of their arguments (the fp32 matrix core as an ordered fma chain, the
  * canonical exp / log, IEEE division and square root, the split-f16 GEMM, one f16 matrix-core instruction).  They touch no handle. */
 int urf_probe_fma_gemm(const float *A, const float *B, const float *bias, int M, int N, int K, float *C, int device);

@@ -1,0 +1,147 @@
+// attention_api.hip -- the attention operator behind the C ABI: argument checks, the choice of the forward kernel's shape, the
+// workspace.  The kernels: attention_op.h.
+#include "attention_op.h"
+
+#include <math.h>
+
+namespace urf {
+hipError_t attn_forward_f32(const AttnArgs &, int, hipStream_t);
+hipError_t attn_forward_f16(const AttnArgs &, int, hipStream_t);
+hipError_t attn_forward_bf16(const AttnArgs &, int, hipStream_t);
+hipError_t attn_backward_f32(const AttnArgs &, hipStream_t);
+hipError_t attn_backward_f16(const AttnArgs &, hipStream_t);
+hipError_t attn_backward_bf16(const AttnArgs &, hipStream_t);
+}  // namespace urf
+using namespace urf;
+
+namespace {
+
+struct Shape { int narrow, splits; };
+
+// How the forward pass is cut.  128-row workgroups read the keys least often; where they are fewer than the 256 CUs, 32-row
+// workgroups; where those are fewer as well, the keys are split until there are two workgroups per CU, at least 256 keys each.
+Shape forward_shape(const urf_attn_config &c) {
+  const long long rows = (long long)c.q_len * (c.q_heads / c.kv_heads), groups = (long long)c.batch * c.kv_heads;
+  if ((rows + 127) / 128 * groups >= 256) return {0, 1};
+  const long long blocks = (rows + 31) / 32 * groups;
+  if (blocks >= 256) return {1, 1};
+  const long long most = (c.k_len + 255) / 256, want = (512 + blocks - 1) / blocks;
+  const long long s = want < most ? want : most;
+  return {1, (int)(s < 1 ? 1 : s > 64 ? 64 : s)};
+}
+
+size_t forward_bytes(const urf_attn_config &c) {
+  const Shape sh = forward_shape(c);
+  if (sh.splits == 1) return 0;
+  const size_t rows = ((size_t)c.q_len * (c.q_heads / c.kv_heads) + 31) / 32 * 32 * c.batch * c.kv_heads * sh.splits;
+  return rows * ((c.head_dim <= 64 ? 64 : 128) + 2) * sizeof(float);
+}
+
+size_t backward_bytes(const urf_attn_config &c) { return (size_t)c.batch * c.q_heads * c.q_len * sizeof(float); }
+
+int check_config(const urf_attn_config *c, const char *who) {
+  URF_CHECK(c, "%s: null configuration", who);
+  URF_CHECK(dtype_bytes(c->dtype), "%s: element type %d (URF_F32, URF_F16 or URF_BF16)", who, c->dtype);
+  URF_CHECK(c->batch >= 1 && c->q_len >= 1 && c->k_len >= 0, "%s: batch %d, %d rows, %d keys", who, c->batch, c->q_len, c->k_len);
+  URF_CHECK(c->kv_heads >= 1 && c->q_heads >= 1 && c->q_heads % c->kv_heads == 0, "%s: %d query heads over %d key heads", who, c->q_heads, c->kv_heads);
+  URF_CHECK(c->head_dim >= 8 && c->head_dim <= 128 && c->head_dim % 8 == 0, "%s: head size %d (a multiple of 8 up to 128)", who, c->head_dim);
+  URF_CHECK(isfinite(c->scale) && c->scale >= 0.0f, "%s: scale %g", who, (double)c->scale);
+  // row and key indices and the grid are 32-bit; element offsets are 64-bit
+  const long long rows = (long long)c->q_len * (c->q_heads / c->kv_heads), groups = (long long)c->batch * c->kv_heads;
+  URF_CHECK(rows <= (1ll << 30) && c->k_len <= (1 << 30) && groups * ((rows + 31) / 32) <= (1ll << 24) * 64 && groups * ((c->k_len + 31) / 32) <= (1ll << 24) * 64 &&
+            (long long)c->batch * c->q_heads <= (1ll << 30), "%s: too many rows, keys or heads", who);
+  return 0;
+}
+
+int check_tensor(const urf_attn_tensor *t, const urf_attn_config *c, const char *who, const char *name) {
+  URF_CHECK(t && t->data, "%s: %s is null", who, name);
+  const long long per = 16 / dtype_bytes(c->dtype);
+  URF_CHECK(((uintptr_t)t->data & 15) == 0 && t->batch_stride % per == 0 && t->row_stride % per == 0 && t->head_stride % per == 0,
+            "%s: %s: base and strides have to be multiples of 16 bytes", who, name);
+  return 0;
+}
+
+int check_out(const urf_attn_tensor *t, const urf_attn_config *c, int len, int heads, const char *who, const char *name) {
+  if (check_tensor(t, c, who, name)) return -2;
+  // two elements of an output may not share memory: no stride of a dimension longer than one below the head size
+  const long long D = c->head_dim;
+  URF_CHECK((c->batch == 1 || llabs(t->batch_stride) >= D) && (len <= 1 || llabs(t->row_stride) >= D) && (heads == 1 || llabs(t->head_stride) >= D),
+            "%s: the rows of output %s overlap", who, name);
+  return 0;
+}
+
+AttnView view(const urf_attn_tensor *t) { return {t->data, t->batch_stride, t->row_stride, t->head_stride}; }
+
+AttnArgs args_of(const urf_attn_config *c, const urf_attn_tensor *q, const urf_attn_tensor *k, const urf_attn_tensor *v, const int *d_q_lens, const int *d_k_lens) {
+  AttnArgs a = {};
+  a.q = view(q); a.k = view(k); a.v = view(v);
+  a.q_lens = d_q_lens; a.k_lens = d_k_lens;
+  a.B = c->batch; a.Hq = c->q_heads; a.Hk = c->kv_heads; a.G = c->q_heads / c->kv_heads;
+  a.Lq = c->q_len; a.Lk = c->k_len; a.D = c->head_dim; a.causal = c->causal != 0; a.splits = 1;
+  a.scale = c->scale > 0.0f ? c->scale : 1.0f / sqrtf((float)c->head_dim);
+  a.scale2 = (float)((double)a.scale * 1.4426950408889634);
+  return a;
+}
+
+}  // namespace
+
+extern "C" int urf_attn_workspace(const urf_attn_config *cfg, int backward, size_t *bytes) {
+  if (check_config(cfg, "urf_attn_workspace")) return -2;
+  URF_CHECK(bytes, "urf_attn_workspace: null pointer");
+  *bytes = backward ? backward_bytes(*cfg) : forward_bytes(*cfg);
+  return 0;
+}
+
+extern "C" int urf_attn_forward(const urf_attn_config *cfg, const urf_attn_tensor *q, const urf_attn_tensor *k, const urf_attn_tensor *v,
+                                const int *d_q_lens, const int *d_k_lens, const urf_attn_tensor *o, float *d_lse, void *d_work,
+                                size_t work_bytes, void *stream) {
+  const char *who = "urf_attn_forward";
+  if (check_config(cfg, who) || check_tensor(q, cfg, who, "q") || check_tensor(k, cfg, who, "k") || check_tensor(v, cfg, who, "v") ||
+      check_out(o, cfg, cfg->q_len, cfg->q_heads, who, "o")) return -2;
+  URF_CHECK(d_lse, "%s: lse is null", who);
+  URF_CHECK(o->data != q->data && o->data != k->data && o->data != v->data, "%s: o may not be an input", who);
+  const size_t need = forward_bytes(*cfg);
+  URF_CHECK(need == 0 || (d_work && work_bytes >= need && ((uintptr_t)d_work & 15) == 0), "%s: workspace of %zu bytes, %zu needed", who, work_bytes, need);
+  const Shape sh = forward_shape(*cfg);
+  AttnArgs a = args_of(cfg, q, k, v, d_q_lens, d_k_lens);
+  a.o = view(o);
+  a.lse = d_lse;
+  a.splits = sh.splits;
+  if (sh.splits > 1) {
+    const size_t rows = ((size_t)a.Lq * a.G + 31) / 32 * 32 * a.B * a.Hk * sh.splits;
+    a.part_o = (float *)d_work;
+    a.part_ml = a.part_o + rows * (a.D <= 64 ? 64 : 128);
+  }
+  OnDevice on(cfg->device);
+  URF_HIP(on.rc);
+  const hipStream_t st = (hipStream_t)stream;
+  URF_HIP(cfg->dtype == URF_F32 ? attn_forward_f32(a, sh.narrow, st) : cfg->dtype == URF_F16 ? attn_forward_f16(a, sh.narrow, st) : attn_forward_bf16(a, sh.narrow, st));
+  return 0;
+}
+
+extern "C" int urf_attn_backward(const urf_attn_config *cfg, const urf_attn_tensor *q, const urf_attn_tensor *k, const urf_attn_tensor *v,
+                                 const urf_attn_tensor *o, const float *d_lse, const urf_attn_tensor *d_o, const int *d_q_lens,
+                                 const int *d_k_lens, const urf_attn_tensor *dq, const urf_attn_tensor *dk, const urf_attn_tensor *dv,
+                                 void *d_work, size_t work_bytes, void *stream) {
+  const char *who = "urf_attn_backward";
+  if (check_config(cfg, who) || check_tensor(q, cfg, who, "q") || check_tensor(k, cfg, who, "k") || check_tensor(v, cfg, who, "v") ||
+      check_tensor(o, cfg, who, "o") || check_tensor(d_o, cfg, who, "the gradient of o") || check_out(dq, cfg, cfg->q_len, cfg->q_heads, who, "dq") ||
+      check_out(dk, cfg, cfg->k_len, cfg->kv_heads, who, "dk") || check_out(dv, cfg, cfg->k_len, cfg->kv_heads, who, "dv")) return -2;
+  URF_CHECK(d_lse, "%s: lse is null", who);
+  const void *in[5] = {q->data, k->data, v->data, o->data, d_o->data}, *out[3] = {dq->data, dk->data, dv->data};
+  for (int x = 0; x < 3; ++x) {
+    for (int y = 0; y < 5; ++y) URF_CHECK(out[x] != in[y], "%s: an output may not be an input", who);
+    for (int y = 0; y < x; ++y) URF_CHECK(out[x] != out[y], "%s: two outputs share a base", who);
+  }
+  const size_t need = backward_bytes(*cfg);
+  URF_CHECK(d_work && work_bytes >= need && ((uintptr_t)d_work & 15) == 0, "%s: workspace of %zu bytes, %zu needed", who, work_bytes, need);
+  AttnArgs a = args_of(cfg, q, k, v, d_q_lens, d_k_lens);
+  a.o = view(o); a.dout = view(d_o); a.dq = view(dq); a.dk = view(dk); a.dv = view(dv);
+  a.lse = (float *)d_lse;
+  a.delta = (float *)d_work;
+  OnDevice on(cfg->device);
+  URF_HIP(on.rc);
+  const hipStream_t st = (hipStream_t)stream;
+  URF_HIP(cfg->dtype == URF_F32 ? attn_backward_f32(a, st) : cfg->dtype == URF_F16 ? attn_backward_f16(a, st) : attn_backward_bf16(a, st));
+  return 0;
+}
