@@ -625,6 +625,40 @@ int urf_attn_backward(const urf_attn_config *cfg, const urf_attn_tensor *q, cons
                       const int *d_k_lens, const urf_attn_tensor *dq, const urf_attn_tensor *dk, const urf_attn_tensor *dv,
                       void *d_work, size_t work_bytes, void *stream);
 
+#define URF_TOP_MAX 64        /* targets, alternatives or listed entries per row */
+typedef struct {
+  int dtype;                  /* URF_F32, URF_F16, URF_BF16: of the scores and their gradient; everything else is f32 */
+  int rows, classes;          /* rows may be 0 */
+  long long row_stride;       /* elements between rows of the scores (any, also 0 or less than `classes`: they are only read) */
+  float scale;                /* the scores are multiplied by it first: 1 / temperature; positive */
+  int device;
+} urf_rows_config;
+/* z = scale * logits of a row.  lse[row] = log sum exp z; entropy[row] of softmax(z), in nats; log_prob[row][n] = z[targets[row][n]]
+ * - lse, 0 for a target outside [0, classes) (-1: none); top_index / top_log_prob[row][top]: the `top` largest scores, descending,
+ * equal ones by index.  Scores may be -infinity (log probability -infinity); a row of nothing else has lse -infinity and entropy 0.
+ * A row with a NaN or +infinity has NaN everywhere and -1 as its alternatives.  d_targets may be NULL with n_targets = 0. */
+int urf_log_probs(const urf_rows_config *cfg, const void *logits, const int *d_targets, int n_targets, int top, float *d_log_prob,
+                  float *d_entropy, float *d_lse, int *d_top_index, float *d_top_log_prob, void *stream);
+/* d_logits (rows of d_logits_stride elements) = the gradient of sum(log_prob * d_log_prob) + sum(entropy * d_entropy), from the
+ * forward call's lse and entropy; d_entropy may be NULL.  A candidate that is a target twice gets both.  Rows without a score above
+ * -infinity get 0. */
+int urf_log_probs_backward(const urf_rows_config *cfg, const void *logits, const int *d_targets, int n_targets, const float *d_lse,
+                           const float *d_entropy, const float *d_d_log_prob, const float *d_d_entropy, void *d_logits,
+                           long long d_logits_stride, void *stream);
+/* Distillation from a teacher's top alternatives, cfg->scale = 1 / temperature: index[row][listed] (int; outside [0, classes), e.g.
+ * -1: unused, its value is not looked at) and value[row][listed].  q = softmax(scale * logits) is the student.
+ *   tail = 0: value holds logits (or log probabilities) of the teacher, p = softmax(scale * value) over the listed entries;
+ *             loss = sum p (log p - log q)
+ *   tail = 1: value holds log probabilities at this temperature (urf_log_probs with this scale and `top`), p = exp(value), and
+ *             what they leave (from 2^-20 on) is one more outcome, whose student probability is that of everything unlisted.
+ * loss[row], lse[row] = log sum exp(scale * logits), log_tail[row] = log of the student's unlisted probability (tail = 1). */
+int urf_distill(const urf_rows_config *cfg, const void *logits, const int *d_index, const float *d_value, int listed, int tail,
+                float *d_loss, float *d_lse, float *d_log_tail, void *stream);
+/* d_logits = the gradient of sum(loss * d_loss) with respect to the student's logits, from the forward call's lse and log_tail */
+int urf_distill_backward(const urf_rows_config *cfg, const void *logits, const int *d_index, const float *d_value, int listed, int tail,
+                         const float *d_lse, const float *d_log_tail, const float *d_d_loss, void *d_logits,
+                         long long d_logits_stride, void *stream);
+
 /* arithmetic taps of the GPU parity tests: pure functions of their arguments (the fp32 matrix core as an ordered fma chain, the
  * canonical exp / log, IEEE division and square root, the split-f16 GEMM, one f16 matrix-core instruction).  They touch no handle. */
 int urf_probe_fma_gemm(const float *A, const float *B, const float *bias, int M, int N, int K, float *C, int device);

@@ -1,0 +1,640 @@
+// logits_ops.hip -- operators over rows of scores (logits, log-assignments) on caller-owned tensors: log probabilities of given
+// candidates with entropy and top alternatives, distillation from a teacher's top alternatives, and their gradients.
+//
+// With c = scale log2(e), x_v = c z_v and m = max x:  S = sum 2^(x_v - m),  lse = (m + log2 S) ln 2,  and the entropy is
+// (log2 S - A / S) ln 2 with A = sum 2^(x_v - m) (x_v - m): one pass over the row, every lane with a running maximum of its own
+// that rescales its sums when it grows.  The gradients need lse only and are one more pass: read a score, write its gradient.
+// All of it is bound by memory: a score is read once per pass, 16 bytes a lane and load, four loads in flight per lane.
+//
+// A row belongs to W waves (1, 4 or 16, one workgroup): 1 where the rows are short, 16 where there are too few rows to fill the
+// chip with 4.  Sums are joined in a fixed order.  Rows may start at any element: the loads are declared with the elements' own
+// alignment (this hardware takes a 16-byte access at any address).
+//
+// "Listed" candidates (targets, a teacher's alternatives): at most 64 a row, one per lane of every wave.  A wave asks by ballot
+// whether any lies among the elements it is about to handle, which is rare in a long row, and only then looks whose they are.
+// Their gradients are added to the element's own before its one rounding, in the list's order, so that a candidate listed twice
+// gets both; there are no atomics and no second write.
+#include "operator_common.h"
+
+#include <math.h>
+
+namespace urf {
+
+static_assert(URF_TOP_MAX == 64, "one listed candidate per lane");
+constexpr int kUnroll = 4;               // 16-byte loads in flight per lane
+constexpr float kFloor = -1.0e4f;        // 2^kFloor is 0: a masked score (-inf) adds 0 * kFloor to A, not 0 * inf
+
+struct RowsArgs {
+  const void *z;                 // [R] rows of V scores
+  long long stride;              // elements between rows
+  int R, V;
+  float c;                       // scale * log2(e)
+  float scale;                   // 1 / temperature for the distillation
+  // log probabilities
+  const int *targets; int N;     // [R][N]
+  int K;                         // alternatives (log_probs), listed per row (distillation)
+  float *log_prob, *entropy, *lse, *top_log_prob;
+  int *top_index;
+  // distillation
+  const int *t_index; const float *t_value;      // [R][K]
+  float *loss, *log_tail;
+  // gradients
+  const float *g1, *g2;          // d_log_prob [R][N] (or d_loss [R]); d_entropy [R]
+  void *dz; long long dz_stride;
+  int per_row;                   // gradients: waves per row
+};
+
+// ------------------------------------------------------------------ rows
+template <typename T> struct Row {
+  static constexpr int kPer = 16 / (int)sizeof(T);
+  typedef T Vec __attribute__((ext_vector_type(kPer), aligned(sizeof(T))));
+  static __device__ __forceinline__ void load(const T *p, float (&f)[kPer]) {
+    const Vec v = *(const Vec *)p;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) f[e] = (float)v[e];
+  }
+};
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) v = fmaxf(v, __shfl_xor(v, x, 64));
+  return v;
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) v += __shfl_xor(v, x, 64);
+  return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) v += __shfl_xor(v, x, 64);
+  return v;
+}
+
+// running maximum (of x) and sums of a lane, a wave, a row
+struct Stat { float m, s, a; };
+__device__ __forceinline__ Stat join(Stat p, Stat q) {
+  const float m = fmaxf(p.m, q.m), mu = m == -INFINITY ? 0.0f : m;
+  const float fp = exp2f(p.m - mu), fq = exp2f(q.m - mu), dp = fmaxf(p.m - mu, kFloor), dq = fmaxf(q.m - mu, kFloor);
+  // x - m = (x - p.m) + (p.m - m)
+  return {m, p.s * fp + q.s * fq, fmaf(p.s, dp, p.a) * fp + fmaf(q.s, dq, q.a) * fq};
+}
+__device__ __forceinline__ Stat wave_join(Stat v) {
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) {
+    const Stat o = {__shfl_xor(v.m, x, 64), __shfl_xor(v.s, x, 64), __shfl_xor(v.a, x, 64)};
+    v = (threadIdx.x & x) ? join(o, v) : join(v, o);      // the same operand order on both sides: the same bits in every lane
+  }
+  return v;
+}
+
+// ------------------------------------------------------------------ top alternatives
+// A wave's 64 best so far, descending, one key per lane: the score as an ordered integer above, the complement of its index below
+// (equal scores: the lower index wins).  Every row has its list in registers; a key is 0 where the list is not full yet.
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 key_of(float z, int index) {
+  const unsigned u = __float_as_uint(z + 0.0f);           // -0 counts as 0
+  const unsigned o = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return ((u64)o << 32) | (unsigned)~index;
+}
+__device__ __forceinline__ float key_score(u64 k) {
+  const unsigned o = (unsigned)(k >> 32);
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+__device__ __forceinline__ u64 shfl64(u64 v, int src) {
+  return ((u64)(unsigned)__shfl((int)(v >> 32), src, 64) << 32) | (unsigned)__shfl((int)(unsigned)v, src, 64);
+}
+__device__ __forceinline__ u64 exchange(u64 v, int x, bool keep_max) {
+  const u64 o = ((u64)(unsigned)__shfl_xor((int)(v >> 32), x, 64) << 32) | (unsigned)__shfl_xor((int)(unsigned)v, x, 64);
+  return (v > o) == keep_max ? v : o;
+}
+__device__ __forceinline__ u64 sort_desc(u64 v, int lane) {
+  for (int n = 2; n <= 64; n <<= 1)
+    for (int x = n >> 1; x >= 1; x >>= 1) v = exchange(v, x, ((lane & n) == 0) == ((lane & x) == 0));
+  return v;
+}
+// both descending: the 64 largest of the two, descending
+__device__ __forceinline__ u64 merge_desc(u64 a, u64 b, int lane) {
+  const u64 r = shfl64(b, 63 - lane);
+  u64 v = a > r ? a : r;
+  for (int x = 32; x >= 1; x >>= 1) v = exchange(v, x, (lane & x) == 0);
+  return v;
+}
+// takes in one candidate per lane (0 = none): a few are inserted one by one, many are sorted and merged, so that no input costs
+// more than one sort per 64 scores
+__device__ __forceinline__ void take(u64 &list, u64 &last, u64 cand, int K, int lane) {
+  u64 pass = __ballot(cand > last);
+  if (__popcll(pass) > 6) {
+    list = merge_desc(list, sort_desc(cand, lane), lane);
+  } else {
+    while (pass) {
+      const u64 c = shfl64(cand, (int)__ffsll((long long)pass) - 1);
+      pass &= pass - 1;
+      const int at = __popcll(__ballot(list > c));
+      const u64 up = shfl64(list, lane > 0 ? lane - 1 : 0);
+      list = lane < at ? list : lane == at ? c : up;
+    }
+  }
+  last = shfl64(list, K - 1);
+}
+
+// ------------------------------------------------------------------ listed candidates
+// `mine` = this lane's listed index or -1, `hits` = the lanes whose index lies in the range at hand, f = elements first + 0 .. n - 1
+template <int n> __device__ __forceinline__ void hide_listed(float *f, int first, int mine, u64 hits) {
+  while (hits) {
+    const int src = (int)__ffsll((long long)hits) - 1;
+    hits &= hits - 1;
+    const int at = __shfl(mine, src, 64) - first;
+#pragma unroll
+    for (int e = 0; e < n; ++e)
+      if (e == at) f[e] = -INFINITY;
+  }
+}
+
+// One pass of a wave over its share of a row.  TOP: keeps the alternatives; TAIL: leaves the listed candidates out, so that a
+// tail far below them keeps its own maximum.
+template <typename T, bool ENTROPY, bool TOP, bool TAIL>
+__device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, int parts, int lane, int mine, int K, u64 &list) {
+  typedef Row<T> RW;
+  constexpr int kPer = RW::kPer, kStep = 64 * kPer;
+  Stat st = {-INFINITY, 0.0f, 0.0f};
+  u64 last = 0;
+  auto absorb = [&](const float *f, int n) {
+    float top = f[0];
+#pragma unroll
+    for (int e = 1; e < n; ++e) top = fmaxf(top, f[e]);
+    const float m = fmaxf(st.m, top * c), mu = m == -INFINITY ? 0.0f : m;
+    const float f0 = __builtin_amdgcn_exp2f(st.m - mu);
+    if (ENTROPY) st.a = fmaf(st.s, fmaxf(st.m - mu, kFloor), st.a) * f0;
+    st.s *= f0;
+    st.m = m;
+#pragma unroll
+    for (int e = 0; e < n; ++e) {
+      const float x = fmaf(f[e], c, -mu), p = __builtin_amdgcn_exp2f(x);
+      st.s += p;
+      if (ENTROPY) st.a = fmaf(p, fmaxf(x, kFloor), st.a);
+    }
+    return top;
+  };
+  const int steps = (V / kPer + 63) / 64;                        // of 64 whole vectors; what is left is done by part 0
+  const int b0 = (int)((long long)steps * part / parts), b1 = (int)((long long)steps * (part + 1) / parts);
+  for (int b = b0; b < b1; b += kUnroll) {
+    float f[kUnroll][kPer];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int first = (b + u) * kStep + lane * kPer;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) f[u][e] = -INFINITY;
+      if (b + u < b1 && first + kPer <= V) RW::load(z + first, f[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (b + u < b1) {
+        const int base = (b + u) * kStep, first = base + lane * kPer;
+        if (TAIL) {
+          const u64 hits = __ballot(mine >= base && mine < base + kStep);
+          if (hits) hide_listed<kPer>(f[u], first, mine, hits);
+        }
+        const float top = absorb(f[u], kPer);
+        if (TOP) {
+          const float least = key_score(last);                   // NaN while the list is not full: everything passes
+          if (__any(!(top < least))) {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+              if (__any(!(f[u][e] < key_score(last)))) take(list, last, first + kPer <= V ? key_of(f[u][e], first + e) : 0, K, lane);
+          }
+        }
+      }
+  }
+  if (part == 0 && V % kPer) {
+    const int v = V - V % kPer + lane;
+    float f[1] = {-INFINITY};
+    if (v < V) f[0] = (float)z[v];
+    if (TAIL) {
+      const u64 hits = __ballot(mine >= V - V % kPer);
+      if (hits) hide_listed<1>(f, v, mine, hits);
+    }
+    absorb(f, 1);
+    if (TOP) take(list, last, v < V ? key_of(f[0], v) : 0, K, lane);
+  }
+  return st;
+}
+
+// joins the parts of a row: wave 0 of the row returns with the row's sums and list
+template <int W, bool TOP>
+__device__ __forceinline__ Stat row_join(Stat st, u64 &list, int wave, int lane, char *lds) {
+  st = wave_join(st);
+  if constexpr (W > 1) {
+    Stat *ss = (Stat *)lds;
+    u64 *ls = (u64 *)(lds + 16 * W);
+    if (lane == 0) ss[wave] = st;
+    if (TOP) ls[wave * 64 + lane] = list;
+    lds_barrier();
+    if (TOP) {
+      for (int n = W / 2; n >= 1; n >>= 1) {
+        if (wave < n) {
+          list = merge_desc(list, ls[(wave + n) * 64 + lane], lane);
+          ls[wave * 64 + lane] = list;
+        }
+        lds_barrier();
+      }
+    }
+    if (wave == 0) {
+      st = ss[0];
+#pragma unroll
+      for (int w = 1; w < W; ++w) st = join(st, ss[w]);
+    }
+  }
+  return st;
+}
+
+// ------------------------------------------------------------------ forward kernels
+template <typename T, int W, bool TOP>
+__global__ void __launch_bounds__(W == 16 ? 1024 : 256) log_probs_kernel(RowsArgs a) {
+  __shared__ __align__(16) char lds[W > 1 ? 16 * W + (TOP ? 512 * W : 0) : 16];
+  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6;
+  const int r = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (r >= a.R) return;
+  const T *z = (const T *)a.z + (long long)r * a.stride;
+  u64 list = 0;
+  Stat st = row_pass<T, true, TOP, false>(z, a.V, a.c, wave, W, lane, -1, a.K, list);
+  st = row_join<W, TOP>(st, list, wave, lane, lds);
+  if (wave) return;
+  // a NaN or +inf score leaves no distribution: everything is NaN and the alternatives are -1.  A row without any score above
+  // -inf: lse -inf, entropy 0, every log probability -inf.
+  const bool broken = !(st.s >= 0.0f) || st.m == INFINITY, empty = st.m == -INFINITY && !broken;
+  const float ls = log2f(st.s), nan = __uint_as_float(0x7fc00000u);
+  if (lane == 0) {
+    a.lse[r] = broken ? nan : empty ? -INFINITY : (st.m + ls) * kLn2;
+    a.entropy[r] = broken ? nan : empty ? 0.0f : (ls - st.a / st.s) * kLn2;
+  }
+  auto log_prob = [&](float x) { return broken ? nan : empty || x == -INFINITY ? -INFINITY : (fmaf(x, a.c, -st.m) - ls) * kLn2; };
+  if (lane < a.N) {
+    const int t = a.targets[(long long)r * a.N + lane];
+    a.log_prob[(long long)r * a.N + lane] = t >= 0 && t < a.V ? log_prob((float)z[t]) : 0.0f;
+  }
+  if (TOP && lane < a.K) {
+    a.top_index[(long long)r * a.K + lane] = broken ? -1 : (int)~(unsigned)list;
+    a.top_log_prob[(long long)r * a.K + lane] = log_prob(key_score(list));
+  }
+}
+
+// the teacher's side of a row: lane k holds alternative k (index -1 where there is none), its probability and log probability
+struct Teacher { int index; float p, lp; float mass, rest; };
+template <bool TAIL>
+__device__ __forceinline__ Teacher teacher_of(const RowsArgs &a, int r, int lane) {
+  Teacher t = {-1, 0.0f, 0.0f, 0.0f, 0.0f};
+  float v = -INFINITY;
+  if (lane < a.K) {
+    t.index = a.t_index[(long long)r * a.K + lane];
+    if (t.index < 0 || t.index >= a.V) t.index = -1;
+    else v = a.t_value[(long long)r * a.K + lane];
+  }
+  if (TAIL) {
+    t.lp = v;
+    const double p = exp((double)v), sum = wave_sum(p);   // 1 - sum cancels: in 64 bits
+    t.p = (float)p;
+    const float rest = (float)fmax(1.0 - sum, 0.0);
+    t.rest = rest < 0x1p-20f ? 0.0f : rest;               // below the rounding of the listed probabilities: there is no rest
+    t.mass = (float)sum + t.rest;
+  } else {
+    v *= a.scale;
+    const float m = wave_max(v), e = m == -INFINITY ? 0.0f : expf(v - m), sum = wave_sum(e);
+    t.p = sum == 0.0f ? 0.0f : e / sum;
+    t.lp = v - m - logf(sum);
+    t.mass = wave_sum(t.p);
+  }
+  return t;
+}
+
+template <typename T, int W, bool TAIL>
+__global__ void __launch_bounds__(W == 16 ? 1024 : 256) distill_kernel(RowsArgs a) {
+  __shared__ __align__(16) char lds[W > 1 ? 16 * W : 16];
+  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6;
+  const int r = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (r >= a.R) return;
+  const T *z = (const T *)a.z + (long long)r * a.stride;
+  const Teacher t = teacher_of<TAIL>(a, r, lane);
+  u64 none = 0;
+  Stat st = row_pass<T, false, false, TAIL>(z, a.V, a.c, wave, W, lane, t.index, 0, none);
+  st = row_join<W, false>(st, none, wave, lane, lds);
+  if (wave) return;
+  const bool used = t.index >= 0;
+  const float zk = used ? (float)z[t.index] : -INFINITY;
+  float m = st.m, sum = st.s;                             // of the whole row
+  if (TAIL) {
+    // the pass left the listed candidates out: add each of them once
+    bool first = used;
+    for (int k = 0; k < a.K; ++k) {
+      const int other = __shfl(t.index, k, 64);
+      if (k < lane && other == t.index) first = false;
+    }
+    m = fmaxf(m, wave_max(zk * a.c));
+    const float mu = m == -INFINITY ? 0.0f : m;
+    sum = st.s * exp2f(st.m - mu) + wave_sum(first ? exp2f(fmaf(zk, a.c, -mu)) : 0.0f);
+  }
+  const float ls = log2f(sum), nan = __uint_as_float(0x7fc00000u);
+  const bool broken = !(sum >= 0.0f) || m == INFINITY, empty = m == -INFINITY && !broken;
+  const float lq = zk == -INFINITY ? -INFINITY : (fmaf(zk, a.c, -m) - ls) * kLn2;
+  float loss = wave_sum(t.p != 0.0f ? t.p * (t.lp - lq) : 0.0f), tail = 0.0f;
+  if (TAIL) {
+    tail = (st.m + log2f(st.s) - m - ls) * kLn2;          // log of the student's probability of everything unlisted
+    if (t.rest > 0.0f) loss += t.rest * (logf(t.rest) - tail);
+  }
+  if (empty) loss = t.mass != 0.0f ? INFINITY : 0.0f;     // the student allows nothing
+  if (lane == 0) {
+    a.loss[r] = broken ? nan : loss;
+    a.lse[r] = broken ? nan : empty ? -INFINITY : (m + ls) * kLn2;
+    if (TAIL) a.log_tail[r] = broken ? nan : empty ? -INFINITY : tail;
+  }
+}
+
+// ------------------------------------------------------------------ gradients
+// dz = coefficient * 2^(x - shift) [ * (1 + ...) ] + what the listed candidates add; one read, one write per score
+struct GradRow {
+  float shift;       // log2 units: of lse (or of lse and the tail's probability)
+  float coef;        // of the probability
+  float h, ent2;     // ENTROPY: -h p (log2 p + ent2), in log2 units
+  float lshift, lcoef;   // TAIL: of a listed candidate's probability
+  int mine;          // this lane's listed index (-1: none) and what it adds
+  float add;
+};
+
+template <typename T, bool ENTROPY, bool TAIL>
+__device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float c, const GradRow &g, int part, int parts, int lane) {
+  typedef Row<T> RW;
+  constexpr int kPer = RW::kPer, kStep = 64 * kPer;
+  auto grad = [&](float f) {
+    const float x = fmaf(f, c, -g.shift), p = __builtin_amdgcn_exp2f(x);
+    if (ENTROPY) return p * fmaf(-g.h, fmaxf(x, kFloor) + g.ent2, g.coef);
+    return p * g.coef;
+  };
+  // elements first + 0 .. n - 1 of the lane, some of the wave's are listed
+  auto listed = [&](const float *f, float *d, int n, int first, u64 hits) {
+    if (TAIL)                                              // their own terms, not the tail's
+      for (u64 h = hits; h; h &= h - 1) {
+        const int at = __shfl(g.mine, (int)__ffsll((long long)h) - 1, 64) - first;
+#pragma unroll
+        for (int e = 0; e < n; ++e)
+          if (e == at) d[e] = g.lcoef * __builtin_amdgcn_exp2f(fmaf(f[e], c, -g.lshift));
+      }
+    for (u64 h = hits; h; h &= h - 1) {                    // what each mention adds, in the list's order
+      const int src = (int)__ffsll((long long)h) - 1, at = __shfl(g.mine, src, 64) - first;
+      const float add = __shfl(g.add, src, 64);
+#pragma unroll
+      for (int e = 0; e < n; ++e)
+        if (e == at) d[e] += add;
+    }
+  };
+  const int steps = (V / kPer + 63) / 64;
+  const int b0 = (int)((long long)steps * part / parts), b1 = (int)((long long)steps * (part + 1) / parts);
+  for (int b = b0; b < b1; b += kUnroll) {
+    float f[kUnroll][kPer];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int first = (b + u) * kStep + lane * kPer;
+      if (b + u < b1 && first + kPer <= V) RW::load(z + first, f[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (b + u < b1) {
+        const int base = (b + u) * kStep, first = base + lane * kPer;
+        float d[kPer];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) d[e] = grad(f[u][e]);
+        const u64 hits = __ballot(g.mine >= base && g.mine < base + kStep);
+        if (hits) listed(f[u], d, kPer, first, hits);
+        if (first + kPer <= V) {
+          typename RW::Vec o;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) o[e] = (T)d[e];
+          *(typename RW::Vec *)(dz + first) = o;
+        }
+      }
+  }
+  if (part == 0 && V % kPer) {
+    const int v = V - V % kPer + lane;
+    const float f[1] = {v < V ? (float)z[v] : -INFINITY};
+    float d[1] = {grad(f[0])};
+    const u64 hits = __ballot(g.mine >= V - V % kPer);
+    if (hits) listed(f, d, 1, v, hits);
+    if (v < V) dz[v] = (T)d[0];
+  }
+}
+
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(256) log_probs_backward_kernel(RowsArgs a) {
+  const int lane = threadIdx.x & 63;
+  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int r = (int)(w / a.per_row), part = (int)(w % a.per_row);
+  if (r >= a.R) return;
+  const float lse = a.lse[r];
+  const bool empty = lse == -INFINITY;                    // no score to choose from: constant outputs, no gradient
+  GradRow g = {};
+  g.mine = -1;
+  float own = 0.0f;
+  if (lane < a.N) {
+    g.mine = a.targets[(long long)r * a.N + lane];
+    if (g.mine < 0 || g.mine >= a.V || empty) g.mine = -1;
+    else own = a.g1[(long long)r * a.N + lane];
+  }
+  g.add = own * a.scale;
+  g.shift = empty ? 0.0f : lse * kLog2e;
+  g.coef = empty ? 0.0f : -wave_sum(own) * a.scale;
+  if (ENTROPY && !empty) {
+    g.h = a.g2[r] * a.scale * kLn2;
+    g.ent2 = a.entropy[r] * kLog2e;
+  }
+  grad_pass<T, ENTROPY, false>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.c, g, part, a.per_row, lane);
+}
+
+template <typename T, bool TAIL>
+__global__ void __launch_bounds__(256) distill_backward_kernel(RowsArgs a) {
+  const int lane = threadIdx.x & 63;
+  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int r = (int)(w / a.per_row), part = (int)(w % a.per_row);
+  if (r >= a.R) return;
+  const Teacher t = teacher_of<TAIL>(a, r, lane);
+  const float lse = a.lse[r], gs = a.g1[r] * a.scale;
+  const bool empty = lse == -INFINITY;
+  GradRow g = {};
+  g.mine = empty ? -1 : t.index;
+  g.add = -gs * t.p;
+  g.shift = empty ? 0.0f : lse * kLog2e;
+  g.coef = empty ? 0.0f : gs * t.mass;
+  if (TAIL) {
+    g.lshift = g.shift;
+    g.lcoef = g.coef;
+    // unlisted v: mass q_v - rest q_v / q_tail = (mass q_tail - rest) 2^(x - shift) with the tail's probability in the shift,
+    // a probability within the tail: nothing overflows however small q_tail is
+    const float tail = a.log_tail[r];
+    if (!empty && tail != -INFINITY) {
+      g.shift += tail * kLog2e;
+      g.coef = gs * (t.mass * expf(tail) - t.rest);
+    }
+  }
+  grad_pass<T, false, TAIL>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.c, g, part, a.per_row, lane);
+}
+
+// ------------------------------------------------------------------ launches
+// waves per row: one for short rows; sixteen where four per row would leave the 256 CUs with less than two workgroups each
+inline int row_waves(int R, int V) { return V <= 2048 ? 1 : R <= 512 && V > 8192 ? 16 : 4; }
+// gradients: a wave takes about 16 KiB of scores, less where that leaves waves to spare
+inline int grad_waves(int R, int V, int bytes) {
+  const long long by_size = ((long long)V * bytes + 16383) / 16384, steps = (long long)V * bytes / 1024;
+  const long long fill = (4096 + R - 1) / R, n = by_size > fill ? by_size : fill;
+  return (int)(n < 1 || steps < 1 ? 1 : n > steps ? steps : n);
+}
+
+template <typename T> hipError_t launch_log_probs(const RowsArgs &a, hipStream_t st) {
+  const int W = row_waves(a.R, a.V);
+  const dim3 grid(W == 1 ? (a.R + 3) / 4 : a.R), block(W == 16 ? 1024 : 256);
+  auto kernel = W == 1 ? (a.K ? log_probs_kernel<T, 1, true> : log_probs_kernel<T, 1, false>)
+              : W == 4 ? (a.K ? log_probs_kernel<T, 4, true> : log_probs_kernel<T, 4, false>)
+                       : (a.K ? log_probs_kernel<T, 16, true> : log_probs_kernel<T, 16, false>);
+  hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
+  return hipGetLastError();
+}
+template <typename T> hipError_t launch_distill(const RowsArgs &a, bool tail, hipStream_t st) {
+  const int W = row_waves(a.R, a.V);
+  const dim3 grid(W == 1 ? (a.R + 3) / 4 : a.R), block(W == 16 ? 1024 : 256);
+  auto kernel = W == 1 ? (tail ? distill_kernel<T, 1, true> : distill_kernel<T, 1, false>)
+              : W == 4 ? (tail ? distill_kernel<T, 4, true> : distill_kernel<T, 4, false>)
+                       : (tail ? distill_kernel<T, 16, true> : distill_kernel<T, 16, false>);
+  hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
+  return hipGetLastError();
+}
+template <typename T> hipError_t launch_log_probs_backward(RowsArgs a, hipStream_t st) {
+  a.per_row = grad_waves(a.R, a.V, sizeof(T));
+  const dim3 grid((unsigned)(((long long)a.R * a.per_row + 3) / 4));
+  auto kernel = a.g2 ? log_probs_backward_kernel<T, true> : log_probs_backward_kernel<T, false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+template <typename T> hipError_t launch_distill_backward(RowsArgs a, bool tail, hipStream_t st) {
+  a.per_row = grad_waves(a.R, a.V, sizeof(T));
+  const dim3 grid((unsigned)(((long long)a.R * a.per_row + 3) / 4));
+  auto kernel = tail ? distill_backward_kernel<T, true> : distill_backward_kernel<T, false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+}  // namespace urf
+using namespace urf;
+
+namespace {
+
+#define URF_BY_TYPE(dtype, f, ...) \
+  ((dtype) == URF_F32 ? f<float>(__VA_ARGS__) : (dtype) == URF_F16 ? f<_Float16>(__VA_ARGS__) : f<__bf16>(__VA_ARGS__))
+
+int check_rows(const urf_rows_config *c, const void *logits, const char *who) {
+  URF_CHECK(c, "%s: null configuration", who);
+  URF_CHECK(dtype_bytes(c->dtype), "%s: element type %d (URF_F32, URF_F16 or URF_BF16)", who, c->dtype);
+  URF_CHECK(c->rows >= 0 && c->classes >= 1 && c->classes <= (1 << 30), "%s: %d rows of %d classes", who, c->rows, c->classes);
+  URF_CHECK(isfinite(c->scale) && c->scale > 0.0f, "%s: scale %g (positive)", who, (double)c->scale);
+  URF_CHECK(c->rows == 0 || logits, "%s: logits is null", who);
+  URF_CHECK(((uintptr_t)logits & (dtype_bytes(c->dtype) - 1)) == 0, "%s: logits is not aligned to its elements", who);
+  return 0;
+}
+
+// the gradient's rows may not touch each other or the logits
+int check_grad(const urf_rows_config *c, const void *logits, const void *d, long long stride, const char *who) {
+  URF_CHECK(c->rows == 0 || d, "%s: d_logits is null", who);
+  const long long b = dtype_bytes(c->dtype);
+  URF_CHECK(((uintptr_t)d & (b - 1)) == 0, "%s: d_logits is not aligned to its elements", who);
+  URF_CHECK(c->rows <= 1 || stride >= c->classes, "%s: the rows of d_logits overlap (stride %lld, %d classes)", who, stride, c->classes);
+  if (c->rows == 0) return 0;
+  const long long in = c->row_stride * (c->rows - 1), n = c->classes;
+  const char *z = (const char *)logits, *z0 = z + (in < 0 ? in : 0) * b, *z1 = z + ((in > 0 ? in : 0) + n) * b;
+  const char *d0 = (const char *)d, *d1 = d0 + (stride * (c->rows - 1) + n) * b;
+  URF_CHECK(d1 <= z0 || z1 <= d0, "%s: d_logits overlaps the logits", who);
+  return 0;
+}
+
+RowsArgs rows_of(const urf_rows_config *c, const void *logits) {
+  RowsArgs a = {};
+  a.z = logits;
+  a.stride = c->row_stride;
+  a.R = c->rows;
+  a.V = c->classes;
+  a.scale = c->scale;
+  a.c = (float)((double)c->scale * 1.4426950408889634);
+  return a;
+}
+
+}  // namespace
+
+extern "C" int urf_log_probs(const urf_rows_config *cfg, const void *logits, const int *d_targets, int n_targets, int top,
+                             float *d_log_prob, float *d_entropy, float *d_lse, int *d_top_index, float *d_top_log_prob, void *stream) {
+  const char *who = "urf_log_probs";
+  if (check_rows(cfg, logits, who)) return -2;
+  URF_CHECK(n_targets >= 0 && n_targets <= URF_TOP_MAX, "%s: %d targets per row (0 .. %d)", who, n_targets, URF_TOP_MAX);
+  URF_CHECK(top >= 0 && top <= URF_TOP_MAX && top <= cfg->classes, "%s: %d alternatives (0 .. %d, at most the %d classes)", who, top, URF_TOP_MAX, cfg->classes);
+  if (cfg->rows == 0) return 0;
+  URF_CHECK(d_entropy && d_lse && (n_targets == 0 || (d_targets && d_log_prob)) && (top == 0 || (d_top_index && d_top_log_prob)), "%s: null pointer", who);
+  RowsArgs a = rows_of(cfg, logits);
+  a.targets = d_targets; a.N = n_targets; a.K = top;
+  a.log_prob = d_log_prob; a.entropy = d_entropy; a.lse = d_lse; a.top_index = d_top_index; a.top_log_prob = d_top_log_prob;
+  OnDevice on(cfg->device);
+  URF_HIP(on.rc);
+  URF_HIP(URF_BY_TYPE(cfg->dtype, launch_log_probs, a, (hipStream_t)stream));
+  return 0;
+}
+
+extern "C" int urf_log_probs_backward(const urf_rows_config *cfg, const void *logits, const int *d_targets, int n_targets,
+                                      const float *d_lse, const float *d_entropy, const float *d_d_log_prob,
+                                      const float *d_d_entropy, void *d_logits, long long d_logits_stride, void *stream) {
+  const char *who = "urf_log_probs_backward";
+  if (check_rows(cfg, logits, who) || check_grad(cfg, logits, d_logits, d_logits_stride, who)) return -2;
+  URF_CHECK(n_targets >= 0 && n_targets <= URF_TOP_MAX, "%s: %d targets per row (0 .. %d)", who, n_targets, URF_TOP_MAX);
+  if (cfg->rows == 0) return 0;
+  URF_CHECK(d_lse && (n_targets == 0 || (d_targets && d_d_log_prob)) && (!d_d_entropy || d_entropy), "%s: null pointer", who);
+  RowsArgs a = rows_of(cfg, logits);
+  a.targets = d_targets; a.N = n_targets;
+  a.lse = (float *)d_lse; a.entropy = (float *)d_entropy; a.g1 = d_d_log_prob; a.g2 = d_d_entropy;
+  a.dz = d_logits; a.dz_stride = d_logits_stride;
+  OnDevice on(cfg->device);
+  URF_HIP(on.rc);
+  URF_HIP(URF_BY_TYPE(cfg->dtype, launch_log_probs_backward, a, (hipStream_t)stream));
+  return 0;
+}
+
+static int distill_args(const urf_rows_config *cfg, const void *logits, const int *d_index, const float *d_value, int listed, int tail,
+                        const char *who, RowsArgs *a) {
+  if (check_rows(cfg, logits, who)) return -2;
+  URF_CHECK(listed >= 1 && listed <= URF_TOP_MAX, "%s: %d listed alternatives (1 .. %d)", who, listed, URF_TOP_MAX);
+  URF_CHECK(cfg->rows == 0 || (d_index && d_value), "%s: the teacher's alternatives are null", who);
+  *a = rows_of(cfg, logits);
+  a->t_index = d_index; a->t_value = d_value; a->K = listed;
+  return 0;
+}
+
+extern "C" int urf_distill(const urf_rows_config *cfg, const void *logits, const int *d_index, const float *d_value, int listed,
+                           int tail, float *d_loss, float *d_lse, float *d_log_tail, void *stream) {
+  const char *who = "urf_distill";
+  RowsArgs a;
+  if (distill_args(cfg, logits, d_index, d_value, listed, tail, who, &a)) return -2;
+  if (cfg->rows == 0) return 0;
+  URF_CHECK(d_loss && d_lse && (!tail || d_log_tail), "%s: null pointer", who);
+  a.loss = d_loss; a.lse = d_lse; a.log_tail = d_log_tail;
+  OnDevice on(cfg->device);
+  URF_HIP(on.rc);
+  URF_HIP(URF_BY_TYPE(cfg->dtype, launch_distill, a, tail != 0, (hipStream_t)stream));
+  return 0;
+}
+
+extern "C" int urf_distill_backward(const urf_rows_config *cfg, const void *logits, const int *d_index, const float *d_value, int listed,
+                                    int tail, const float *d_lse, const float *d_log_tail, const float *d_d_loss, void *d_logits,
+                                    long long d_logits_stride, void *stream) {
+  const char *who = "urf_distill_backward";
+  RowsArgs a;
+  if (distill_args(cfg, logits, d_index, d_value, listed, tail, who, &a) || check_grad(cfg, logits, d_logits, d_logits_stride, who)) return -2;
+  if (cfg->rows == 0) return 0;
+  URF_CHECK(d_lse && d_d_loss && (!tail || d_log_tail), "%s: null pointer", who);
+  a.lse = (float *)d_lse; a.log_tail = (float *)d_log_tail; a.g1 = d_d_loss;
+  a.dz = d_logits; a.dz_stride = d_logits_stride;
+  OnDevice on(cfg->device);
+  URF_HIP(on.rc);
+  URF_HIP(URF_BY_TYPE(cfg->dtype, launch_distill_backward, a, tail != 0, (hipStream_t)stream));
+  return 0;
+}

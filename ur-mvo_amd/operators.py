@@ -5,14 +5,18 @@ included, from torch's allocator: calls on several streams share nothing, and a 
 backward are separate calls, as in the C ABI; nothing here records for autograd (inputs that require a gradient are refused while
 it is enabled, rather than silently cut from the graph).
 """
+import collections
 import ctypes as C
 import math
 
 import torch
 
 from . import _lib
-from ._lib import AttnConfig, AttnTensor, check
+from ._lib import AttnConfig, AttnTensor, RowsConfig, check
 
+TOP_MAX = 64                                                          # URF_TOP_MAX
+LogProbs = collections.namedtuple("LogProbs", "log_prob entropy lse top_index top_log_prob")
+Distill = collections.namedtuple("Distill", "loss lse log_tail")
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # URF_F32, URF_F16, URF_BF16
 
 
@@ -118,3 +122,109 @@ def attention_backward(do, q, k, v, o, lse, *, causal=False, scale=None, q_lens=
                                        _p(lse), C.byref(_view(do)), _p(q_lens), _p(k_lens), C.byref(_view(dq)), C.byref(_view(dk)),
                                        C.byref(_view(dv)), _p(work), n, _stream(device)), "urf_attn_backward")
     return dq, dk, dv
+
+
+def _rows_config(who, logits, scale):
+    _require(logits.dim() == 2, f"{who}: logits has to be [rows, classes]")
+    _require(logits.shape[1] >= 1 and (logits.stride(1) == 1 or logits.shape[1] == 1), f"{who}: the rows of logits have to be contiguous")
+    _require(math.isfinite(scale) and scale > 0, f"{who}: scale {scale} (positive)")
+    return RowsConfig(DTYPES[logits.dtype], logits.shape[0], logits.shape[1], logits.stride(0), scale, logits.device.index)
+
+
+def _targets(who, targets, logits):
+    if targets is None:
+        return 0
+    _require(isinstance(targets, torch.Tensor) and targets.dim() in (1, 2), f"{who}: targets has to be [rows] or [rows, n]")
+    _ints(who, "targets", targets, (logits.shape[0],) + tuple(targets.shape[1:]), logits.device)
+    n = targets.shape[1] if targets.dim() == 2 else 1
+    _require(n <= TOP_MAX, f"{who}: {n} targets per row (at most {TOP_MAX})")
+    return n
+
+
+def _f32(who, name, t, shape, device):
+    _require(isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.device == device and tuple(t.shape) == tuple(shape)
+             and t.is_contiguous(), f"{who}: {name} has to be a contiguous float32 tensor {tuple(shape)} on {device}")
+    return t
+
+
+def log_probs(logits, targets=None, *, top=0, scale=1.0):
+    """LogProbs(log_prob, entropy, lse, top_index, top_log_prob) of softmax(scale * logits) per row of [rows, classes].  targets: int32
+    [rows] or [rows, n] (n <= 64; -1 = none, log probability 0); `top` <= 64 alternatives, descending, equal scores by index.  What was
+    not asked for is None."""
+    who = "log_probs"
+    device = _floats(who, logits=logits)
+    cfg = _rows_config(who, logits, scale)
+    n = _targets(who, targets, logits)
+    _require(0 <= top <= min(TOP_MAX, cfg.classes), f"{who}: top {top} (0 .. {TOP_MAX}, at most {cfg.classes} classes)")
+    entropy, lse = (torch.empty(cfg.rows, dtype=torch.float32, device=device) for _ in range(2))
+    log_prob = None if targets is None else torch.empty(targets.shape, dtype=torch.float32, device=device)
+    top_index = torch.empty((cfg.rows, top), dtype=torch.int32, device=device) if top else None
+    top_log_prob = torch.empty((cfg.rows, top), dtype=torch.float32, device=device) if top else None
+    check(_lib.lib().urf_log_probs(C.byref(cfg), _p(logits), _p(targets), n, top, _p(log_prob), _p(entropy), _p(lse), _p(top_index),
+                                   _p(top_log_prob), _stream(device)), "urf_log_probs")
+    return LogProbs(log_prob, entropy, lse, top_index, top_log_prob)
+
+
+def log_probs_backward(logits, targets, lse, entropy, *, d_log_prob=None, d_entropy=None, scale=1.0):
+    """The gradient of sum(log_prob * d_log_prob) + sum(entropy * d_entropy) with respect to logits; lse and entropy are
+    log_probs()'s for the same logits, targets and scale."""
+    who = "log_probs_backward"
+    device = _floats(who, logits=logits)
+    cfg = _rows_config(who, logits, scale)
+    if d_log_prob is None:
+        targets = None
+    n = _targets(who, targets, logits)
+    _require((targets is None) == (d_log_prob is None), f"{who}: d_log_prob without targets")
+    if targets is not None:
+        _f32(who, "d_log_prob", d_log_prob, targets.shape, device)
+    _f32(who, "lse", lse, (cfg.rows,), device)
+    _f32(who, "entropy", entropy, (cfg.rows,), device)
+    if d_entropy is not None:
+        _f32(who, "d_entropy", d_entropy, (cfg.rows,), device)
+    d = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    check(_lib.lib().urf_log_probs_backward(C.byref(cfg), _p(logits), _p(targets), n, _p(lse), _p(entropy), _p(d_log_prob), _p(d_entropy),
+                                            _p(d), C.c_longlong(cfg.classes), _stream(device)), "urf_log_probs_backward")
+    return d
+
+
+def _teacher(who, logits, index, value):
+    _require(isinstance(index, torch.Tensor) and index.dim() == 2 and 1 <= index.shape[1] <= TOP_MAX,
+             f"{who}: the teacher's indices have to be [rows, 1 .. {TOP_MAX}]")
+    _ints(who, "teacher_index", index, (logits.shape[0], index.shape[1]), logits.device)
+    _f32(who, "teacher_value", value, index.shape, logits.device)
+    return index.shape[1]
+
+
+def distill(logits, teacher_index, teacher_value, *, temperature=1.0, tail=False):
+    """Distill(loss, lse, log_tail) per row: the divergence of softmax(logits / temperature) from a teacher known by its top
+    alternatives (int32 indices, -1 = unused, and float32 values, both [rows, listed]).  tail=False: the values are logits, the listed
+    alternatives are all there is.  tail=True: the values are log probabilities at this temperature (log_probs(teacher, top=...,
+    scale=1 / temperature)), and what they leave is one more outcome.  log_tail is None without tail."""
+    who = "distill"
+    device = _floats(who, logits=logits)
+    _require(math.isfinite(temperature) and temperature > 0, f"{who}: temperature {temperature}")
+    cfg = _rows_config(who, logits, 1.0 / temperature)
+    listed = _teacher(who, logits, teacher_index, teacher_value)
+    loss, lse = (torch.empty(cfg.rows, dtype=torch.float32, device=device) for _ in range(2))
+    log_tail = torch.empty(cfg.rows, dtype=torch.float32, device=device) if tail else None
+    check(_lib.lib().urf_distill(C.byref(cfg), _p(logits), _p(teacher_index), _p(teacher_value), listed, int(bool(tail)), _p(loss), _p(lse),
+                                 _p(log_tail), _stream(device)), "urf_distill")
+    return Distill(loss, lse, log_tail)
+
+
+def distill_backward(d_loss, logits, teacher_index, teacher_value, lse, log_tail=None, *, temperature=1.0, tail=False):
+    """The gradient of sum(loss * d_loss) with respect to logits; lse, log_tail and the other arguments are distill()'s."""
+    who = "distill_backward"
+    device = _floats(who, logits=logits)
+    _require(math.isfinite(temperature) and temperature > 0, f"{who}: temperature {temperature}")
+    cfg = _rows_config(who, logits, 1.0 / temperature)
+    listed = _teacher(who, logits, teacher_index, teacher_value)
+    _f32(who, "d_loss", d_loss, (cfg.rows,), device)
+    _f32(who, "lse", lse, (cfg.rows,), device)
+    if tail:
+        _f32(who, "log_tail", log_tail, (cfg.rows,), device)
+    d = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    check(_lib.lib().urf_distill_backward(C.byref(cfg), _p(logits), _p(teacher_index), _p(teacher_value), listed, int(bool(tail)), _p(lse),
+                                          _p(log_tail if tail else None), _p(d_loss), _p(d), C.c_longlong(cfg.classes), _stream(device)),
+          "urf_distill_backward")
+    return d
