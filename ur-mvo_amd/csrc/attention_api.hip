@@ -8,9 +8,9 @@ namespace urf {
 hipError_t attn_forward_f32(const AttnArgs &, int, hipStream_t);
 hipError_t attn_forward_f16(const AttnArgs &, int, hipStream_t);
 hipError_t attn_forward_bf16(const AttnArgs &, int, hipStream_t);
-hipError_t attn_backward_f32(const AttnArgs &, hipStream_t);
-hipError_t attn_backward_f16(const AttnArgs &, hipStream_t);
-hipError_t attn_backward_bf16(const AttnArgs &, hipStream_t);
+hipError_t attn_backward_f32(const AttnArgs &, int, int, hipStream_t);
+hipError_t attn_backward_f16(const AttnArgs &, int, int, hipStream_t);
+hipError_t attn_backward_bf16(const AttnArgs &, int, int, hipStream_t);
 }  // namespace urf
 using namespace urf;
 
@@ -37,7 +37,29 @@ size_t forward_bytes(const urf_attn_config &c) {
   return rows * ((c.head_dim <= 64 ? 64 : 128) + 2) * sizeof(float);
 }
 
-size_t backward_bytes(const urf_attn_config &c) { return (size_t)c.batch * c.q_heads * c.q_len * sizeof(float); }
+// How the backward kernels are cut: 128 keys (rows) a workgroup, and where that leaves less than two workgroups per CU, the rows
+// (keys) in ranges of at least 256, whose partial sums are added in fp32 afterwards.
+int backward_splits(long long own, long long other, long long groups, bool causal) {
+  const long long blocks = (own + 127) / 128 * groups, most = other / 256, want = ((causal ? 768 : 512) + blocks - 1) / (blocks > 0 ? blocks : 1);
+  const long long s = want < most ? want : most;
+  return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
+}
+void backward_shape(const urf_attn_config &c, int *kv_splits, int *q_splits) {
+  const long long rows = (long long)c.q_len * (c.q_heads / c.kv_heads), groups = (long long)c.batch * c.kv_heads;
+  *kv_splits = backward_splits(c.k_len, rows, groups, c.causal);
+  *q_splits = backward_splits(rows, c.k_len, groups, c.causal);
+}
+
+size_t delta_bytes(const urf_attn_config &c) { return ((size_t)c.batch * c.q_heads * c.q_len * sizeof(float) + 15) / 16 * 16; }
+
+// delta, then the partial sums of dk and dv, and after them those of dq in the same place
+size_t backward_bytes(const urf_attn_config &c) {
+  int kv, q;
+  backward_shape(c, &kv, &q);
+  const size_t dp = (c.head_dim <= 64 ? 64 : 128) * sizeof(float);
+  const size_t a = kv > 1 ? 2 * (size_t)kv * c.batch * c.kv_heads * c.k_len * dp : 0, b = q > 1 ? (size_t)q * c.batch * c.q_heads * c.q_len * dp : 0;
+  return delta_bytes(c) + (a > b ? a : b);
+}
 
 int check_config(const urf_attn_config *c, const char *who) {
   URF_CHECK(c, "%s: null configuration", who);
@@ -139,9 +161,12 @@ extern "C" int urf_attn_backward(const urf_attn_config *cfg, const urf_attn_tens
   a.o = view(o); a.dout = view(d_o); a.dq = view(dq); a.dk = view(dk); a.dv = view(dv);
   a.lse = (float *)d_lse;
   a.delta = (float *)d_work;
+  a.part_o = (float *)((char *)d_work + delta_bytes(*cfg));
+  int kv, qs;
+  backward_shape(*cfg, &kv, &qs);
   OnDevice on(cfg->device);
   URF_HIP(on.rc);
   const hipStream_t st = (hipStream_t)stream;
-  URF_HIP(cfg->dtype == URF_F32 ? attn_backward_f32(a, st) : cfg->dtype == URF_F16 ? attn_backward_f16(a, st) : attn_backward_bf16(a, st));
+  URF_HIP(cfg->dtype == URF_F32 ? attn_backward_f32(a, kv, qs, st) : cfg->dtype == URF_F16 ? attn_backward_f16(a, kv, qs, st) : attn_backward_bf16(a, kv, qs, st));
   return 0;
 }

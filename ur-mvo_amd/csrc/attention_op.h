@@ -117,23 +117,45 @@ template <typename T, int DP> struct Tile {
   }
 };
 
-// Copies R rows (from `first`, valid below `end`) of one head into a tile: chunks beyond the head size and rows at or behind
-// `end` become zero -- what lies behind a sequence's end may be anything, NaN included, and never enters a product.
-// `group` > 1 walks (i, g) rows of a query tensor.  Two halves: the loads into registers, and the LDS writes.
+// Copies tiles of R consecutive rows into LDS, one after the other, through registers: load() fetches the next tile, store() writes
+// it.  Rows at or behind `end` and chunks beyond the head size become zero -- what lies behind a sequence's end may be anything,
+// NaN included, and never enters a product.  Every thread walks pointers of its own: an (i, g) row advances by R rows without a
+// division.
 template <typename T, int DP, int R> struct Stage {
   typedef Tile<T, DP> TL;
   static constexpr int kN = R * TL::kChunks / 256;
+  static_assert(R * TL::kChunks % 256 == 0, "whole chunks per thread");
   u32x4 x[kN];
-  __device__ __forceinline__ void load(const T *head, long long srow, long long shead, int group, int first, int end, int D, int tid) {
+  const T *p[kN];
+  int g[kN], row, group;            // row of chunk 0; chunk n is 256 / kChunks * n rows further
+  long long step, wrap;
+  bool inner;                       // the chunk lies within the head size
+  __device__ __forceinline__ void start(const T *head, long long srow, long long shead, int grp, int first, int D, int tid) {
+    group = grp;
+    row = first + tid / TL::kChunks;
+    const int c = tid % TL::kChunks;
+    inner = c * TL::kPer < D;
+    step = (long long)(R / grp) * srow + (long long)(R % grp) * shead;
+    wrap = srow - (long long)grp * shead;
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-      const int u = tid + 256 * n, r = first + u / TL::kChunks, c = u % TL::kChunks;
+      const int r = row + 256 / TL::kChunks * n, i = grp == 1 ? r : r / grp;
+      g[n] = r - i * grp;
+      p[n] = head + (long long)i * srow + (long long)g[n] * shead + c * TL::kPer;
+    }
+  }
+  __device__ __forceinline__ void load(int end) {
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
       x[n] = u32x4{0, 0, 0, 0};
-      if (r < end && c * TL::kPer < D) {
-        const int i = group == 1 ? r : r / group, g = group == 1 ? 0 : r - i * group;
-        x[n] = *(const u32x4 *)(head + (long long)i * srow + (long long)g * shead + c * TL::kPer);
+      if (inner && row + 256 / TL::kChunks * n < end) x[n] = *(const u32x4 *)p[n];
+      p[n] += step;
+      if (group > 1) {
+        g[n] += R % group;
+        if (g[n] >= group) { g[n] -= group; p[n] += wrap; }
       }
     }
+    row += R;
   }
   __device__ __forceinline__ void store(char *tile, int tid) const {
 #pragma unroll
@@ -165,11 +187,23 @@ template <typename T> __device__ __forceinline__ void store4(T *p, float a, floa
   *(T4 *)p = T4{(T)a, (T)b, (T)c, (T)d};
 }
 
+// a lane's column of a transposed accumulator (row `p` of the output): four consecutive elements at a time
+template <typename T, int DP> __device__ __forceinline__ void store_rows(T *p, const f32x16 *acc, float f, int D, int half) {
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = 32 * dt + 2 * r + 4 * half;
+      if (d < D) store4<T>(p + d, acc[dt][r] * f, acc[dt][r + 1] * f, acc[dt][r + 2] * f, acc[dt][r + 3] * f);
+    }
+}
+
 __device__ __forceinline__ int clamp_len(const int *lens, int b, int most) {
   return lens ? min(max(lens[b], 0), most) : most;      // lengths come from device memory: never trusted beyond the tensor
 }
 
 // ------------------------------------------------------------------ forward
+constexpr float kSlack = 6.0f;      // log2: probabilities up to 64 before normalisation, in range of every type
 // One workgroup: SPLIT = 0: 128 rows, 32 per wave, over tiles of 64 keys; SPLIT = 1: 32 rows, each of the four waves a quarter of
 // a 128-key tile, joined through LDS at the end (few rows: more workgroups, more loads in flight).  The key range may be cut in
 // `splits` parts, joined by attn_join_kernel.
@@ -212,16 +246,18 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
   for (int dt = 0; dt < kDt; ++dt) acc[dt] = f32x16{};
   float m = -INFINITY, l = 0.0f;          // running maximum (log2 units) and this half wave's share of the sum
   Stage<T, DP, kKeys> ks, vs;
-  ks.load(kh, a.k.r, 0, 1, begin, min(nk, block_end), a.D, tid);
-  vs.load(vh, a.v.r, 0, 1, begin, min(nk, block_end), a.D, tid);
+  ks.start(kh, a.k.r, 0, 1, begin, a.D, tid);
+  vs.start(vh, a.v.r, 0, 1, begin, a.D, tid);
+  ks.load(block_end);
+  vs.load(block_end);
   for (int key0 = begin; key0 < block_end; key0 += kKeys) {
     lds_barrier();                        // the previous tile has been read
     ks.store(kt, tid);
     vs.store(vt, tid);
     lds_barrier();
     if (key0 + kKeys < block_end) {
-      ks.load(kh, a.k.r, 0, 1, key0 + kKeys, min(nk, block_end), a.D, tid);
-      vs.load(vh, a.v.r, 0, 1, key0 + kKeys, min(nk, block_end), a.D, tid);
+      ks.load(block_end);
+      vs.load(block_end);
     }
     f32x16 s[kSub];
 #pragma unroll
@@ -244,9 +280,16 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
       }
     }
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float mn = fmaxf(m, top), mu = mn == -INFINITY ? 0.0f : mn;      // nothing visible yet: all the exponentials are 0
-    const float alpha = exp2f(m - mu);
-    m = mn;
+    // The running maximum only has to keep the exponentials in range: it moves when some row of the wave has grown by more than
+    // 2^kSlack, so that the accumulators are rescaled once or twice per row, not once per tile.
+    if (__any(top > m + kSlack)) {
+      const float mn = fmaxf(m, top), alpha = mn == -INFINITY ? 1.0f : exp2f(m - mn);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < kDt; ++dt) acc[dt] *= alpha;
+    }
+    const float mu = m == -INFINITY ? 0.0f : m;           // nothing visible yet: all the exponentials are 0
     float sum = 0.0f;
 #pragma unroll
     for (int u = 0; u < kSub; ++u)
@@ -255,9 +298,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
         s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - mu);
         sum += s[u][r];
       }
-    l = l * alpha + sum;
-#pragma unroll
-    for (int dt = 0; dt < kDt; ++dt) acc[dt] *= alpha;
+    l += sum;
 #pragma unroll
     for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -311,14 +352,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
     }
   } else if (inside) {
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    T *orow = (T *)a.o.p + (long long)b * a.o.b + (long long)i * a.o.r + (long long)(hk * a.G + g) * a.o.h;
-#pragma unroll
-    for (int dt = 0; dt < kDt; ++dt)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int d = 32 * dt + 2 * r + 4 * half;
-        if (d < a.D) store4<T>(orow + d, acc[dt][r] * inv, acc[dt][r + 1] * inv, acc[dt][r + 2] * inv, acc[dt][r + 3] * inv);
-      }
+    store_rows<T, DP>((T *)a.o.p + (long long)b * a.o.b + (long long)i * a.o.r + (long long)(hk * a.G + g) * a.o.h, acc, inv, a.D, half);
     if (half == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
   }
 }
@@ -379,66 +413,86 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a) {
   if (inside && c == 0) a.delta[((long long)b * a.Hq + h) * a.Lq + i] = s;
 }
 
-// dk and dv of 128 keys, 32 per wave, whose k and v rows stay in registers; walks the query rows in tiles of 32.
+// dk and dv of 128 keys, 32 per wave; walks the query rows in tiles of 32 (or one of `splits` equal ranges of them).  k stays in
+// registers, v in LDS: with both in registers the accumulators leave room for one wave per SIMD only, and nothing runs beside its
+// waits.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, 1) attn_backward_kv_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_kv_kernel(AttnArgs a) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::Frag Frag;
   constexpr int kRows = 32, kKc = DP / 16, kDt = DP / 32;
   extern __shared__ __align__(16) char lds[];
-  char *qt = lds, *dt_ = lds + kRows * TL::kBytes;
-  float *lt = (float *)(lds + 2 * kRows * TL::kBytes), *et = lt + kRows;      // lse (log2 units) and delta of the rows
+  char *vt = lds, *qt = vt + 128 * TL::kBytes, *dt_ = qt + kRows * TL::kBytes;
+  float *lt = (float *)(dt_ + kRows * TL::kBytes), *et = lt + kRows;          // lse (log2 units) and delta of the rows
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
   int tile, group;
-  xcd_group_map(blockIdx.x, a.tiles, a.B * a.Hk, tile, group);
+  xcd_group_map(blockIdx.x, a.tiles * a.splits, a.B * a.Hk, tile, group);     // causal: the first keys, seen by most rows, first
+  const int split = tile % a.splits;
+  tile /= a.splits;
   const int b = group / a.Hk, hk = group % a.Hk;
   const int nq = clamp_len(a.q_lens, b, a.Lq), nk = clamp_len(a.k_lens, b, a.Lk);
   const int key = tile * 128 + 32 * wave + col;
-  const bool inside = key < a.Lk, active = key < nk;
-  const T *qh = (const T *)a.q.p + (long long)b * a.q.b + (long long)hk * a.G * a.q.h;
-  const T *dh = (const T *)a.dout.p + (long long)b * a.dout.b + (long long)hk * a.G * a.dout.h;
   const T *krow = (const T *)a.k.p + (long long)b * a.k.b + (long long)key * a.k.r + (long long)hk * a.k.h;
-  const T *vrow = (const T *)a.v.p + (long long)b * a.v.b + (long long)key * a.v.r + (long long)hk * a.v.h;
-  Frag k[kKc], v[kKc];
+  Frag k[kKc];
 #pragma unroll
-  for (int kc = 0; kc < kKc; ++kc) { k[kc] = load_frag<T>(krow, active, kc, half, a.D); v[kc] = load_frag<T>(vrow, active, kc, half, a.D); }
+  for (int kc = 0; kc < kKc; ++kc) k[kc] = load_frag<T>(krow, key < nk, kc, half, a.D);
+  {
+    Stage<T, DP, 32> vs;
+    vs.start((const T *)a.v.p + (long long)b * a.v.b + (long long)hk * a.v.h, a.v.r, 0, 1, tile * 128, a.D, tid);
+    for (int n = 0; n < 4; ++n) {
+      vs.load(nk);
+      vs.store(vt + n * 32 * TL::kBytes, tid);
+    }
+  }
   f32x16 dk[kDt], dv[kDt];
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt) dk[dt] = dv[dt] = f32x16{};
-  // rows [row_first, rows) see some key of the workgroup; causal: key j is seen by i >= j - (nk - nq)
-  const int rows = tile * 128 < nk ? nq * a.G : 0;
-  const int i_min = a.causal ? max(0, tile * 128 - (nk - nq)) : 0;
-  const int row_first = min((long long)i_min * a.G, (long long)rows) / kRows * kRows;
+  // rows [begin, rows) see some key of the workgroup; causal: key j is seen by i >= j - (nk - nq), which is row >= first_row
+  int rows = tile * 128 < nk ? nq * a.G : 0;
+  const int seen_by = a.causal ? max(0, key - (nk - nq)) : 0, first_row = key < nk && seen_by < nq ? seen_by * a.G : rows;
+  const int i_min = a.causal ? min(nq, max(0, tile * 128 - (nk - nq))) : 0, i_all = a.causal ? max(0, tile * 128 + 127 - (nk - nq)) : 0;
+  const long long all_from = tile * 128 + 128 <= nk ? (long long)i_all * a.G : rows;    // from here on every row sees every key
+  int begin = min(i_min * a.G, rows) / kRows * kRows;
+  {
+    const int t = (rows - begin + kRows - 1) / kRows, per = (t + a.splits - 1) / a.splits;
+    begin = min(rows, begin + split * per * kRows);
+    rows = (int)min((long long)rows, (long long)begin + (long long)per * kRows);
+  }
   Stage<T, DP, kRows> qs, ds;
-  float lse_next = 0.0f;
-  auto load = [&](int r0) {
-    qs.load(qh, a.q.r, a.q.h, a.G, r0, rows, a.D, tid);
-    ds.load(dh, a.dout.r, a.dout.h, a.G, r0, rows, a.D, tid);
+  qs.start((const T *)a.q.p + (long long)b * a.q.b + (long long)hk * a.G * a.q.h, a.q.r, a.q.h, a.G, begin, a.D, tid);
+  ds.start((const T *)a.dout.p + (long long)b * a.dout.b + (long long)hk * a.G * a.dout.h, a.dout.r, a.dout.h, a.G, begin, a.D, tid);
+  // threads 0..31 carry the rows' lse, 32..63 their delta
+  int stat_row = begin + (tid & (kRows - 1)), stat_i = stat_row / a.G, stat_g = stat_row - stat_i * a.G;
+  const float *stat = (tid < kRows ? a.lse : a.delta) + ((long long)b * a.Hq + hk * a.G) * a.Lq;
+  float stat_next = 0.0f;
+  auto load = [&]() {
+    qs.load(rows);
+    ds.load(rows);
     if (tid < 2 * kRows) {
-      const int r = r0 + (tid & (kRows - 1)), i = r / a.G, g = r - i * a.G;
-      lse_next = 0.0f;
-      if (r < rows) {
-        const long long at = ((long long)b * a.Hq + hk * a.G + g) * a.Lq + i;
-        lse_next = tid < kRows ? a.lse[at] * kLog2e : a.delta[at];
-      }
+      stat_next = 0.0f;
+      if (stat_row < rows) stat_next = stat[(long long)stat_g * a.Lq + stat_i] * (tid < kRows ? kLog2e : 1.0f);
+      stat_row += kRows;
+      stat_i += kRows / a.G;
+      stat_g += kRows % a.G;
+      if (stat_g >= a.G) { stat_g -= a.G; ++stat_i; }
     }
   };
-  if (row_first < rows) load(row_first);
-  for (int r0 = row_first; r0 < rows; r0 += kRows) {
+  if (begin < rows) load();
+  for (int r0 = begin; r0 < rows; r0 += kRows) {
     lds_barrier();
     qs.store(qt, tid);
     ds.store(dt_, tid);
-    if (tid < 2 * kRows) lt[tid] = lse_next;
+    if (tid < 2 * kRows) lt[tid] = stat_next;
     lds_barrier();
-    if (r0 + kRows < rows) load(r0 + kRows);
+    if (r0 + kRows < rows) load();
     f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
     for (int kc = 0; kc < kKc; ++kc) {
       s = Elem<T>::mma(TL::row(qt, col, kc, half), k[kc], s);
-      dp = Elem<T>::mma(TL::row(dt_, col, kc, half), v[kc], dp);
+      dp = Elem<T>::mma(TL::row(dt_, col, kc, half), TL::row(vt, 32 * wave + col, kc, half), dp);
     }
     // some row of the tile does not see some key of the workgroup (or there is no such row)
-    const bool edge = r0 + kRows > rows || tile * 128 + 128 > nk || (a.causal && tile * 128 + 127 > r0 / a.G + nk - nq);
+    const bool edge = r0 + kRows > rows || r0 < all_from;
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
       const f32x4 ls = *(const f32x4 *)(lt + 8 * r4 + 4 * half), de = *(const f32x4 *)(et + 8 * r4 + 4 * half);
@@ -447,8 +501,8 @@ __global__ void __launch_bounds__(256, 1) attn_backward_kv_kernel(AttnArgs a) {
         const int r = 4 * r4 + e;
         float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -ls[e]));
         if (edge) {
-          const int row = r0 + 8 * r4 + 4 * half + e, i = row / a.G;
-          if (!(row < rows && active && (!a.causal || key <= i + nk - nq))) p = 0.0f;
+          const int row = r0 + 8 * r4 + 4 * half + e;
+          if (row < first_row || row >= rows) p = 0.0f;
         }
         s[r] = p;
         dp[r] = p * (dp[r] - de[e]);
@@ -464,24 +518,20 @@ __global__ void __launch_bounds__(256, 1) attn_backward_kv_kernel(AttnArgs a) {
       }
     }
   }
-  if (!inside) return;
-  T *dkrow = (T *)a.dk.p + (long long)b * a.dk.b + (long long)key * a.dk.r + (long long)hk * a.dk.h;
-  T *dvrow = (T *)a.dv.p + (long long)b * a.dv.b + (long long)key * a.dv.r + (long long)hk * a.dv.h;
-#pragma unroll
-  for (int dt = 0; dt < kDt; ++dt)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int d = 32 * dt + 2 * r + 4 * half;
-      if (d < a.D) {
-        store4<T>(dkrow + d, dk[dt][r] * a.scale, dk[dt][r + 1] * a.scale, dk[dt][r + 2] * a.scale, dk[dt][r + 3] * a.scale);
-        store4<T>(dvrow + d, dv[dt][r], dv[dt][r + 1], dv[dt][r + 2], dv[dt][r + 3]);
-      }
-    }
+  if (key >= a.Lk) return;
+  if (a.splits > 1) {
+    const long long at = ((long long)split * a.B * a.Hk + group) * a.Lk + key, other = (long long)a.splits * a.B * a.Hk * a.Lk * DP;
+    store_rows<float, DP>(a.part_o + at * DP, dk, a.scale, DP, half);
+    store_rows<float, DP>(a.part_o + other + at * DP, dv, 1.0f, DP, half);
+  } else {
+    store_rows<T, DP>((T *)a.dk.p + (long long)b * a.dk.b + (long long)key * a.dk.r + (long long)hk * a.dk.h, dk, a.scale, a.D, half);
+    store_rows<T, DP>((T *)a.dv.p + (long long)b * a.dv.b + (long long)key * a.dv.r + (long long)hk * a.dv.h, dv, 1.0f, a.D, half);
+  }
 }
 
-// dq of 128 rows, 32 per wave, whose q and do rows stay in registers; walks the keys in tiles of 32.
+// dq of 128 rows, 32 per wave, whose q and do rows stay in registers; walks the keys (or one of `splits` ranges) in tiles of 32.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256, 1) attn_backward_q_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_q_kernel(AttnArgs a) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::Frag Frag;
   constexpr int kKeys = 32, kKc = DP / 16, kDt = DP / 32;
@@ -489,17 +539,24 @@ __global__ void __launch_bounds__(256, 1) attn_backward_q_kernel(AttnArgs a) {
   char *kt = lds, *vt = lds + kKeys * TL::kBytes;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
   int tile, group;
-  xcd_group_map(blockIdx.x, a.tiles, a.B * a.Hk, tile, group);
-  tile = a.tiles - 1 - tile;
+  xcd_group_map(blockIdx.x, a.tiles * a.splits, a.B * a.Hk, tile, group);
+  const int split = tile % a.splits;
+  tile = a.tiles - 1 - tile / a.splits;
   const int b = group / a.Hk, hk = group % a.Hk;
   const int nq = clamp_len(a.q_lens, b, a.Lq), nk = clamp_len(a.k_lens, b, a.Lk);
   const int row = tile * 128 + 32 * wave + col, i = row / a.G, g = row - i * a.G;
   const bool inside = row < a.Lq * a.G, active = i < nq;
   const int seen = !active ? 0 : a.causal ? min(nk, max(0, i + 1 + nk - nq)) : nk;
   const int i_last = min(nq, (min((tile + 1) * 128, a.Lq * a.G) - 1) / a.G + 1) - 1, i_first = tile * 128 / a.G;
-  const int block_end = i_first >= nq ? 0 : a.causal ? min(nk, max(0, i_last + 1 + nk - nq)) : nk;
+  int block_end = i_first >= nq ? 0 : a.causal ? min(nk, max(0, i_last + 1 + nk - nq)) : nk;
   const int full_end = a.causal ? min(nk, max(0, i_first + 1 + nk - nq)) : nk;
   const bool all_active = (i_last + 1) * a.G >= (tile + 1) * 128;
+  int begin = 0;
+  {
+    const int n = (block_end + kKeys - 1) / kKeys, per = (n + a.splits - 1) / a.splits;
+    begin = min(block_end, split * per * kKeys);
+    block_end = min(block_end, begin + per * kKeys);
+  }
   const int h = hk * a.G + g;
   const T *qrow = (const T *)a.q.p + (long long)b * a.q.b + (long long)i * a.q.r + (long long)h * a.q.h;
   const T *drow = (const T *)a.dout.p + (long long)b * a.dout.b + (long long)i * a.dout.r + (long long)h * a.dout.h;
@@ -514,16 +571,18 @@ __global__ void __launch_bounds__(256, 1) attn_backward_q_kernel(AttnArgs a) {
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt) dq[dt] = f32x16{};
   Stage<T, DP, kKeys> ks, vs;
-  ks.load(kh, a.k.r, 0, 1, 0, block_end, a.D, tid);
-  vs.load(vh, a.v.r, 0, 1, 0, block_end, a.D, tid);
-  for (int key0 = 0; key0 < block_end; key0 += kKeys) {
+  ks.start(kh, a.k.r, 0, 1, begin, a.D, tid);
+  vs.start(vh, a.v.r, 0, 1, begin, a.D, tid);
+  ks.load(block_end);
+  vs.load(block_end);
+  for (int key0 = begin; key0 < block_end; key0 += kKeys) {
     lds_barrier();
     ks.store(kt, tid);
     vs.store(vt, tid);
     lds_barrier();
     if (key0 + kKeys < block_end) {
-      ks.load(kh, a.k.r, 0, 1, key0 + kKeys, block_end, a.D, tid);
-      vs.load(vh, a.v.r, 0, 1, key0 + kKeys, block_end, a.D, tid);
+      ks.load(block_end);
+      vs.load(block_end);
     }
     f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
@@ -531,11 +590,11 @@ __global__ void __launch_bounds__(256, 1) attn_backward_q_kernel(AttnArgs a) {
       s = Elem<T>::mma(TL::row(kt, col, kc, half), q[kc], s);
       dp = Elem<T>::mma(TL::row(vt, col, kc, half), d[kc], dp);
     }
-    const bool edge = key0 + kKeys > full_end || !all_active;
+    const bool edge = key0 + kKeys > min(full_end, block_end) || !all_active;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -ls));
-      if (edge && key0 + 8 * (r >> 2) + 4 * half + (r & 3) >= seen) p = 0.0f;
+      if (edge && key0 + 8 * (r >> 2) + 4 * half + (r & 3) >= min(seen, block_end)) p = 0.0f;
       dp[r] = p * (dp[r] - de);
     }
 #pragma unroll
@@ -546,14 +605,22 @@ __global__ void __launch_bounds__(256, 1) attn_backward_q_kernel(AttnArgs a) {
     }
   }
   if (!inside) return;
-  T *out = (T *)a.dq.p + (long long)b * a.dq.b + (long long)i * a.dq.r + (long long)h * a.dq.h;
-#pragma unroll
-  for (int dt = 0; dt < kDt; ++dt)
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int e = 32 * dt + 2 * r + 4 * half;
-      if (e < a.D) store4<T>(out + e, dq[dt][r] * a.scale, dq[dt][r + 1] * a.scale, dq[dt][r + 2] * a.scale, dq[dt][r + 3] * a.scale);
-    }
+  if (a.splits > 1)
+    store_rows<float, DP>(a.part_o + (((long long)split * a.B * a.Hk + group) * ((long long)a.Lq * a.G) + row) * DP, dq, a.scale, DP, half);
+  else
+    store_rows<T, DP>((T *)a.dq.p + (long long)b * a.dq.b + (long long)i * a.dq.r + (long long)h * a.dq.h, dq, a.scale, a.D, half);
+}
+
+// out = the sum of `splits` partial gradients, in their order; rows (group, row) of DP floats, row = i * per_i + g
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) attn_sum_kernel(const float *part, AttnView out, int groups, int heads, int rows, int per_i, int splits, int D) {
+  const long long u = (long long)blockIdx.x * 256 + threadIdx.x, r = u / (DP / 4);
+  const int d = (int)(u % (DP / 4)) * 4;
+  if (r >= (long long)groups * rows || d >= D) return;
+  f32x4 s = *(const f32x4 *)(part + r * DP + d);
+  for (int n = 1; n < splits; ++n) s += *(const f32x4 *)(part + ((long long)n * groups * rows + r) * DP + d);
+  const int group = (int)(r / rows), row = (int)(r % rows), b = group / heads, hk = group % heads, i = row / per_i, g = row - i * per_i;
+  store4<T>((T *)out.p + (long long)b * out.b + (long long)i * out.r + (long long)(hk * per_i + g) * out.h + d, s[0], s[1], s[2], s[3]);
 }
 
 // ------------------------------------------------------------------ launches
@@ -583,26 +650,45 @@ template <typename T, int DP> hipError_t attn_forward_dp(AttnArgs a, int narrow,
   return hipGetLastError();
 }
 
-template <typename T, int DP> hipError_t attn_backward_dp(AttnArgs a, hipStream_t st) {
+template <typename T, int DP>
+hipError_t launch_sum(const float *part, const AttnView &out, const AttnArgs &a, int rows, int per_i, hipStream_t st) {
+  const long long n = (long long)a.B * a.Hk * rows * (DP / 4);
+  hipLaunchKernelGGL((attn_sum_kernel<T, DP>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, out, a.B * a.Hk, a.Hk, rows, per_i, a.splits, a.D);
+  return hipGetLastError();
+}
+
+template <typename T, int DP> hipError_t attn_backward_dp(AttnArgs a, int kv_splits, int q_splits, hipStream_t st) {
   const long long rows = (long long)a.B * a.Lq * a.Hq;
   hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
-  const int lds = 2 * 32 * Tile<T, DP>::kBytes;
-  a.tiles = (a.Lk + 127) / 128;
-  hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP>), dim3((unsigned)a.tiles * a.B * a.Hk), dim3(256), lds + 256, st, a);
-  rc = hipGetLastError();
-  if (rc != hipSuccess) return rc;
+  constexpr int kBytes = Tile<T, DP>::kBytes;
+  if (a.Lk > 0) {
+    static DeviceOnce once;
+    const int lds = (128 + 2 * 32) * kBytes + 256;
+    rc = allow_lds(once, (const void *)attn_backward_kv_kernel<T, DP>, lds);
+    if (rc != hipSuccess) return rc;
+    a.tiles = (a.Lk + 127) / 128;
+    a.splits = kv_splits;
+    hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP>), dim3((unsigned)a.tiles * a.splits * a.B * a.Hk), dim3(256), lds, st, a);
+    rc = hipGetLastError();
+    if (rc == hipSuccess && a.splits > 1) rc = launch_sum<T, DP>(a.part_o, a.dk, a, a.Lk, 1, st);
+    if (rc == hipSuccess && a.splits > 1) rc = launch_sum<T, DP>(a.part_o + (long long)a.splits * a.B * a.Hk * a.Lk * DP, a.dv, a, a.Lk, 1, st);
+    if (rc != hipSuccess) return rc;
+  }
   a.tiles = (a.Lq * a.G + 127) / 128;
-  hipLaunchKernelGGL((attn_backward_q_kernel<T, DP>), dim3((unsigned)a.tiles * a.B * a.Hk), dim3(256), lds, st, a);
-  return hipGetLastError();
+  a.splits = q_splits;
+  hipLaunchKernelGGL((attn_backward_q_kernel<T, DP>), dim3((unsigned)a.tiles * a.splits * a.B * a.Hk), dim3(256), 2 * 32 * kBytes, st, a);
+  rc = hipGetLastError();
+  if (rc == hipSuccess && a.splits > 1) rc = launch_sum<T, DP>(a.part_o, a.dq, a, a.Lq * a.G, a.G, st);
+  return rc;
 }
 
 template <typename T> hipError_t attn_forward_t(const AttnArgs &a, int narrow, hipStream_t st) {
   return a.D <= 64 ? attn_forward_dp<T, 64>(a, narrow, st) : attn_forward_dp<T, 128>(a, narrow, st);
 }
-template <typename T> hipError_t attn_backward_t(const AttnArgs &a, hipStream_t st) {
-  return a.D <= 64 ? attn_backward_dp<T, 64>(a, st) : attn_backward_dp<T, 128>(a, st);
+template <typename T> hipError_t attn_backward_t(const AttnArgs &a, int kv_splits, int q_splits, hipStream_t st) {
+  return a.D <= 64 ? attn_backward_dp<T, 64>(a, kv_splits, q_splits, st) : attn_backward_dp<T, 128>(a, kv_splits, q_splits, st);
 }
 
 }  // namespace urf
