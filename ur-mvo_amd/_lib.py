@@ -89,20 +89,6 @@ class PoseOptStereoConfig(C.Structure):
                 ("chi2_mono", C.c_double), ("chi2_stereo", C.c_double)]
 
 
-class AttnConfig(C.Structure):
-    _fields_ = [("dtype", C.c_int), ("batch", C.c_int), ("q_heads", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
-                ("q_len", C.c_int), ("k_len", C.c_int), ("causal", C.c_int), ("scale", C.c_float), ("device", C.c_int)]
-
-
-class AttnTensor(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("batch_stride", C.c_longlong), ("row_stride", C.c_longlong), ("head_stride", C.c_longlong)]
-
-
-class RowsConfig(C.Structure):
-    _fields_ = [("dtype", C.c_int), ("rows", C.c_int), ("classes", C.c_int), ("row_stride", C.c_longlong), ("scale", C.c_float),
-                ("device", C.c_int)]
-
-
 class DMatch(C.Structure):
     _fields_ = [("queryIdx", C.c_int), ("trainIdx", C.c_int), ("distance", C.c_float)]
 
@@ -151,6 +137,15 @@ def lib():
         L.urf_sp_stream.restype = C.c_void_p
         L.urf_sp_result_stream.restype = C.c_void_p
         L.urf_pm_stream.restype = C.c_void_p
+        # the operators on torch tensors (operators.py): addresses are plain integers, structs come as bytes
+        P, B, I, Z = C.c_void_p, C.c_char_p, C.c_int, C.c_size_t
+        L.urf_attn_workspace.argtypes = [B, I, P]
+        L.urf_attn_forward.argtypes = [B] * 4 + [P, P, B, P, P, Z, P]
+        L.urf_attn_backward.argtypes = [B] * 5 + [P, B, P, P, B, B, B, P, Z, P]
+        L.urf_log_probs.argtypes = [B, P, P, I, I, P, P, P, P, P, P]
+        L.urf_log_probs_backward.argtypes = [B, P, P, I, P, P, P, P, P, C.c_longlong, P]
+        L.urf_distill.argtypes = [B, P, P, P, I, I, P, P, P, P]
+        L.urf_distill_backward.argtypes = [B, P, P, P, I, I, P, P, P, P, C.c_longlong, P]
         _lib = L
     return _lib
 

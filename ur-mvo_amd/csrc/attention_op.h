@@ -76,42 +76,54 @@ template <typename T, int DP> struct Tile {
     else if constexpr (kBytes == 256) return ((r & 3) << 2) | ((r >> 2) & 3);
     else return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
   }
-  static __device__ __forceinline__ const char *at(const char *tile, int r, int c) { return tile + r * kBytes + ((c ^ swizzle(r)) << 4); }
   static __device__ __forceinline__ char *at(char *tile, int r, int c) { return tile + r * kBytes + ((c ^ swizzle(r)) << 4); }
-  // elements 16 kc + 8 half .. + 7 of row r
-  static __device__ __forceinline__ typename Elem<T>::Frag row(const char *tile, int r, int kc, int half) {
+  // Elements 16 kc + 8 half .. + 7 of row r0 + r: `base` = row_base(r, half), once; r0 a multiple of 16 (the swizzle's period), so
+  // that a read costs one xor of the address, the rest is its immediate offset.
+  static __device__ __forceinline__ unsigned row_base(int r, int half) {
+    return r * kBytes + (((sizeof(T) == 2 ? half : 2 * half) ^ swizzle(r)) << 4);
+  }
+  static __device__ __forceinline__ typename Elem<T>::Frag row(const char *tile, unsigned base, int r0, int kc) {
+    const char *p = tile + r0 * kBytes;
     if constexpr (sizeof(T) == 2) {
-      return *(const typename Elem<T>::Frag *)at(tile, r, 2 * kc + half);
+      return *(const typename Elem<T>::Frag *)(p + (base ^ (kc << 5)));
     } else {
-      const f32x4 a = *(const f32x4 *)at(tile, r, 4 * kc + 2 * half), b = *(const f32x4 *)at(tile, r, 4 * kc + 2 * half + 1);
+      const f32x4 a = *(const f32x4 *)(p + (base ^ (kc << 6))), b = *(const f32x4 *)(p + (base ^ (kc << 6) ^ 16));
       f32x8 f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) { f[e] = a[e]; f[4 + e] = b[e]; }
       return f;
     }
   }
-  // column 32 dt + l % 32 of rows r0 + 16 t + {4 half + 0..3, 8 + 4 half + 0..3}: the left operand of a product over rows
-  static __device__ __forceinline__ typename Elem<T>::Frag column(const char *tile, int r0, int dt, int lane) {
+  // Column 32 dt + l % 32 of rows r0 + {4 half + 0..3, 8 + 4 half + 0..3}, r0 a multiple of 16: the left operand of a product over
+  // rows.  16-bit types: the 16 lanes of a group read four rows of 16 elements, four elements a lane, and get one column of four
+  // rows each.
+  struct ColBase { unsigned a, b; };
+  static __device__ __forceinline__ ColBase col_base(int lane) {
     const int half = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, r = 4 * half + (i >> 2), c = 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
+      return {(unsigned)(r * kBytes + ((c ^ swizzle(r)) << 4) + 8 * (i & 1)), (unsigned)((r + 8) * kBytes + ((c ^ swizzle(r + 8)) << 4) + 8 * (i & 1))};
+    } else {
+      const int d = lane & 31, r = 4 * half;               // rows r + 0..3 differ in the swizzle's bits 5 and 6 of the address
+      return {(unsigned)(r * kBytes + (((d >> 2) ^ swizzle(r)) << 4) + 4 * (d & 3)), (unsigned)((r + 8) * kBytes + (((d >> 2) ^ swizzle(r + 8)) << 4) + 4 * (d & 3))};
+    }
+  }
+  static __device__ __forceinline__ typename Elem<T>::Frag column(const char *tile, const ColBase &base, int r0, int dt) {
+    const char *p = tile + r0 * kBytes;
     typename Elem<T>::Frag f;
     if constexpr (sizeof(T) == 2) {
-      // the 16 lanes of a group read four rows of 16 elements, four elements a lane, and get one column of four rows each
       typedef short s16x4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s16x4 lds4;
-      const int i = lane & 15, r = r0 + 4 * half + (i >> 2), c = 4 * dt + 2 * ((lane >> 4) & 1) + ((i >> 1) & 1);
-      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(at(tile, r, c) + 8 * (i & 1)));
-      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(at(tile, r + 8, c) + 8 * (i & 1)));
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + (base.a ^ (dt << 6))));
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + (base.b ^ (dt << 6))));
       typedef T T4 __attribute__((ext_vector_type(4)));
       const T4 x = __builtin_bit_cast(T4, a), y = __builtin_bit_cast(T4, b);
 #pragma unroll
       for (int e = 0; e < 4; ++e) { f[e] = x[e]; f[4 + e] = y[e]; }
     } else {
-      const int d = 32 * dt + (lane & 31);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int r = r0 + 8 * (e >> 2) + 4 * half + (e & 3);
-        f[e] = *(const float *)(at(tile, r, d >> 2) + 4 * (d & 3));
-      }
+      for (int e = 0; e < 8; ++e)
+        f[e] = *(const float *)(p + (e & 3) * kBytes + ((e < 4 ? base.a : base.b) ^ (dt << 7) ^ ((e & 3) << 5)));
     }
     return f;
   }
@@ -158,11 +170,9 @@ template <typename T, int DP, int R> struct Stage {
     row += R;
   }
   __device__ __forceinline__ void store(char *tile, int tid) const {
+    char *p = TL::at(tile, tid / TL::kChunks, tid % TL::kChunks);
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      const int u = tid + 256 * n;
-      *(u32x4 *)TL::at(tile, u / TL::kChunks, u % TL::kChunks) = x[n];
-    }
+    for (int n = 0; n < kN; ++n) *(u32x4 *)(p + n * (256 / TL::kChunks) * TL::kBytes) = x[n];
   }
 };
 
@@ -213,8 +223,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
   typedef typename Elem<T>::Frag Frag;
   constexpr int kKeys = SPLIT ? 128 : 64, kRows = SPLIT ? 32 : 128, kKc = DP / 16, kDt = DP / 32, kSub = SPLIT ? 1 : 2;
   extern __shared__ __align__(16) char lds[];
-  char *kt = lds, *vt = lds + kKeys * TL::kBytes;
+  constexpr int kTile = kKeys * TL::kBytes;                // k, then v; SPLIT = 0: two buffers, one barrier per tile
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
+  const unsigned row_base = TL::row_base(col, half);
+  const typename TL::ColBase col_base = TL::col_base(lane);
   int tile, group;
   xcd_group_map(blockIdx.x, a.tiles * a.splits, a.B * a.Hk, tile, group);
   const int split = tile % a.splits;
@@ -250,12 +262,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
   vs.start(vh, a.v.r, 0, 1, begin, a.D, tid);
   ks.load(block_end);
   vs.load(block_end);
+  ks.store(lds, tid);
+  vs.store(lds + kTile, tid);
+  int buffer = 0;
   for (int key0 = begin; key0 < block_end; key0 += kKeys) {
-    lds_barrier();                        // the previous tile has been read
-    ks.store(kt, tid);
-    vs.store(vt, tid);
-    lds_barrier();
-    if (key0 + kKeys < block_end) {
+    lds_barrier();                        // this tile is written, the other buffer (if any) has been read
+    const char *kt = lds + buffer * 2 * kTile, *vt = kt + kTile;
+    const bool more = key0 + kKeys < block_end;
+    if (more) {
       ks.load(block_end);
       vs.load(block_end);
     }
@@ -263,23 +277,25 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
       s[u] = f32x16{};
-      const int r0 = SPLIT ? 32 * wave : 32 * u;
 #pragma unroll
-      for (int kc = 0; kc < kKc; ++kc) s[u] = Elem<T>::mma(TL::row(kt, r0 + col, kc, half), q[kc], s[u]);
+      for (int kc = 0; kc < kKc; ++kc) s[u] = Elem<T>::mma(TL::row(kt, row_base, SPLIT ? 32 * wave : 32 * u, kc), q[kc], s[u]);
     }
-    const bool edge = key0 + kKeys > min(full_end, block_end) || !all_active;
-    float top = -INFINITY;
+    if (key0 + kKeys > min(full_end, block_end) || !all_active) {
+      const int end = min(seen, block_end);
 #pragma unroll
-    for (int u = 0; u < kSub; ++u) {
-      const int k0 = key0 + (SPLIT ? 32 * wave : 32 * u) + 4 * half;
+      for (int u = 0; u < kSub; ++u) {
+        const int k0 = key0 + (SPLIT ? 32 * wave : 32 * u) + 4 * half;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[u][r] *= a.scale2;
-        if (edge && k0 + 8 * (r >> 2) + (r & 3) >= min(seen, block_end)) s[u][r] = -INFINITY;
-        top = fmaxf(top, s[u][r]);
+        for (int r = 0; r < 16; ++r)
+          if (k0 + 8 * (r >> 2) + (r & 3) >= end) s[u][r] = -INFINITY;
       }
     }
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    float top = s[0][0];
+#pragma unroll
+    for (int u = 0; u < kSub; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.scale2;
     // The running maximum only has to keep the exponentials in range: it moves when some row of the wave has grown by more than
     // 2^kSlack, so that the accumulators are rescaled once or twice per row, not once per tile.
     if (__any(top > m + kSlack)) {
@@ -295,7 +311,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
     for (int u = 0; u < kSub; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - mu);
+        s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], a.scale2, -mu));
         sum += s[u][r];
       }
     l += sum;
@@ -304,10 +320,15 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const Frag p = to_frag<T>(s[u], t);
-        const int r0 = (SPLIT ? 32 * wave : 32 * u) + 16 * t;
 #pragma unroll
-        for (int dt = 0; dt < kDt; ++dt) acc[dt] = Elem<T>::mma(TL::column(vt, r0, dt, lane), p, acc[dt]);
+        for (int dt = 0; dt < kDt; ++dt) acc[dt] = Elem<T>::mma(TL::column(vt, col_base, (SPLIT ? 32 * wave : 32 * u) + 16 * t, dt), p, acc[dt]);
       }
+    if constexpr (!SPLIT) buffer ^= 1;
+    if (more) {
+      if constexpr (SPLIT) lds_barrier();
+      ks.store(lds + buffer * 2 * kTile, tid);
+      vs.store(lds + buffer * 2 * kTile + kTile, tid);
+    }
   }
   l += __shfl_xor(l, 32, 64);
   if constexpr (SPLIT) {                  // join the four waves: the maxima and sums, then the scaled accumulators
@@ -422,9 +443,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_kv_
   typedef typename Elem<T>::Frag Frag;
   constexpr int kRows = 32, kKc = DP / 16, kDt = DP / 32;
   extern __shared__ __align__(16) char lds[];
-  char *vt = lds, *qt = vt + 128 * TL::kBytes, *dt_ = qt + kRows * TL::kBytes;
-  float *lt = (float *)(dt_ + kRows * TL::kBytes), *et = lt + kRows;          // lse (log2 units) and delta of the rows
+  constexpr int kTile = kRows * TL::kBytes, kBuffer = 2 * kTile + 8 * kRows;   // q, do, lse (log2 units) and delta of the rows; two buffers
+  char *vt = lds, *tiles = lds + 128 * TL::kBytes;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
+  const unsigned row_base = TL::row_base(col, half);
+  const typename TL::ColBase col_base = TL::col_base(lane);
   int tile, group;
   xcd_group_map(blockIdx.x, a.tiles * a.splits, a.B * a.Hk, tile, group);     // causal: the first keys, seen by most rows, first
   const int split = tile % a.splits;
@@ -477,19 +500,27 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_kv_
       if (stat_g >= a.G) { stat_g -= a.G; ++stat_i; }
     }
   };
-  if (begin < rows) load();
+  auto store = [&](char *to) {
+    qs.store(to, tid);
+    ds.store(to + kTile, tid);
+    if (tid < 2 * kRows) ((float *)(to + 2 * kTile))[tid] = stat_next;
+  };
+  if (begin < rows) {
+    load();
+    store(tiles);
+  }
+  int buffer = 0;
   for (int r0 = begin; r0 < rows; r0 += kRows) {
-    lds_barrier();
-    qs.store(qt, tid);
-    ds.store(dt_, tid);
-    if (tid < 2 * kRows) lt[tid] = stat_next;
-    lds_barrier();
-    if (r0 + kRows < rows) load();
+    lds_barrier();                        // this tile is written, the other buffer has been read
+    const char *qt = tiles + buffer * kBuffer, *dt_ = qt + kTile;
+    const float *lt = (const float *)(qt + 2 * kTile), *et = lt + kRows;
+    const bool more = r0 + kRows < rows;
+    if (more) load();
     f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
     for (int kc = 0; kc < kKc; ++kc) {
-      s = Elem<T>::mma(TL::row(qt, col, kc, half), k[kc], s);
-      dp = Elem<T>::mma(TL::row(dt_, col, kc, half), TL::row(vt, 32 * wave + col, kc, half), dp);
+      s = Elem<T>::mma(TL::row(qt, row_base, 0, kc), k[kc], s);
+      dp = Elem<T>::mma(TL::row(dt_, row_base, 0, kc), TL::row(vt, row_base, 32 * wave, kc), dp);
     }
     // some row of the tile does not see some key of the workgroup (or there is no such row)
     const bool edge = r0 + kRows > rows || r0 < all_from;
@@ -513,10 +544,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_kv_
       const Frag p = to_frag<T>(s, t), d = to_frag<T>(dp, t);
 #pragma unroll
       for (int dt = 0; dt < kDt; ++dt) {
-        dv[dt] = Elem<T>::mma(TL::column(dt_, 16 * t, dt, lane), p, dv[dt]);
-        dk[dt] = Elem<T>::mma(TL::column(qt, 16 * t, dt, lane), d, dk[dt]);
+        dv[dt] = Elem<T>::mma(TL::column(dt_, col_base, 16 * t, dt), p, dv[dt]);
+        dk[dt] = Elem<T>::mma(TL::column(qt, col_base, 16 * t, dt), d, dk[dt]);
       }
     }
+    buffer ^= 1;
+    if (more) store(tiles + buffer * kBuffer);
   }
   if (key >= a.Lk) return;
   if (a.splits > 1) {
@@ -536,8 +569,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_q_k
   typedef typename Elem<T>::Frag Frag;
   constexpr int kKeys = 32, kKc = DP / 16, kDt = DP / 32;
   extern __shared__ __align__(16) char lds[];
-  char *kt = lds, *vt = lds + kKeys * TL::kBytes;
+  constexpr int kTile = kKeys * TL::kBytes;                // k, then v; two buffers
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
+  const unsigned row_base = TL::row_base(col, half);
+  const typename TL::ColBase col_base = TL::col_base(lane);
   int tile, group;
   xcd_group_map(blockIdx.x, a.tiles * a.splits, a.B * a.Hk, tile, group);
   const int split = tile % a.splits;
@@ -575,20 +610,22 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_q_k
   vs.start(vh, a.v.r, 0, 1, begin, a.D, tid);
   ks.load(block_end);
   vs.load(block_end);
+  ks.store(lds, tid);
+  vs.store(lds + kTile, tid);
+  int buffer = 0;
   for (int key0 = begin; key0 < block_end; key0 += kKeys) {
     lds_barrier();
-    ks.store(kt, tid);
-    vs.store(vt, tid);
-    lds_barrier();
-    if (key0 + kKeys < block_end) {
+    const char *kt = lds + buffer * 2 * kTile, *vt = kt + kTile;
+    const bool more = key0 + kKeys < block_end;
+    if (more) {
       ks.load(block_end);
       vs.load(block_end);
     }
     f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
     for (int kc = 0; kc < kKc; ++kc) {
-      s = Elem<T>::mma(TL::row(kt, col, kc, half), q[kc], s);
-      dp = Elem<T>::mma(TL::row(vt, col, kc, half), d[kc], dp);
+      s = Elem<T>::mma(TL::row(kt, row_base, 0, kc), q[kc], s);
+      dp = Elem<T>::mma(TL::row(vt, row_base, 0, kc), d[kc], dp);
     }
     const bool edge = key0 + kKeys > min(full_end, block_end) || !all_active;
 #pragma unroll
@@ -601,7 +638,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_q_k
     for (int t = 0; t < 2; ++t) {
       const Frag x = to_frag<T>(dp, t);
 #pragma unroll
-      for (int dt = 0; dt < kDt; ++dt) dq[dt] = Elem<T>::mma(TL::column(kt, 16 * t, dt, lane), x, dq[dt]);
+      for (int dt = 0; dt < kDt; ++dt) dq[dt] = Elem<T>::mma(TL::column(kt, col_base, 16 * t, dt), x, dq[dt]);
+    }
+    buffer ^= 1;
+    if (more) {
+      ks.store(lds + buffer * 2 * kTile, tid);
+      vs.store(lds + buffer * 2 * kTile + kTile, tid);
     }
   }
   if (!inside) return;
@@ -635,7 +677,7 @@ inline hipError_t allow_lds(DeviceOnce &once, const void *kernel, int bytes) {
 template <typename T, int DP> hipError_t attn_forward_dp(AttnArgs a, int narrow, hipStream_t st) {
   const int rows = a.Lq * a.G, kRows = narrow ? 32 : 128, kKeys = narrow ? 128 : 64;
   a.tiles = (rows + kRows - 1) / kRows;
-  const int tile_bytes = 2 * kKeys * Tile<T, DP>::kBytes, join_bytes = narrow ? (4 * 32 * 2 + 4 * 32 * DP) * 4 : 0;
+  const int tile_bytes = (narrow ? 2 : 4) * kKeys * Tile<T, DP>::kBytes, join_bytes = narrow ? (4 * 32 * 2 + 4 * 32 * DP) * 4 : 0;
   const int lds = tile_bytes > join_bytes ? tile_bytes : join_bytes;
   const unsigned grid = (unsigned)a.tiles * a.splits * a.B * a.Hk;
   auto kernel = narrow ? attn_forward_kernel<T, DP, 1> : attn_forward_kernel<T, DP, 0>;
@@ -665,7 +707,7 @@ template <typename T, int DP> hipError_t attn_backward_dp(AttnArgs a, int kv_spl
   constexpr int kBytes = Tile<T, DP>::kBytes;
   if (a.Lk > 0) {
     static DeviceOnce once;
-    const int lds = (128 + 2 * 32) * kBytes + 256;
+    const int lds = (128 + 4 * 32) * kBytes + 512;
     rc = allow_lds(once, (const void *)attn_backward_kv_kernel<T, DP>, lds);
     if (rc != hipSuccess) return rc;
     a.tiles = (a.Lk + 127) / 128;
@@ -678,7 +720,7 @@ template <typename T, int DP> hipError_t attn_backward_dp(AttnArgs a, int kv_spl
   }
   a.tiles = (a.Lq * a.G + 127) / 128;
   a.splits = q_splits;
-  hipLaunchKernelGGL((attn_backward_q_kernel<T, DP>), dim3((unsigned)a.tiles * a.splits * a.B * a.Hk), dim3(256), 2 * 32 * kBytes, st, a);
+  hipLaunchKernelGGL((attn_backward_q_kernel<T, DP>), dim3((unsigned)a.tiles * a.splits * a.B * a.Hk), dim3(256), 4 * 32 * kBytes, st, a);
   rc = hipGetLastError();
   if (rc == hipSuccess && a.splits > 1) rc = launch_sum<T, DP>(a.part_o, a.dq, a, a.Lq * a.G, a.G, st);
   return rc;
