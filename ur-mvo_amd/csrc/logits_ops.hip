@@ -22,13 +22,14 @@ namespace urf {
 
 static_assert(URF_TOP_MAX == 64, "one listed candidate per lane");
 constexpr int kUnroll = 4;               // 16-byte loads in flight per lane
+constexpr double kLog2eDouble = 1.4426950408889634, kLn2Double = 0.6931471805599453;
 constexpr float kFloor = -1.0e4f;        // 2^kFloor is 0: a masked score (-inf) adds 0 * kFloor to A, not 0 * inf
 
 struct RowsArgs {
   const void *z;                 // [R] rows of V scores
   long long stride;              // elements between rows
   int R, V;
-  float c;                       // scale * log2(e)
+  float c, clo;                  // scale * log2(e), and what the float lacks of it
   float scale;                   // 1 / temperature for the distillation
   // log probabilities
   const int *targets; int N;     // [R][N]
@@ -89,8 +90,12 @@ __device__ __forceinline__ Stat wave_join(Stat v) {
 }
 
 // ------------------------------------------------------------------ top alternatives
-// A wave's 64 best so far, descending, one key per lane: the score as an ordered integer above, the complement of its index below
-// (equal scores: the lower index wins).  Every row has its list in registers; a key is 0 where the list is not full yet.
+// The pass over a row only notes, per lane, its largest score and where it was (three instructions per 16 bytes).  The K-th largest
+// of the lanes' best scores bounds the K-th largest of the row from below, so that afterwards only lanes whose best is not below it
+// -- about K of the row's 64, 256 or 1024 -- have their scores read again, cooperatively, and only scores that are not below it
+// are candidates: about K again.  They are sorted 64 at a time.  (Keeping a list during the pass costs more than the pass: 190 us
+// for 2048 rows of 100003 bf16 scores, against 129 us without alternatives.)
+// Keys: the score as an ordered integer above, the complement of its index below (equal scores: the lower index wins); 0 = none.
 typedef unsigned long long u64;
 __device__ __forceinline__ u64 key_of(float z, int index) {
   const unsigned u = __float_as_uint(z + 0.0f);           // -0 counts as 0
@@ -101,41 +106,38 @@ __device__ __forceinline__ float key_score(u64 k) {
   const unsigned o = (unsigned)(k >> 32);
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
-__device__ __forceinline__ u64 shfl64(u64 v, int src) {
-  return ((u64)(unsigned)__shfl((int)(v >> 32), src, 64) << 32) | (unsigned)__shfl((int)(unsigned)v, src, 64);
+// the value of lane ^ x, x a power of two, in the vector pipe (through the LDS crossbar a sort costs four times as much)
+__device__ __forceinline__ int lane_xor(int v, int x, int lane) {
+  switch (x) {
+    case 1: return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, false);
+    case 2: return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, false);
+    case 4: return __builtin_amdgcn_update_dpp(0, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false), 0x1B, 0xf, 0xf, false);   // ^7, then ^3
+    case 8: return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false);
+    case 16: { const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false); return (lane & 16) ? r[0] : r[1]; }
+    default: { const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false); return (lane & 32) ? r[0] : r[1]; }
+  }
 }
-__device__ __forceinline__ u64 exchange(u64 v, int x, bool keep_max) {
-  const u64 o = ((u64)(unsigned)__shfl_xor((int)(v >> 32), x, 64) << 32) | (unsigned)__shfl_xor((int)(unsigned)v, x, 64);
+__device__ __forceinline__ u64 exchange(u64 v, int x, bool keep_max, int lane) {
+  const u64 o = ((u64)(unsigned)lane_xor((int)(v >> 32), x, lane) << 32) | (unsigned)lane_xor((int)(unsigned)v, x, lane);
   return (v > o) == keep_max ? v : o;
 }
 __device__ __forceinline__ u64 sort_desc(u64 v, int lane) {
+#pragma unroll
   for (int n = 2; n <= 64; n <<= 1)
-    for (int x = n >> 1; x >= 1; x >>= 1) v = exchange(v, x, ((lane & n) == 0) == ((lane & x) == 0));
+#pragma unroll
+    for (int x = n >> 1; x >= 1; x >>= 1) v = exchange(v, x, ((lane & n) == 0) == ((lane & x) == 0), lane);
   return v;
+}
+__device__ __forceinline__ u64 shfl64(u64 v, int src) {
+  return ((u64)(unsigned)__shfl((int)(v >> 32), src, 64) << 32) | (unsigned)__shfl((int)(unsigned)v, src, 64);
 }
 // both descending: the 64 largest of the two, descending
 __device__ __forceinline__ u64 merge_desc(u64 a, u64 b, int lane) {
   const u64 r = shfl64(b, 63 - lane);
   u64 v = a > r ? a : r;
-  for (int x = 32; x >= 1; x >>= 1) v = exchange(v, x, (lane & x) == 0);
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) v = exchange(v, x, (lane & x) == 0, lane);
   return v;
-}
-// takes in one candidate per lane (0 = none): a few are inserted one by one, many are sorted and merged, so that no input costs
-// more than one sort per 64 scores
-__device__ __forceinline__ void take(u64 &list, u64 &last, u64 cand, int K, int lane) {
-  u64 pass = __ballot(cand > last);
-  if (__popcll(pass) > 6) {
-    list = merge_desc(list, sort_desc(cand, lane), lane);
-  } else {
-    while (pass) {
-      const u64 c = shfl64(cand, (int)__ffsll((long long)pass) - 1);
-      pass &= pass - 1;
-      const int at = __popcll(__ballot(list > c));
-      const u64 up = shfl64(list, lane > 0 ? lane - 1 : 0);
-      list = lane < at ? list : lane == at ? c : up;
-    }
-  }
-  last = shfl64(list, K - 1);
 }
 
 // ------------------------------------------------------------------ listed candidates
@@ -151,14 +153,23 @@ template <int n> __device__ __forceinline__ void hide_listed(float *f, int first
   }
 }
 
-// One pass of a wave over its share of a row.  TOP: keeps the alternatives; TAIL: leaves the listed candidates out, so that a
-// tail far below them keeps its own maximum.
+// what the pass of a wave over its share of a row leaves in a lane, beside the sums
+struct Share {
+  int b0, b1;        // the share: steps of 64 vectors of 16 bytes
+  float best;        // the lane's largest score (whole vectors), and the first step it was in (-1: the lane has no vector)
+  int best_at;
+  float extra;       // what is left of the row behind the whole vectors: one score a lane of part 0, its index or -1
+  int extra_at;
+};
+
+// One pass of a wave over its share of a row.  TOP: notes the lanes' best scores; TAIL: leaves the listed candidates out, so that a
+// tail far below them keeps its own maximum.  `clo`: what c lacks of scale * log2(e) (fp32 scores only: their gradients are told
+// apart to the last bits; 16-bit scores have none to tell).
 template <typename T, bool ENTROPY, bool TOP, bool TAIL>
-__device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, int parts, int lane, int mine, int K, u64 &list) {
+__device__ __forceinline__ Stat row_pass(const T *z, int V, float c, float clo, int part, int parts, int lane, int mine, Share &sh) {
   typedef Row<T> RW;
   constexpr int kPer = RW::kPer, kStep = 64 * kPer;
   Stat st = {-INFINITY, 0.0f, 0.0f};
-  u64 last = 0;
   auto absorb = [&](const float *f, int n) {
     float top = f[0];
 #pragma unroll
@@ -170,80 +181,140 @@ __device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, i
     st.m = m;
 #pragma unroll
     for (int e = 0; e < n; ++e) {
-      const float x = fmaf(f[e], c, -mu), p = __builtin_amdgcn_exp2f(x);
+      float x = fmaf(f[e], c, -mu);
+      if (sizeof(T) == 4) x = f[e] == -INFINITY ? x : fmaf(f[e], clo, x);
+      const float p = __builtin_amdgcn_exp2f(x);
       st.s += p;
       if (ENTROPY) st.a = fmaf(p, fmaxf(x, kFloor), st.a);
     }
     return top;
   };
-  const int steps = (V / kPer + 63) / 64;                        // of 64 whole vectors; what is left is done by part 0
-  const int b0 = (int)((long long)steps * part / parts), b1 = (int)((long long)steps * (part + 1) / parts);
-  for (int b = b0; b < b1; b += kUnroll) {
+  const int steps = (V / kPer + 63) / 64;
+  sh.b0 = (int)((long long)steps * part / parts);
+  sh.b1 = (int)((long long)steps * (part + 1) / parts);
+  sh.best = -INFINITY;
+  sh.best_at = sh.b0 < sh.b1 && sh.b0 * kStep + (lane + 1) * kPer <= V ? sh.b0 : -1;
+  for (int b = sh.b0; b < sh.b1; b += kUnroll) {
     float f[kUnroll][kPer];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int first = (b + u) * kStep + lane * kPer;
 #pragma unroll
       for (int e = 0; e < kPer; ++e) f[u][e] = -INFINITY;
-      if (b + u < b1 && first + kPer <= V) RW::load(z + first, f[u]);
+      if (b + u < sh.b1 && first + kPer <= V) RW::load(z + first, f[u]);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (b + u < b1) {
+      if (b + u < sh.b1) {
         const int base = (b + u) * kStep, first = base + lane * kPer;
         if (TAIL) {
           const u64 hits = __ballot(mine >= base && mine < base + kStep);
           if (hits) hide_listed<kPer>(f[u], first, mine, hits);
         }
         const float top = absorb(f[u], kPer);
-        if (TOP) {
-          const float least = key_score(last);                   // NaN while the list is not full: everything passes
-          if (__any(!(top < least))) {
-#pragma unroll
-            for (int e = 0; e < kPer; ++e)
-              if (__any(!(f[u][e] < key_score(last)))) take(list, last, first + kPer <= V ? key_of(f[u][e], first + e) : 0, K, lane);
-          }
-        }
+        if (TOP && top > sh.best) { sh.best = top; sh.best_at = b + u; }
       }
   }
-  if (part == 0 && V % kPer) {
-    const int v = V - V % kPer + lane;
-    float f[1] = {-INFINITY};
-    if (v < V) f[0] = (float)z[v];
+  sh.extra = -INFINITY;
+  sh.extra_at = part == 0 && lane < V % kPer ? V - V % kPer + lane : -1;
+  if (V % kPer && part == 0) {
+    if (sh.extra_at >= 0) sh.extra = (float)z[sh.extra_at];
     if (TAIL) {
       const u64 hits = __ballot(mine >= V - V % kPer);
-      if (hits) hide_listed<1>(f, v, mine, hits);
+      if (hits) hide_listed<1>(&sh.extra, V - V % kPer + lane, mine, hits);
     }
-    absorb(f, 1);
-    if (TOP) take(list, last, v < V ? key_of(f[0], v) : 0, K, lane);
+    absorb(&sh.extra, 1);
   }
   return st;
 }
 
-// joins the parts of a row: wave 0 of the row returns with the row's sums and list
-template <int W, bool TOP>
-__device__ __forceinline__ Stat row_join(Stat st, u64 &list, int wave, int lane, char *lds) {
+// The row's 64 largest keys of the waves' sorted lists, in wave 0 and in its part of the LDS (64 keys per wave).
+template <int W> __device__ __forceinline__ u64 lists_join(u64 list, int wave, int lane, u64 *lds) {
+  if constexpr (W > 1) {
+    lds_barrier();
+    lds[wave * 64 + lane] = list;
+    lds_barrier();
+    for (int n = W / 2; n >= 1; n >>= 1) {
+      if (wave < n) {
+        list = merge_desc(list, lds[(wave + n) * 64 + lane], lane);
+        lds[wave * 64 + lane] = list;
+      }
+      lds_barrier();
+    }
+  }
+  return list;
+}
+
+// the alternatives of a row, descending, one key per lane, in wave 0.  LDS: 64 keys per wave to join, 160 of the wave's own
+template <typename T, int W>
+__device__ __forceinline__ u64 top_alternatives(const T *z, int V, int K, const Share &sh, int wave, int lane, u64 *lds, u64 *own_lds) {
+  typedef Row<T> RW;
+  constexpr int kPer = RW::kPer, kStep = 64 * kPer;
+  float f[kPer];
+  u64 best = sh.extra_at >= 0 ? key_of(sh.extra, sh.extra_at) : 0;
+  if (sh.best_at >= 0) {
+    const int first = sh.best_at * kStep + lane * kPer;
+    RW::load(z + first, f);
+    int at = 0;
+#pragma unroll
+    for (int e = kPer - 1; e >= 0; --e)
+      if (f[e] == sh.best) at = e;
+    const u64 k = key_of(sh.best, first + at);
+    best = k > best ? k : best;
+  }
+  u64 list = lists_join<W>(sort_desc(best, lane), wave, lane, lds);
+  u64 bound = shfl64(list, K - 1);
+  if constexpr (W > 1) bound = lds[K - 1];                 // wave 0's list
+  // the winners' scores, (winner, step) pairs spread over the lanes
+  const u64 winners = __ballot(sh.best_at >= 0 && best >= bound);
+  u64 *wait = own_lds;
+  int *who = (int *)(own_lds + 128);
+  if ((winners >> lane) & 1) who[__popcll(winners & ((1ull << lane) - 1))] = lane;
+  __builtin_amdgcn_wave_barrier();
+  list = 0;
+  int count = 0;
+  // takes in a candidate per lane (0 = none); sorts and merges whenever 64 wait, or what there is
+  auto take = [&](u64 key, bool all) {
+    const u64 pass = __ballot(key && key >= bound);
+    if ((pass >> lane) & 1) wait[count + __popcll(pass & ((1ull << lane) - 1))] = key;
+    count += __popcll(pass);
+    while (count >= 64 || (all && count > 0)) {
+      __builtin_amdgcn_wave_barrier();
+      list = merge_desc(list, sort_desc(lane < count ? wait[lane] : 0, lane), lane);
+      const u64 rest = lane + 64 < count ? wait[lane + 64] : 0;
+      __builtin_amdgcn_wave_barrier();
+      wait[lane] = rest;
+      __builtin_amdgcn_wave_barrier();
+      count = max(0, count - 64);
+      const u64 kth = shfl64(list, K - 1);
+      bound = kth > bound ? kth : bound;
+    }
+  };
+  const int ns = sh.b1 - sh.b0, pairs = __popcll(winners) * ns;
+  for (int i0 = 0; i0 < pairs; i0 += 64) {
+    const int i = i0 + lane, w = i / max(ns, 1), first = (sh.b0 + i - w * ns) * kStep + (i < pairs ? who[w] : 0) * kPer;
+    const bool valid = i < pairs && first + kPer <= V;
+    if (valid) RW::load(z + first, f);
+#pragma unroll 1
+    for (int e = 0; e < kPer; ++e) {
+      take(valid ? key_of(f[0], first + e) : 0, false);
+#pragma unroll
+      for (int x = 0; x + 1 < kPer; ++x) f[x] = f[x + 1];
+    }
+  }
+  take(sh.extra_at >= 0 ? key_of(sh.extra, sh.extra_at) : 0, true);
+  return lists_join<W>(list, wave, lane, lds);
+}
+
+// joins the parts of a row, in every wave
+template <int W> __device__ __forceinline__ Stat row_join(Stat st, int wave, int lane, Stat *lds) {
   st = wave_join(st);
   if constexpr (W > 1) {
-    Stat *ss = (Stat *)lds;
-    u64 *ls = (u64 *)(lds + 16 * W);
-    if (lane == 0) ss[wave] = st;
-    if (TOP) ls[wave * 64 + lane] = list;
+    if (lane == 0) lds[wave] = st;
     lds_barrier();
-    if (TOP) {
-      for (int n = W / 2; n >= 1; n >>= 1) {
-        if (wave < n) {
-          list = merge_desc(list, ls[(wave + n) * 64 + lane], lane);
-          ls[wave * 64 + lane] = list;
-        }
-        lds_barrier();
-      }
-    }
-    if (wave == 0) {
-      st = ss[0];
+    st = lds[0];
 #pragma unroll
-      for (int w = 1; w < W; ++w) st = join(st, ss[w]);
-    }
+    for (int w = 1; w < W; ++w) st = join(st, lds[w]);
   }
   return st;
 }
@@ -251,24 +322,28 @@ __device__ __forceinline__ Stat row_join(Stat st, u64 &list, int wave, int lane,
 // ------------------------------------------------------------------ forward kernels
 template <typename T, int W, bool TOP>
 __global__ void __launch_bounds__(W == 16 ? 1024 : 256) log_probs_kernel(RowsArgs a) {
-  __shared__ __align__(16) char lds[W > 1 ? 16 * W + (TOP ? 512 * W : 0) : 16];
+  constexpr int kWaves = W == 16 ? 16 : 4;
+  __shared__ Stat stats[kWaves];
+  __shared__ u64 keys[TOP ? (64 + 160) * kWaves : 1];
   const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6;
   const int r = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (r >= a.R) return;
   const T *z = (const T *)a.z + (long long)r * a.stride;
+  Share sh;
+  Stat st = row_pass<T, true, TOP, false>(z, a.V, a.c, a.clo, wave, W, lane, -1, sh);
+  st = row_join<W>(st, wave, lane, stats);
   u64 list = 0;
-  Stat st = row_pass<T, true, TOP, false>(z, a.V, a.c, wave, W, lane, -1, a.K, list);
-  st = row_join<W, TOP>(st, list, wave, lane, lds);
+  if constexpr (TOP) list = top_alternatives<T, W>(z, a.V, a.K, sh, wave, lane, keys, keys + 64 * kWaves + 160 * (threadIdx.x >> 6));
   if (wave) return;
   // a NaN or +inf score leaves no distribution: everything is NaN and the alternatives are -1.  A row without any score above
   // -inf: lse -inf, entropy 0, every log probability -inf.
   const bool broken = !(st.s >= 0.0f) || st.m == INFINITY, empty = st.m == -INFINITY && !broken;
   const float ls = log2f(st.s), nan = __uint_as_float(0x7fc00000u);
   if (lane == 0) {
-    a.lse[r] = broken ? nan : empty ? -INFINITY : (st.m + ls) * kLn2;
+    a.lse[r] = broken ? nan : empty ? -INFINITY : (float)(((double)st.m + log2((double)st.s)) * kLn2Double);
     a.entropy[r] = broken ? nan : empty ? 0.0f : (ls - st.a / st.s) * kLn2;
   }
-  auto log_prob = [&](float x) { return broken ? nan : empty || x == -INFINITY ? -INFINITY : (fmaf(x, a.c, -st.m) - ls) * kLn2; };
+  auto log_prob = [&](float x) { return broken ? nan : empty || x == -INFINITY ? -INFINITY : (fmaf(x, a.clo, fmaf(x, a.c, -st.m)) - ls) * kLn2; };
   if (lane < a.N) {
     const int t = a.targets[(long long)r * a.N + lane];
     a.log_prob[(long long)r * a.N + lane] = t >= 0 && t < a.V ? log_prob((float)z[t]) : 0.0f;
@@ -280,11 +355,12 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) log_probs_kernel(RowsArg
 }
 
 // the teacher's side of a row: lane k holds alternative k (index -1 where there is none), its probability and log probability
-struct Teacher { int index; float p, lp; float mass, rest; };
+// (in 64 bits: what is left of 1, and of teacher and student where they agree, is a difference)
+struct Teacher { int index; double p, lp, mass, rest; };
 template <bool TAIL>
 __device__ __forceinline__ Teacher teacher_of(const RowsArgs &a, int r, int lane) {
-  Teacher t = {-1, 0.0f, 0.0f, 0.0f, 0.0f};
-  float v = -INFINITY;
+  Teacher t = {-1, 0.0, 0.0, 0.0, 0.0};
+  double v = -INFINITY;
   if (lane < a.K) {
     t.index = a.t_index[(long long)r * a.K + lane];
     if (t.index < 0 || t.index >= a.V) t.index = -1;
@@ -292,36 +368,40 @@ __device__ __forceinline__ Teacher teacher_of(const RowsArgs &a, int r, int lane
   }
   if (TAIL) {
     t.lp = v;
-    const double p = exp((double)v), sum = wave_sum(p);   // 1 - sum cancels: in 64 bits
-    t.p = (float)p;
-    const float rest = (float)fmax(1.0 - sum, 0.0);
-    t.rest = rest < 0x1p-20f ? 0.0f : rest;               // below the rounding of the listed probabilities: there is no rest
-    t.mass = (float)sum + t.rest;
+    t.p = exp(v);
+    const double sum = wave_sum(t.p);
+    t.rest = fmax(1.0 - sum, 0.0);
+    if (t.rest < 0x1p-20) t.rest = 0.0;                   // below the rounding of the listed probabilities: there is no rest
+    t.mass = sum + t.rest;
   } else {
-    v *= a.scale;
-    const float m = wave_max(v), e = m == -INFINITY ? 0.0f : expf(v - m), sum = wave_sum(e);
+    v *= (double)a.scale;
+    const float m = wave_max((float)v);
+    const float e = m == -INFINITY ? 0.0f : expf((float)(v - m)), sum = wave_sum(e);
     t.p = sum == 0.0f ? 0.0f : e / sum;
     t.lp = v - m - logf(sum);
-    t.mass = wave_sum(t.p);
+    t.mass = sum == 0.0f ? 0.0 : sum == sum ? 1.0 : sum;
   }
   return t;
 }
 
 template <typename T, int W, bool TAIL>
 __global__ void __launch_bounds__(W == 16 ? 1024 : 256) distill_kernel(RowsArgs a) {
-  __shared__ __align__(16) char lds[W > 1 ? 16 * W : 16];
+  __shared__ Stat stats[W];
   const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6;
   const int r = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (r >= a.R) return;
   const T *z = (const T *)a.z + (long long)r * a.stride;
   const Teacher t = teacher_of<TAIL>(a, r, lane);
-  u64 none = 0;
-  Stat st = row_pass<T, false, false, TAIL>(z, a.V, a.c, wave, W, lane, t.index, 0, none);
-  st = row_join<W, false>(st, none, wave, lane, lds);
+  Share sh;
+  Stat st = row_pass<T, false, false, TAIL>(z, a.V, a.c, a.clo, wave, W, lane, t.index, sh);
+  st = row_join<W>(st, wave, lane, stats);
   if (wave) return;
+  // What follows is a few operations per row, in 64 bits: a divergence close to zero is a difference of far larger terms.
   const bool used = t.index >= 0;
   const float zk = used ? (float)z[t.index] : -INFINITY;
-  float m = st.m, sum = st.s;                             // of the whole row
+  const double c = (double)a.c + a.clo;
+  float m = st.m;                                         // of the whole row
+  double sum = st.s, listed = 0.0;
   if (TAIL) {
     // the pass left the listed candidates out: add each of them once
     bool first = used;
@@ -330,42 +410,60 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) distill_kernel(RowsArgs 
       if (k < lane && other == t.index) first = false;
     }
     m = fmaxf(m, wave_max(zk * a.c));
-    const float mu = m == -INFINITY ? 0.0f : m;
-    sum = st.s * exp2f(st.m - mu) + wave_sum(first ? exp2f(fmaf(zk, a.c, -mu)) : 0.0f);
+    const double mu = m == -INFINITY ? 0.0 : m;
+    listed = wave_sum(first ? (double)exp2f((float)((double)zk * c - mu)) : 0.0);
+    sum = st.s * exp2f((float)(st.m - mu));
   }
-  const float ls = log2f(sum), nan = __uint_as_float(0x7fc00000u);
-  const bool broken = !(sum >= 0.0f) || m == INFINITY, empty = m == -INFINITY && !broken;
-  const float lq = zk == -INFINITY ? -INFINITY : (fmaf(zk, a.c, -m) - ls) * kLn2;
-  float loss = wave_sum(t.p != 0.0f ? t.p * (t.lp - lq) : 0.0f), tail = 0.0f;
+  const double all = sum + listed;
+  // the logarithms, each in a lane of its own: of the sum, of the unlisted share of it, of the teacher's rest.  Where the unlisted
+  // share is too small for the sum's scale, its own maximum counts.
+  const bool far = TAIL && sum < 0x1p-100 * all;
+  const double logs = log(lane == 0 ? all : lane == 1 ? (far ? (double)st.s : listed < sum ? 1.0 - listed / all : sum / all) : t.rest);
+  const double log_all = __shfl(logs, 0, 64), lse = m * kLn2Double + log_all;
+  const float nan = __uint_as_float(0x7fc00000u);
+  const bool broken = !(all >= 0.0) || m == INFINITY, empty = m == -INFINITY && !broken;
+  const double lq = zk == -INFINITY ? -INFINITY : ((double)zk * c - m) * kLn2Double - log_all;
+  double loss = wave_sum(t.p != 0.0 ? t.p * (t.lp - lq) : 0.0), tail = 0.0;
   if (TAIL) {
-    tail = (st.m + log2f(st.s) - m - ls) * kLn2;          // log of the student's probability of everything unlisted
-    if (t.rest > 0.0f) loss += t.rest * (logf(t.rest) - tail);
+    // log of the student's probability of everything unlisted
+    tail = __shfl(logs, 1, 64);
+    if (far) tail += (st.m - (double)m) * kLn2Double - log_all;
+    if (t.rest > 0.0) loss += t.rest * (__shfl(logs, 2, 64) - tail);
   }
-  if (empty) loss = t.mass != 0.0f ? INFINITY : 0.0f;     // the student allows nothing
+  if (empty) loss = t.mass != 0.0 ? INFINITY : 0.0;       // the student allows nothing
   if (lane == 0) {
-    a.loss[r] = broken ? nan : loss;
-    a.lse[r] = broken ? nan : empty ? -INFINITY : (m + ls) * kLn2;
-    if (TAIL) a.log_tail[r] = broken ? nan : empty ? -INFINITY : tail;
+    a.loss[r] = broken ? nan : (float)loss;
+    a.lse[r] = broken ? nan : empty ? -INFINITY : (float)lse;
+    if (TAIL) a.log_tail[r] = broken ? nan : empty ? -INFINITY : (float)tail;
   }
 }
 
 // ------------------------------------------------------------------ gradients
 // dz = coefficient * 2^(x - shift) [ * (1 + ...) ] + what the listed candidates add; one read, one write per score
 struct GradRow {
-  float shift;       // log2 units: of lse (or of lse and the tail's probability)
+  float shift, slo;  // log2 units: of lse (or of lse and the tail's probability), and what the float lacks (fp32 scores)
   float coef;        // of the probability
   float h, ent2;     // ENTROPY: -h p (log2 p + ent2), in log2 units
-  float lshift, lcoef;   // TAIL: of a listed candidate's probability
+  float lshift, lslo, lcoef;   // TAIL: of a listed candidate's probability
   int mine;          // this lane's listed index (-1: none) and what it adds
   float add;
 };
 
+__device__ __forceinline__ void set_shift(float &hi, float &lo, double shift) {
+  hi = (float)shift;
+  lo = (float)(shift - (double)hi);
+}
+
 template <typename T, bool ENTROPY, bool TAIL>
-__device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float c, const GradRow &g, int part, int parts, int lane) {
+__device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float c, float clo, const GradRow &g, int part, int parts, int lane) {
   typedef Row<T> RW;
   constexpr int kPer = RW::kPer, kStep = 64 * kPer;
+  auto exponent = [&](float f, float shift, float slo) {
+    const float x = fmaf(f, c, -shift);
+    return sizeof(T) == 4 && f != -INFINITY ? x + fmaf(f, clo, -slo) : x;
+  };
   auto grad = [&](float f) {
-    const float x = fmaf(f, c, -g.shift), p = __builtin_amdgcn_exp2f(x);
+    const float x = exponent(f, g.shift, g.slo), p = __builtin_amdgcn_exp2f(x);
     if (ENTROPY) return p * fmaf(-g.h, fmaxf(x, kFloor) + g.ent2, g.coef);
     return p * g.coef;
   };
@@ -376,7 +474,7 @@ __device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float c, con
         const int at = __shfl(g.mine, (int)__ffsll((long long)h) - 1, 64) - first;
 #pragma unroll
         for (int e = 0; e < n; ++e)
-          if (e == at) d[e] = g.lcoef * __builtin_amdgcn_exp2f(fmaf(f[e], c, -g.lshift));
+          if (e == at) d[e] = g.lcoef * __builtin_amdgcn_exp2f(exponent(f[e], g.lshift, g.lslo));
       }
     for (u64 h = hits; h; h &= h - 1) {                    // what each mention adds, in the list's order
       const int src = (int)__ffsll((long long)h) - 1, at = __shfl(g.mine, src, 64) - first;
@@ -439,13 +537,13 @@ __global__ void __launch_bounds__(256) log_probs_backward_kernel(RowsArgs a) {
     else own = a.g1[(long long)r * a.N + lane];
   }
   g.add = own * a.scale;
-  g.shift = empty ? 0.0f : lse * kLog2e;
+  set_shift(g.shift, g.slo, empty ? 0.0 : lse * kLog2eDouble);
   g.coef = empty ? 0.0f : -wave_sum(own) * a.scale;
   if (ENTROPY && !empty) {
     g.h = a.g2[r] * a.scale * kLn2;
     g.ent2 = a.entropy[r] * kLog2e;
   }
-  grad_pass<T, ENTROPY, false>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.c, g, part, a.per_row, lane);
+  grad_pass<T, ENTROPY, false>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.c, a.clo, g, part, a.per_row, lane);
 }
 
 template <typename T, bool TAIL>
@@ -455,25 +553,27 @@ __global__ void __launch_bounds__(256) distill_backward_kernel(RowsArgs a) {
   const int r = (int)(w / a.per_row), part = (int)(w % a.per_row);
   if (r >= a.R) return;
   const Teacher t = teacher_of<TAIL>(a, r, lane);
-  const float lse = a.lse[r], gs = a.g1[r] * a.scale;
+  const float lse = a.lse[r];
+  const double gs = (double)a.g1[r] * a.scale;
   const bool empty = lse == -INFINITY;
   GradRow g = {};
   g.mine = empty ? -1 : t.index;
-  g.add = -gs * t.p;
-  g.shift = empty ? 0.0f : lse * kLog2e;
-  g.coef = empty ? 0.0f : gs * t.mass;
+  g.add = (float)(-gs * t.p);
+  set_shift(g.shift, g.slo, empty ? 0.0 : lse * kLog2eDouble);
+  g.coef = empty ? 0.0f : (float)(gs * t.mass);
   if (TAIL) {
     g.lshift = g.shift;
+    g.lslo = g.slo;
     g.lcoef = g.coef;
     // unlisted v: mass q_v - rest q_v / q_tail = (mass q_tail - rest) 2^(x - shift) with the tail's probability in the shift,
     // a probability within the tail: nothing overflows however small q_tail is
     const float tail = a.log_tail[r];
     if (!empty && tail != -INFINITY) {
-      g.shift += tail * kLog2e;
-      g.coef = gs * (t.mass * expf(tail) - t.rest);
+      set_shift(g.shift, g.slo, ((double)lse + tail) * kLog2eDouble);
+      g.coef = (float)(gs * (t.mass * expf(tail) - t.rest));
     }
   }
-  grad_pass<T, false, TAIL>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.c, g, part, a.per_row, lane);
+  grad_pass<T, false, TAIL>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.c, a.clo, g, part, a.per_row, lane);
 }
 
 // ------------------------------------------------------------------ launches
@@ -558,7 +658,8 @@ RowsArgs rows_of(const urf_rows_config *c, const void *logits) {
   a.R = c->rows;
   a.V = c->classes;
   a.scale = c->scale;
-  a.c = (float)((double)c->scale * 1.4426950408889634);
+  a.c = (float)((double)c->scale * kLog2eDouble);
+  a.clo = (float)((double)c->scale * kLog2eDouble - (double)a.c);
   return a;
 }
 
