@@ -49,26 +49,54 @@ struct RowsArgs {
 template <typename T> struct Row {
   static constexpr int kPer = 16 / (int)sizeof(T);
   typedef T Vec __attribute__((ext_vector_type(kPer), aligned(sizeof(T))));
-  static __device__ __forceinline__ void load(const T *p, float (&f)[kPer]) {
-    const Vec v = *(const Vec *)p;
+  static __device__ __forceinline__ void load(const T *p, float (&f)[kPer]) { spread(*(const Vec *)p, f); }
+  static __device__ __forceinline__ void spread(const Vec &v, float (&f)[kPer]) {
 #pragma unroll
     for (int e = 0; e < kPer; ++e) f[e] = (float)v[e];
   }
+  // kUnroll steps from step b on: the whole vectors below `end` steps and V scores; the others are -inf
+  static __device__ __forceinline__ void fetch(const T *z, int b, int end, int V, int lane, Vec (&v)[kUnroll]) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int first = (b + u) * 64 * kPer + lane * kPer;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) v[u][e] = (T)-INFINITY;
+      if (b + u < end && first + kPer <= V) v[u] = *(const Vec *)(z + first);
+    }
+  }
 };
+
+// the value of lane ^ x, x a power of two, in the vector pipe (the LDS crossbar's latency is several times that)
+__device__ __forceinline__ int lane_xor(int v, int x) {
+  const int lane = threadIdx.x;
+  switch (x) {
+    case 1: return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, false);
+    case 2: return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, false);
+    case 4: return __builtin_amdgcn_update_dpp(0, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false), 0x1B, 0xf, 0xf, false);   // ^7, then ^3
+    case 8: return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false);
+    case 16: { const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false); return (lane & 16) ? r[0] : r[1]; }
+    default: { const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false); return (lane & 32) ? r[0] : r[1]; }
+  }
+}
+__device__ __forceinline__ float lane_xor(float v, int x) { return __int_as_float(lane_xor(__float_as_int(v), x)); }
+__device__ __forceinline__ double lane_xor(double v, int x) {
+  const long long u = __double_as_longlong(v);
+  return __longlong_as_double(((long long)lane_xor((int)(u >> 32), x) << 32) | (unsigned)lane_xor((int)u, x));
+}
 
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) v = fmaxf(v, __shfl_xor(v, x, 64));
+  for (int x = 32; x >= 1; x >>= 1) v = fmaxf(v, lane_xor(v, x));
   return v;
 }
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) v += __shfl_xor(v, x, 64);
+  for (int x = 32; x >= 1; x >>= 1) v += lane_xor(v, x);
   return v;
 }
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) v += __shfl_xor(v, x, 64);
+  for (int x = 32; x >= 1; x >>= 1) v += lane_xor(v, x);
   return v;
 }
 
@@ -83,7 +111,7 @@ __device__ __forceinline__ Stat join(Stat p, Stat q) {
 __device__ __forceinline__ Stat wave_join(Stat v) {
 #pragma unroll
   for (int x = 32; x >= 1; x >>= 1) {
-    const Stat o = {__shfl_xor(v.m, x, 64), __shfl_xor(v.s, x, 64), __shfl_xor(v.a, x, 64)};
+    const Stat o = {lane_xor(v.m, x), lane_xor(v.s, x), lane_xor(v.a, x)};
     v = (threadIdx.x & x) ? join(o, v) : join(v, o);      // the same operand order on both sides: the same bits in every lane
   }
   return v;
@@ -106,26 +134,15 @@ __device__ __forceinline__ float key_score(u64 k) {
   const unsigned o = (unsigned)(k >> 32);
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
-// the value of lane ^ x, x a power of two, in the vector pipe (through the LDS crossbar a sort costs four times as much)
-__device__ __forceinline__ int lane_xor(int v, int x, int lane) {
-  switch (x) {
-    case 1: return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, false);
-    case 2: return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, false);
-    case 4: return __builtin_amdgcn_update_dpp(0, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false), 0x1B, 0xf, 0xf, false);   // ^7, then ^3
-    case 8: return __builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false);
-    case 16: { const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false); return (lane & 16) ? r[0] : r[1]; }
-    default: { const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false); return (lane & 32) ? r[0] : r[1]; }
-  }
-}
-__device__ __forceinline__ u64 exchange(u64 v, int x, bool keep_max, int lane) {
-  const u64 o = ((u64)(unsigned)lane_xor((int)(v >> 32), x, lane) << 32) | (unsigned)lane_xor((int)(unsigned)v, x, lane);
+__device__ __forceinline__ u64 exchange(u64 v, int x, bool keep_max) {
+  const u64 o = ((u64)(unsigned)lane_xor((int)(v >> 32), x) << 32) | (unsigned)lane_xor((int)(unsigned)v, x);
   return (v > o) == keep_max ? v : o;
 }
 __device__ __forceinline__ u64 sort_desc(u64 v, int lane) {
 #pragma unroll
   for (int n = 2; n <= 64; n <<= 1)
 #pragma unroll
-    for (int x = n >> 1; x >= 1; x >>= 1) v = exchange(v, x, ((lane & n) == 0) == ((lane & x) == 0), lane);
+    for (int x = n >> 1; x >= 1; x >>= 1) v = exchange(v, x, ((lane & n) == 0) == ((lane & x) == 0));
   return v;
 }
 __device__ __forceinline__ u64 shfl64(u64 v, int src) {
@@ -136,7 +153,7 @@ __device__ __forceinline__ u64 merge_desc(u64 a, u64 b, int lane) {
   const u64 r = shfl64(b, 63 - lane);
   u64 v = a > r ? a : r;
 #pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) v = exchange(v, x, (lane & x) == 0, lane);
+  for (int x = 32; x >= 1; x >>= 1) v = exchange(v, x, (lane & x) == 0);
   return v;
 }
 
@@ -165,8 +182,8 @@ struct Share {
 // One pass of a wave over its share of a row.  TOP: notes the lanes' best scores; TAIL: leaves the listed candidates out, so that a
 // tail far below them keeps its own maximum.  `clo`: what c lacks of scale * log2(e) (fp32 scores only: their gradients are told
 // apart to the last bits; 16-bit scores have none to tell).
-template <typename T, bool ENTROPY, bool TOP, bool TAIL>
-__device__ __forceinline__ Stat row_pass(const T *z, int V, float c, float clo, int part, int parts, int lane, int mine, Share &sh) {
+template <typename T, int W, bool ENTROPY, bool TOP, bool TAIL>
+__device__ __forceinline__ Stat row_pass(const T *z, int V, float c, float clo, int part, int lane, int mine, Share &sh) {
   typedef Row<T> RW;
   constexpr int kPer = RW::kPer, kStep = 64 * kPer;
   Stat st = {-INFINITY, 0.0f, 0.0f};
@@ -190,23 +207,22 @@ __device__ __forceinline__ Stat row_pass(const T *z, int V, float c, float clo, 
     return top;
   };
   const int steps = (V / kPer + 63) / 64;
-  sh.b0 = (int)((long long)steps * part / parts);
-  sh.b1 = (int)((long long)steps * (part + 1) / parts);
+  sh.b0 = (int)((long long)steps * part / W);
+  sh.b1 = (int)((long long)steps * (part + 1) / W);
   sh.best = -INFINITY;
   sh.best_at = sh.b0 < sh.b1 && sh.b0 * kStep + (lane + 1) * kPer <= V ? sh.b0 : -1;
+  typename RW::Vec now[kUnroll], next[kUnroll];
+  if (W > 1) RW::fetch(z, sh.b0, sh.b1, V, lane, now);
   for (int b = sh.b0; b < sh.b1; b += kUnroll) {
+    // long rows: the next scores are in flight while these are taken in; short ones are one or two steps
+    if (W > 1) RW::fetch(z, b + kUnroll, sh.b1, V, lane, next);
+    else RW::fetch(z, b, sh.b1, V, lane, now);
     float f[kUnroll][kPer];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int first = (b + u) * kStep + lane * kPer;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) f[u][e] = -INFINITY;
-      if (b + u < sh.b1 && first + kPer <= V) RW::load(z + first, f[u]);
-    }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
       if (b + u < sh.b1) {
         const int base = (b + u) * kStep, first = base + lane * kPer;
+        RW::spread(now[u], f[u]);
         if (TAIL) {
           const u64 hits = __ballot(mine >= base && mine < base + kStep);
           if (hits) hide_listed<kPer>(f[u], first, mine, hits);
@@ -214,6 +230,9 @@ __device__ __forceinline__ Stat row_pass(const T *z, int V, float c, float clo, 
         const float top = absorb(f[u], kPer);
         if (TOP && top > sh.best) { sh.best = top; sh.best_at = b + u; }
       }
+    if (W > 1)
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) now[u] = next[u];
   }
   sh.extra = -INFINITY;
   sh.extra_at = part == 0 && lane < V % kPer ? V - V % kPer + lane : -1;
@@ -330,7 +349,7 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) log_probs_kernel(RowsArg
   if (r >= a.R) return;
   const T *z = (const T *)a.z + (long long)r * a.stride;
   Share sh;
-  Stat st = row_pass<T, true, TOP, false>(z, a.V, a.c, a.clo, wave, W, lane, -1, sh);
+  Stat st = row_pass<T, W, true, TOP, false>(z, a.V, a.c, a.clo, wave, lane, -1, sh);
   st = row_join<W>(st, wave, lane, stats);
   u64 list = 0;
   if constexpr (TOP) list = top_alternatives<T, W>(z, a.V, a.K, sh, wave, lane, keys, keys + 64 * kWaves + 160 * (threadIdx.x >> 6));
@@ -393,7 +412,7 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) distill_kernel(RowsArgs 
   const T *z = (const T *)a.z + (long long)r * a.stride;
   const Teacher t = teacher_of<TAIL>(a, r, lane);
   Share sh;
-  Stat st = row_pass<T, false, false, TAIL>(z, a.V, a.c, a.clo, wave, W, lane, t.index, sh);
+  Stat st = row_pass<T, W, false, false, TAIL>(z, a.V, a.c, a.clo, wave, lane, t.index, sh);
   st = row_join<W>(st, wave, lane, stats);
   if (wave) return;
   // What follows is a few operations per row, in 64 bits: a divergence close to zero is a difference of far larger terms.
@@ -454,7 +473,8 @@ __device__ __forceinline__ void set_shift(float &hi, float &lo, double shift) {
   lo = (float)(shift - (double)hi);
 }
 
-template <typename T, bool ENTROPY, bool TAIL>
+// STREAM: written past the caches (a template: the compiler joins two stores that differ in this only)
+template <typename T, bool ENTROPY, bool TAIL, bool STREAM>
 __device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float c, float clo, const GradRow &g, int part, int parts, int lane) {
   typedef Row<T> RW;
   constexpr int kPer = RW::kPer, kStep = 64 * kPer;
@@ -506,7 +526,8 @@ __device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float c, flo
           typename RW::Vec o;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) o[e] = (T)d[e];
-          *(typename RW::Vec *)(dz + first) = o;
+          if constexpr (STREAM) __builtin_nontemporal_store(o, (typename RW::Vec *)(dz + first));
+          else *(typename RW::Vec *)(dz + first) = o;
         }
       }
   }
@@ -520,12 +541,12 @@ __device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float c, flo
   }
 }
 
-template <typename T, bool ENTROPY>
+template <typename T, bool ENTROPY, bool STREAM>
 __global__ void __launch_bounds__(256) log_probs_backward_kernel(RowsArgs a) {
   const int lane = threadIdx.x & 63;
   const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int r = (int)(w / a.per_row), part = (int)(w % a.per_row);
-  if (r >= a.R) return;
+  const int r = a.R - 1 - (int)(w / a.per_row), part = (int)(w % a.per_row);      // the last rows, read last by the forward pass, first
+  if (r < 0) return;
   const float lse = a.lse[r];
   const bool empty = lse == -INFINITY;                    // no score to choose from: constant outputs, no gradient
   GradRow g = {};
@@ -543,15 +564,15 @@ __global__ void __launch_bounds__(256) log_probs_backward_kernel(RowsArgs a) {
     g.h = a.g2[r] * a.scale * kLn2;
     g.ent2 = a.entropy[r] * kLog2e;
   }
-  grad_pass<T, ENTROPY, false>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.c, a.clo, g, part, a.per_row, lane);
+  grad_pass<T, ENTROPY, false, STREAM>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.c, a.clo, g, part, a.per_row, lane);
 }
 
-template <typename T, bool TAIL>
+template <typename T, bool TAIL, bool STREAM>
 __global__ void __launch_bounds__(256) distill_backward_kernel(RowsArgs a) {
   const int lane = threadIdx.x & 63;
   const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int r = (int)(w / a.per_row), part = (int)(w % a.per_row);
-  if (r >= a.R) return;
+  const int r = a.R - 1 - (int)(w / a.per_row), part = (int)(w % a.per_row);      // the last rows, read last by the forward pass, first
+  if (r < 0) return;
   const Teacher t = teacher_of<TAIL>(a, r, lane);
   const float lse = a.lse[r];
   const double gs = (double)a.g1[r] * a.scale;
@@ -573,7 +594,7 @@ __global__ void __launch_bounds__(256) distill_backward_kernel(RowsArgs a) {
       g.coef = (float)(gs * (t.mass * expf(tail) - t.rest));
     }
   }
-  grad_pass<T, false, TAIL>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.c, a.clo, g, part, a.per_row, lane);
+  grad_pass<T, false, TAIL, STREAM>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.c, a.clo, g, part, a.per_row, lane);
 }
 
 // ------------------------------------------------------------------ launches
@@ -585,6 +606,10 @@ inline int grad_waves(int R, int V, int bytes) {
   const long long fill = (4096 + R - 1) / R, n = by_size > fill ? by_size : fill;
   return (int)(n < 1 || steps < 1 ? 1 : n > steps ? steps : n);
 }
+
+// A gradient beyond half of the 256 MB of the last-level cache is written past it: left there, its lines are written back while the
+// next pass over scores reads, which then takes 130 us instead of 100 (2048 rows of 131072 bf16 scores; 538 MB).
+inline bool streams(const RowsArgs &a, int bytes) { return (long long)a.R * a.V * bytes > (128ll << 20); }
 
 template <typename T> hipError_t launch_log_probs(const RowsArgs &a, hipStream_t st) {
   const int W = row_waves(a.R, a.V);
@@ -606,15 +631,19 @@ template <typename T> hipError_t launch_distill(const RowsArgs &a, bool tail, hi
 }
 template <typename T> hipError_t launch_log_probs_backward(RowsArgs a, hipStream_t st) {
   a.per_row = grad_waves(a.R, a.V, sizeof(T));
+  const bool far = streams(a, sizeof(T));
   const dim3 grid((unsigned)(((long long)a.R * a.per_row + 3) / 4));
-  auto kernel = a.g2 ? log_probs_backward_kernel<T, true> : log_probs_backward_kernel<T, false>;
+  auto kernel = a.g2 ? (far ? log_probs_backward_kernel<T, true, true> : log_probs_backward_kernel<T, true, false>)
+                     : (far ? log_probs_backward_kernel<T, false, true> : log_probs_backward_kernel<T, false, false>);
   hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 template <typename T> hipError_t launch_distill_backward(RowsArgs a, bool tail, hipStream_t st) {
   a.per_row = grad_waves(a.R, a.V, sizeof(T));
+  const bool far = streams(a, sizeof(T));
   const dim3 grid((unsigned)(((long long)a.R * a.per_row + 3) / 4));
-  auto kernel = tail ? distill_backward_kernel<T, true> : distill_backward_kernel<T, false>;
+  auto kernel = tail ? (far ? distill_backward_kernel<T, true, true> : distill_backward_kernel<T, true, false>)
+                     : (far ? distill_backward_kernel<T, false, true> : distill_backward_kernel<T, false, false>);
   hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
