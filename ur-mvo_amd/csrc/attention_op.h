@@ -82,6 +82,7 @@ template <typename T, int DP> struct Tile {
   static __device__ __forceinline__ unsigned row_base(int r, int half) {
     return r * kBytes + (((sizeof(T) == 2 ? half : 2 * half) ^ swizzle(r)) << 4);
   }
+  // (`base` may include an offset into LDS that is a multiple of 512 bytes; `tile` + r0 rows should be constant)
   static __device__ __forceinline__ typename Elem<T>::Frag row(const char *tile, unsigned base, int r0, int kc) {
     const char *p = tile + r0 * kBytes;
     if constexpr (sizeof(T) == 2) {
@@ -97,7 +98,10 @@ template <typename T, int DP> struct Tile {
   // Column 32 dt + l % 32 of rows r0 + {4 half + 0..3, 8 + 4 half + 0..3}, r0 a multiple of 16: the left operand of a product over
   // rows.  16-bit types: the 16 lanes of a group read four rows of 16 elements, four elements a lane, and get one column of four
   // rows each.
-  struct ColBase { unsigned a, b; };
+  struct ColBase {
+    unsigned a, b;
+    __device__ __forceinline__ ColBase operator+(unsigned off) const { return {a + off, b + off}; }
+  };
   static __device__ __forceinline__ ColBase col_base(int lane) {
     const int half = lane >> 5;
     if constexpr (sizeof(T) == 2) {
@@ -156,18 +160,19 @@ template <typename T, int DP, int R> struct Stage {
       p[n] = head + (long long)i * srow + (long long)g[n] * shead + c * TL::kPer;
     }
   }
-  __device__ __forceinline__ void load(int end) {
+  // DOWN: the tiles are walked towards the first row
+  template <bool DOWN = false> __device__ __forceinline__ void load(int end) {
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       x[n] = u32x4{0, 0, 0, 0};
       if (inner && row + 256 / TL::kChunks * n < end) x[n] = *(const u32x4 *)p[n];
-      p[n] += step;
+      p[n] += DOWN ? -step : step;
       if (group > 1) {
-        g[n] += R % group;
-        if (g[n] >= group) { g[n] -= group; p[n] += wrap; }
+        g[n] += DOWN ? -(R % group) : R % group;
+        if (DOWN ? g[n] < 0 : g[n] >= group) { g[n] += DOWN ? group : -group; p[n] += DOWN ? -wrap : wrap; }
       }
     }
-    row += R;
+    row += DOWN ? -R : R;
   }
   __device__ __forceinline__ void store(char *tile, int tid) const {
     char *p = TL::at(tile, tid / TL::kChunks, tid % TL::kChunks);
@@ -208,6 +213,9 @@ template <typename T, int DP> __device__ __forceinline__ void store_rows(T *p, c
     }
 }
 
+// in a branch: keeps the compiler from turning the branch into selects that every tile pays for
+__device__ __forceinline__ void stay_a_branch() { asm volatile(""); }
+
 __device__ __forceinline__ int clamp_len(const int *lens, int b, int most) {
   return lens ? min(max(lens[b], 0), most) : most;      // lengths come from device memory: never trusted beyond the tensor
 }
@@ -225,8 +233,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
   extern __shared__ __align__(16) char lds[];
   constexpr int kTile = kKeys * TL::kBytes;                // k, then v; SPLIT = 0: two buffers, one barrier per tile
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
-  const unsigned row_base = TL::row_base(col, half);
-  const typename TL::ColBase col_base = TL::col_base(lane);
+  const unsigned wave_rows = SPLIT ? 32 * wave * TL::kBytes : 0;       // SPLIT: the wave's own keys of a tile
+  const unsigned row_base = TL::row_base(col, half) + wave_rows;
+  const typename TL::ColBase col_base = TL::col_base(lane) + wave_rows;
   int tile, group;
   xcd_group_map(blockIdx.x, a.tiles * a.splits, a.B * a.Hk, tile, group);
   const int split = tile % a.splits;
@@ -267,7 +276,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
   int buffer = 0;
   for (int key0 = begin; key0 < block_end; key0 += kKeys) {
     lds_barrier();                        // this tile is written, the other buffer (if any) has been read
-    const char *kt = lds + buffer * 2 * kTile, *vt = kt + kTile;
+    const unsigned at = buffer * 2 * kTile;
     const bool more = key0 + kKeys < block_end;
     if (more) {
       ks.load(block_end);
@@ -278,9 +287,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
     for (int u = 0; u < kSub; ++u) {
       s[u] = f32x16{};
 #pragma unroll
-      for (int kc = 0; kc < kKc; ++kc) s[u] = Elem<T>::mma(TL::row(kt, row_base, SPLIT ? 32 * wave : 32 * u, kc), q[kc], s[u]);
+      for (int kc = 0; kc < kKc; ++kc) s[u] = Elem<T>::mma(TL::row(lds, row_base + at, 32 * u, kc), q[kc], s[u]);
     }
     if (key0 + kKeys > min(full_end, block_end) || !all_active) {
+      stay_a_branch();
       const int end = min(seen, block_end);
 #pragma unroll
       for (int u = 0; u < kSub; ++u) {
@@ -321,7 +331,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
       for (int t = 0; t < 2; ++t) {
         const Frag p = to_frag<T>(s[u], t);
 #pragma unroll
-        for (int dt = 0; dt < kDt; ++dt) acc[dt] = Elem<T>::mma(TL::column(vt, col_base, (SPLIT ? 32 * wave : 32 * u) + 16 * t, dt), p, acc[dt]);
+        for (int dt = 0; dt < kDt; ++dt) acc[dt] = Elem<T>::mma(TL::column(lds + kTile, col_base + at, 32 * u + 16 * t, dt), p, acc[dt]);
       }
     if constexpr (!SPLIT) buffer ^= 1;
     if (more) {
@@ -434,124 +444,134 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a) {
   if (inside && c == 0) a.delta[((long long)b * a.Hq + h) * a.Lq + i] = s;
 }
 
-// dk and dv of 128 keys, 32 per wave; walks the query rows in tiles of 32 (or one of `splits` equal ranges of them).  k stays in
-// registers, v in LDS: with both in registers the accumulators leave room for one wave per SIMD only, and nothing runs beside its
-// waits.
+// dk and dv of 128 keys, 32 per wave.  k stays in registers, v in LDS: with both in registers the accumulators leave room for one
+// wave per SIMD only, and nothing runs beside its waits.  The query rows, cut in `splits` ranges of whole tiles of 32, are walked
+// from the last one down, range by range over all key tiles: the workgroups that run together read the same rows at about the same
+// time, and the first of them brings a row into the XCD's L2 for the others, causal or not.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_kv_kernel(AttnArgs a) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::Frag Frag;
   constexpr int kRows = 32, kKc = DP / 16, kDt = DP / 32;
   extern __shared__ __align__(16) char lds[];
-  constexpr int kTile = kRows * TL::kBytes, kBuffer = 2 * kTile + 8 * kRows;   // q, do, lse (log2 units) and delta of the rows; two buffers
-  char *vt = lds, *tiles = lds + 128 * TL::kBytes;
+  constexpr int kTile = kRows * TL::kBytes, kBuffer = 2 * kTile + 512;         // q, do, lse (log2 units) and delta of the rows; two buffers
+  char *const vt = lds + 2 * kBuffer;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
-  const unsigned row_base = TL::row_base(col, half);
+  const unsigned row_base = TL::row_base(col, half), v_base = row_base + 32 * wave * TL::kBytes;
   const typename TL::ColBase col_base = TL::col_base(lane);
   int tile, group;
-  xcd_group_map(blockIdx.x, a.tiles * a.splits, a.B * a.Hk, tile, group);     // causal: the first keys, seen by most rows, first
-  const int split = tile % a.splits;
-  tile /= a.splits;
+  xcd_group_map(blockIdx.x, a.tiles * a.splits, a.B * a.Hk, tile, group);
+  const int split = tile / a.tiles;                                           // 0: the last rows
+  tile -= split * a.tiles;
   const int b = group / a.Hk, hk = group % a.Hk;
   const int nq = clamp_len(a.q_lens, b, a.Lq), nk = clamp_len(a.k_lens, b, a.Lk);
   const int key = tile * 128 + 32 * wave + col;
-  const T *krow = (const T *)a.k.p + (long long)b * a.k.b + (long long)key * a.k.r + (long long)hk * a.k.h;
-  Frag k[kKc];
-#pragma unroll
-  for (int kc = 0; kc < kKc; ++kc) k[kc] = load_frag<T>(krow, key < nk, kc, half, a.D);
+  // rows [begin, rows) see some key of the workgroup; causal: key j is seen by i >= j - (nk - nq), which is row >= first_row, and
+  // from row `diagonal` on every row sees every key
+  int rows = tile * 128 < nk ? nq * a.G : 0;
+  const int first_row = a.causal ? min(nq, max(0, key - (nk - nq))) * a.G : 0;
+  const int i_min = a.causal ? min(nq, max(0, tile * 128 - (nk - nq))) : 0, diagonal = a.causal ? min(nq, max(0, tile * 128 + 127 - (nk - nq))) * a.G : 0;
+  int begin = min(i_min * a.G, rows) / kRows * kRows;
   {
-    Stage<T, DP, 32> vs;
-    vs.start((const T *)a.v.p + (long long)b * a.v.b + (long long)hk * a.v.h, a.v.r, 0, 1, tile * 128, a.D, tid);
-    for (int n = 0; n < 4; ++n) {
-      vs.load(nk);
-      vs.store(vt + n * 32 * TL::kBytes, tid);
-    }
+    const int t = (nq * a.G + kRows - 1) / kRows, per = (t + a.splits - 1) / a.splits * kRows, from = (t * kRows) - (split + 1) * per;
+    begin = max(begin, from);
+    rows = min(rows, from + per);
   }
   f32x16 dk[kDt], dv[kDt];
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt) dk[dt] = dv[dt] = f32x16{};
-  // rows [begin, rows) see some key of the workgroup; causal: key j is seen by i >= j - (nk - nq), which is row >= first_row
-  int rows = tile * 128 < nk ? nq * a.G : 0;
-  const int seen_by = a.causal ? max(0, key - (nk - nq)) : 0, first_row = key < nk && seen_by < nq ? seen_by * a.G : rows;
-  const int i_min = a.causal ? min(nq, max(0, tile * 128 - (nk - nq))) : 0, i_all = a.causal ? max(0, tile * 128 + 127 - (nk - nq)) : 0;
-  const long long all_from = tile * 128 + 128 <= nk ? (long long)i_all * a.G : rows;    // from here on every row sees every key
-  int begin = min(i_min * a.G, rows) / kRows * kRows;
-  {
-    const int t = (rows - begin + kRows - 1) / kRows, per = (t + a.splits - 1) / a.splits;
-    begin = min(rows, begin + split * per * kRows);
-    rows = (int)min((long long)rows, (long long)begin + (long long)per * kRows);
-  }
-  Stage<T, DP, kRows> qs, ds;
-  qs.start((const T *)a.q.p + (long long)b * a.q.b + (long long)hk * a.G * a.q.h, a.q.r, a.q.h, a.G, begin, a.D, tid);
-  ds.start((const T *)a.dout.p + (long long)b * a.dout.b + (long long)hk * a.G * a.dout.h, a.dout.r, a.dout.h, a.G, begin, a.D, tid);
-  // threads 0..31 carry the rows' lse, 32..63 their delta
-  int stat_row = begin + (tid & (kRows - 1)), stat_i = stat_row / a.G, stat_g = stat_row - stat_i * a.G;
-  const float *stat = (tid < kRows ? a.lse : a.delta) + ((long long)b * a.Hq + hk * a.G) * a.Lq;
-  float stat_next = 0.0f;
-  auto load = [&]() {
-    qs.load(rows);
-    ds.load(rows);
-    if (tid < 2 * kRows) {
-      stat_next = 0.0f;
-      if (stat_row < rows) stat_next = stat[(long long)stat_g * a.Lq + stat_i] * (tid < kRows ? kLog2e : 1.0f);
-      stat_row += kRows;
-      stat_i += kRows / a.G;
-      stat_g += kRows % a.G;
-      if (stat_g >= a.G) { stat_g -= a.G; ++stat_i; }
-    }
-  };
-  auto store = [&](char *to) {
-    qs.store(to, tid);
-    ds.store(to + kTile, tid);
-    if (tid < 2 * kRows) ((float *)(to + 2 * kTile))[tid] = stat_next;
-  };
   if (begin < rows) {
-    load();
-    store(tiles);
-  }
-  int buffer = 0;
-  for (int r0 = begin; r0 < rows; r0 += kRows) {
-    lds_barrier();                        // this tile is written, the other buffer has been read
-    const char *qt = tiles + buffer * kBuffer, *dt_ = qt + kTile;
-    const float *lt = (const float *)(qt + 2 * kTile), *et = lt + kRows;
-    const bool more = r0 + kRows < rows;
-    if (more) load();
-    f32x16 s = f32x16{}, dp = f32x16{};
+    const T *krow = (const T *)a.k.p + (long long)b * a.k.b + (long long)key * a.k.r + (long long)hk * a.k.h;
+    Frag k[kKc];
 #pragma unroll
-    for (int kc = 0; kc < kKc; ++kc) {
-      s = Elem<T>::mma(TL::row(qt, row_base, 0, kc), k[kc], s);
-      dp = Elem<T>::mma(TL::row(dt_, row_base, 0, kc), TL::row(vt, row_base, 32 * wave, kc), dp);
+    for (int kc = 0; kc < kKc; ++kc) k[kc] = load_frag<T>(krow, key < nk, kc, half, a.D);
+    {
+      Stage<T, DP, 32> vs;
+      vs.start((const T *)a.v.p + (long long)b * a.v.b + (long long)hk * a.v.h, a.v.r, 0, 1, tile * 128, a.D, tid);
+      for (int n = 0; n < 4; ++n) {
+        vs.load(nk);
+        vs.store(vt + n * 32 * TL::kBytes, tid);
+      }
     }
-    // some row of the tile does not see some key of the workgroup (or there is no such row)
-    const bool edge = r0 + kRows > rows || r0 < all_from;
-#pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      const f32x4 ls = *(const f32x4 *)(lt + 8 * r4 + 4 * half), de = *(const f32x4 *)(et + 8 * r4 + 4 * half);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 4 * r4 + e;
-        float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -ls[e]));
-        if (edge) {
-          const int row = r0 + 8 * r4 + 4 * half + e;
-          if (row < first_row || row >= rows) p = 0.0f;
+    int r0 = (rows - 1) / kRows * kRows;
+    Stage<T, DP, kRows> qs, ds;
+    qs.start((const T *)a.q.p + (long long)b * a.q.b + (long long)hk * a.G * a.q.h, a.q.r, a.q.h, a.G, r0, a.D, tid);
+    ds.start((const T *)a.dout.p + (long long)b * a.dout.b + (long long)hk * a.G * a.dout.h, a.dout.r, a.dout.h, a.G, r0, a.D, tid);
+    // threads 0..31 carry the rows' lse, 32..63 their delta
+    int stat_row = r0 + (tid & (kRows - 1)), stat_i = stat_row / a.G, stat_g = stat_row - stat_i * a.G;
+    const float *stat = (tid < kRows ? a.lse : a.delta) + ((long long)b * a.Hq + hk * a.G) * a.Lq;
+    float stat_next = 0.0f;
+    auto load = [&]() {
+      qs.template load<true>(rows);
+      ds.template load<true>(rows);
+      if (tid < 2 * kRows) {
+        // no such row, or one that sees nothing: probabilities 0
+        stat_next = tid < kRows ? INFINITY : 0.0f;
+        if (stat_row < rows) {
+          const float x = stat[(long long)stat_g * a.Lq + stat_i];
+          stat_next = tid < kRows ? (x == -INFINITY ? INFINITY : x * kLog2e) : x;
         }
-        s[r] = p;
-        dp[r] = p * (dp[r] - de[e]);
+        stat_row -= kRows;
+        stat_i -= kRows / a.G;
+        stat_g -= kRows % a.G;
+        if (stat_g < 0) { stat_g += a.G; --stat_i; }
       }
-    }
+    };
+    auto store = [&](char *to) {
+      qs.store(to, tid);
+      ds.store(to + kTile, tid);
+      if (tid < 2 * kRows) ((float *)(to + 2 * kTile))[tid] = stat_next;
+    };
+    load();
+    store(lds);
+    int buffer = 0;
+    for (; r0 >= begin; r0 -= kRows) {
+      lds_barrier();                      // this tile is written, the other buffer has been read
+      const unsigned at = buffer * kBuffer;
+      const bool more = r0 > begin;
+      if (more) load();
+      f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const Frag p = to_frag<T>(s, t), d = to_frag<T>(dp, t);
-#pragma unroll
-      for (int dt = 0; dt < kDt; ++dt) {
-        dv[dt] = Elem<T>::mma(TL::column(dt_, col_base, 16 * t, dt), p, dv[dt]);
-        dk[dt] = Elem<T>::mma(TL::column(qt, col_base, 16 * t, dt), d, dk[dt]);
+      for (int kc = 0; kc < kKc; ++kc) {
+        s = Elem<T>::mma(TL::row(lds, row_base + at, 0, kc), k[kc], s);
+        dp = Elem<T>::mma(TL::row(lds + kTile, row_base + at, 0, kc), TL::row(vt, v_base, 0, kc), dp);
       }
+      if (r0 < diagonal) {                // causal: some row of the tile does not see some key of the workgroup
+        stay_a_branch();
+        const int low = first_row - r0 - 4 * half;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (8 * (r >> 2) + (r & 3) < low) s[r] = -INFINITY;
+      }
+      const float *lt = (const float *)(lds + 2 * kTile + at) + 4 * half;
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const f32x4 ls = *(const f32x4 *)(lt + 8 * r4), de = *(const f32x4 *)(lt + kRows + 8 * r4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * r4 + e;
+          s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -ls[e]));
+          dp[r] = s[r] * (dp[r] - de[e]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const Frag p = to_frag<T>(s, t), d = to_frag<T>(dp, t);
+#pragma unroll
+        for (int dt = 0; dt < kDt; ++dt) {
+          dv[dt] = Elem<T>::mma(TL::column(lds + kTile, col_base + at, 16 * t, dt), p, dv[dt]);
+          dk[dt] = Elem<T>::mma(TL::column(lds, col_base + at, 16 * t, dt), d, dk[dt]);
+        }
+      }
+      buffer ^= 1;
+      if (more) store(lds + buffer * kBuffer);
     }
-    buffer ^= 1;
-    if (more) store(tiles + buffer * kBuffer);
   }
   if (key >= a.Lk) return;
+  if (key >= nk) {                        // behind the sequence's end: its column held no key
+#pragma unroll
+    for (int dt = 0; dt < kDt; ++dt) dk[dt] = dv[dt] = f32x16{};
+  }
   if (a.splits > 1) {
     const long long at = ((long long)split * a.B * a.Hk + group) * a.Lk + key, other = (long long)a.splits * a.B * a.Hk * a.Lk * DP;
     store_rows<float, DP>(a.part_o + at * DP, dk, a.scale, DP, half);
@@ -585,7 +605,6 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_q_k
   const int i_last = min(nq, (min((tile + 1) * 128, a.Lq * a.G) - 1) / a.G + 1) - 1, i_first = tile * 128 / a.G;
   int block_end = i_first >= nq ? 0 : a.causal ? min(nk, max(0, i_last + 1 + nk - nq)) : nk;
   const int full_end = a.causal ? min(nk, max(0, i_first + 1 + nk - nq)) : nk;
-  const bool all_active = (i_last + 1) * a.G >= (tile + 1) * 128;
   int begin = 0;
   {
     const int n = (block_end + kKeys - 1) / kKeys, per = (n + a.splits - 1) / a.splits;
@@ -601,7 +620,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_q_k
 #pragma unroll
   for (int kc = 0; kc < kKc; ++kc) { q[kc] = load_frag<T>(qrow, active, kc, half, a.D); d[kc] = load_frag<T>(drow, active, kc, half, a.D); }
   const long long at = ((long long)b * a.Hq + h) * a.Lq + i;
-  const float ls = active ? a.lse[at] * kLog2e : 0.0f, de = active ? a.delta[at] : 0.0f;
+  // no such row, or one that sees nothing: probabilities 0
+  const float lse = active ? a.lse[at] : -INFINITY, ls = lse == -INFINITY ? INFINITY : lse * kLog2e, de = active ? a.delta[at] : 0.0f;
   f32x16 dq[kDt];
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt) dq[dt] = f32x16{};
@@ -615,7 +635,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_q_k
   int buffer = 0;
   for (int key0 = begin; key0 < block_end; key0 += kKeys) {
     lds_barrier();
-    const char *kt = lds + buffer * 2 * kTile, *vt = kt + kTile;
+    const unsigned at = buffer * 2 * kTile;
     const bool more = key0 + kKeys < block_end;
     if (more) {
       ks.load(block_end);
@@ -624,21 +644,23 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_q_k
     f32x16 s = f32x16{}, dp = f32x16{};
 #pragma unroll
     for (int kc = 0; kc < kKc; ++kc) {
-      s = Elem<T>::mma(TL::row(kt, row_base, 0, kc), q[kc], s);
-      dp = Elem<T>::mma(TL::row(vt, row_base, 0, kc), d[kc], dp);
+      s = Elem<T>::mma(TL::row(lds, row_base + at, 0, kc), q[kc], s);
+      dp = Elem<T>::mma(TL::row(lds + kTile, row_base + at, 0, kc), d[kc], dp);
     }
-    const bool edge = key0 + kKeys > min(full_end, block_end) || !all_active;
+    if (key0 + kKeys > min(full_end, block_end)) {
+      stay_a_branch();
+      const int end = min(seen, block_end) - key0 - 4 * half;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -ls));
-      if (edge && key0 + 8 * (r >> 2) + 4 * half + (r & 3) >= min(seen, block_end)) p = 0.0f;
-      dp[r] = p * (dp[r] - de);
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r >> 2) + (r & 3) >= end) s[r] = -INFINITY;
     }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -ls)) * (dp[r] - de);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const Frag x = to_frag<T>(dp, t);
 #pragma unroll
-      for (int dt = 0; dt < kDt; ++dt) dq[dt] = Elem<T>::mma(TL::column(kt, col_base, 16 * t, dt), x, dq[dt]);
+      for (int dt = 0; dt < kDt; ++dt) dq[dt] = Elem<T>::mma(TL::column(lds, col_base + at, 16 * t, dt), x, dq[dt]);
     }
     buffer ^= 1;
     if (more) {
@@ -707,7 +729,7 @@ template <typename T, int DP> hipError_t attn_backward_dp(AttnArgs a, int kv_spl
   constexpr int kBytes = Tile<T, DP>::kBytes;
   if (a.Lk > 0) {
     static DeviceOnce once;
-    const int lds = (128 + 4 * 32) * kBytes + 512;
+    const int lds = (128 + 4 * 32) * kBytes + 1024;
     rc = allow_lds(once, (const void *)attn_backward_kv_kernel<T, DP>, lds);
     if (rc != hipSuccess) return rc;
     a.tiles = (a.Lk + 127) / 128;
