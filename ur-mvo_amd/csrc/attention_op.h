@@ -305,11 +305,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
     for (int u = 0; u < kSub; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-    top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.scale2;
     // The running maximum only has to keep the exponentials in range: it moves when some row of the wave has grown by more than
-    // 2^kSlack, so that the accumulators are rescaled once or twice per row, not once per tile.
-    if (__any(top > m + kSlack)) {
-      const float mn = fmaxf(m, top), alpha = mn == -INFINITY ? 1.0f : exp2f(m - mn);
+    // 2^kSlack, so that the accumulators are rescaled once or twice per row, not once per tile, and the half waves' maxima are
+    // brought together only then.
+    if (__any(top * a.scale2 > m + kSlack)) {
+      const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * a.scale2), alpha = mn == -INFINITY ? 1.0f : exp2f(m - mn);
       m = mn;
       l *= alpha;
 #pragma unroll
@@ -444,15 +444,19 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a) {
   if (inside && c == 0) a.delta[((long long)b * a.Hq + h) * a.Lq + i] = s;
 }
 
+// Tiles of 64 rows (keys) where the registers allow it: half the barriers, and the second half's products run beside the first
+// half's exponentials.
+template <typename T, int DP> constexpr int kBackwardSub = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
+
 // dk and dv of 128 keys, 32 per wave.  k stays in registers, v in LDS: with both in registers the accumulators leave room for one
-// wave per SIMD only, and nothing runs beside its waits.  The query rows, cut in `splits` ranges of whole tiles of 32, are walked
+// wave per SIMD only, and nothing runs beside its waits.  The query rows, cut in `splits` ranges of whole tiles, are walked
 // from the last one down, range by range over all key tiles: the workgroups that run together read the same rows at about the same
 // time, and the first of them brings a row into the XCD's L2 for the others, causal or not.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_kv_kernel(AttnArgs a) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::Frag Frag;
-  constexpr int kRows = 32, kKc = DP / 16, kDt = DP / 32;
+  constexpr int kSub = kBackwardSub<T, DP>, kRows = 32 * kSub, kKc = DP / 16, kDt = DP / 32;
   extern __shared__ __align__(16) char lds[];
   constexpr int kTile = kRows * TL::kBytes, kBuffer = 2 * kTile + 512;         // q, do, lse (log2 units) and delta of the rows; two buffers
   char *const vt = lds + 2 * kBuffer;
@@ -497,7 +501,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_kv_
     Stage<T, DP, kRows> qs, ds;
     qs.start((const T *)a.q.p + (long long)b * a.q.b + (long long)hk * a.G * a.q.h, a.q.r, a.q.h, a.G, r0, a.D, tid);
     ds.start((const T *)a.dout.p + (long long)b * a.dout.b + (long long)hk * a.G * a.dout.h, a.dout.r, a.dout.h, a.G, r0, a.D, tid);
-    // threads 0..31 carry the rows' lse, 32..63 their delta
+    // threads 0 .. kRows - 1 carry the rows' lse, the next kRows their delta
     int stat_row = r0 + (tid & (kRows - 1)), stat_i = stat_row / a.G, stat_g = stat_row - stat_i * a.G;
     const float *stat = (tid < kRows ? a.lse : a.delta) + ((long long)b * a.Hq + hk * a.G) * a.Lq;
     float stat_next = 0.0f;
@@ -530,37 +534,46 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_kv_
       const unsigned at = buffer * kBuffer;
       const bool more = r0 > begin;
       if (more) load();
-      f32x16 s = f32x16{}, dp = f32x16{};
+      f32x16 s[kSub], dp[kSub];
 #pragma unroll
-      for (int kc = 0; kc < kKc; ++kc) {
-        s = Elem<T>::mma(TL::row(lds, row_base + at, 0, kc), k[kc], s);
-        dp = Elem<T>::mma(TL::row(lds + kTile, row_base + at, 0, kc), TL::row(vt, v_base, 0, kc), dp);
+      for (int u = 0; u < kSub; ++u) {
+        s[u] = dp[u] = f32x16{};
+#pragma unroll
+        for (int kc = 0; kc < kKc; ++kc) {
+          s[u] = Elem<T>::mma(TL::row(lds, row_base + at, 32 * u, kc), k[kc], s[u]);
+          dp[u] = Elem<T>::mma(TL::row(lds + kTile, row_base + at, 32 * u, kc), TL::row(vt, v_base, 0, kc), dp[u]);
+        }
       }
       if (r0 < diagonal) {                // causal: some row of the tile does not see some key of the workgroup
         stay_a_branch();
         const int low = first_row - r0 - 4 * half;
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (8 * (r >> 2) + (r & 3) < low) s[r] = -INFINITY;
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (32 * u + 8 * (r >> 2) + (r & 3) < low) s[u][r] = -INFINITY;
       }
       const float *lt = (const float *)(lds + 2 * kTile + at) + 4 * half;
 #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        const f32x4 ls = *(const f32x4 *)(lt + 8 * r4), de = *(const f32x4 *)(lt + kRows + 8 * r4);
+      for (int u = 0; u < kSub; ++u) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * r4 + e;
-          s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -ls[e]));
-          dp[r] = s[r] * (dp[r] - de[e]);
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const f32x4 ls = *(const f32x4 *)(lt + 32 * u + 8 * r4), de = *(const f32x4 *)(lt + kRows + 32 * u + 8 * r4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * r4 + e;
+            s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], a.scale2, -ls[e]));
+            dp[u][r] = s[u][r] * (dp[u][r] - de[e]);
+          }
         }
-      }
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const Frag p = to_frag<T>(s, t), d = to_frag<T>(dp, t);
+        for (int t = 0; t < 2; ++t) {
+          const Frag p = to_frag<T>(s[u], t), d = to_frag<T>(dp[u], t);
 #pragma unroll
-        for (int dt = 0; dt < kDt; ++dt) {
-          dv[dt] = Elem<T>::mma(TL::column(lds + kTile, col_base + at, 16 * t, dt), p, dv[dt]);
-          dk[dt] = Elem<T>::mma(TL::column(lds, col_base + at, 16 * t, dt), d, dk[dt]);
+          for (int dt = 0; dt < kDt; ++dt) {
+            dv[dt] = Elem<T>::mma(TL::column(lds + kTile, col_base + at, 32 * u + 16 * t, dt), p, dv[dt]);
+            dk[dt] = Elem<T>::mma(TL::column(lds, col_base + at, 32 * u + 16 * t, dt), d, dk[dt]);
+          }
         }
       }
       buffer ^= 1;
@@ -582,12 +595,12 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_kv_
   }
 }
 
-// dq of 128 rows, 32 per wave, whose q and do rows stay in registers; walks the keys (or one of `splits` ranges) in tiles of 32.
+// dq of 128 rows, 32 per wave, whose q and do rows stay in registers; walks the keys (or one of `splits` ranges).
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_q_kernel(AttnArgs a) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::Frag Frag;
-  constexpr int kKeys = 32, kKc = DP / 16, kDt = DP / 32;
+  constexpr int kSub = kBackwardSub<T, DP>, kKeys = 32 * kSub, kKc = DP / 16, kDt = DP / 32;
   extern __shared__ __align__(16) char lds[];
   constexpr int kTile = kKeys * TL::kBytes;                // k, then v; two buffers
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
@@ -641,26 +654,35 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_q_k
       ks.load(block_end);
       vs.load(block_end);
     }
-    f32x16 s = f32x16{}, dp = f32x16{};
+    f32x16 s[kSub], dp[kSub];
 #pragma unroll
-    for (int kc = 0; kc < kKc; ++kc) {
-      s = Elem<T>::mma(TL::row(lds, row_base + at, 0, kc), q[kc], s);
-      dp = Elem<T>::mma(TL::row(lds + kTile, row_base + at, 0, kc), d[kc], dp);
+    for (int u = 0; u < kSub; ++u) {
+      s[u] = dp[u] = f32x16{};
+#pragma unroll
+      for (int kc = 0; kc < kKc; ++kc) {
+        s[u] = Elem<T>::mma(TL::row(lds, row_base + at, 32 * u, kc), q[kc], s[u]);
+        dp[u] = Elem<T>::mma(TL::row(lds + kTile, row_base + at, 32 * u, kc), d[kc], dp[u]);
+      }
     }
     if (key0 + kKeys > min(full_end, block_end)) {
       stay_a_branch();
       const int end = min(seen, block_end) - key0 - 4 * half;
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (8 * (r >> 2) + (r & 3) >= end) s[r] = -INFINITY;
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * u + 8 * (r >> 2) + (r & 3) >= end) s[u][r] = -INFINITY;
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dp[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -ls)) * (dp[r] - de);
+    for (int u = 0; u < kSub; ++u) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const Frag x = to_frag<T>(dp, t);
+      for (int r = 0; r < 16; ++r) dp[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], a.scale2, -ls)) * (dp[u][r] - de);
 #pragma unroll
-      for (int dt = 0; dt < kDt; ++dt) dq[dt] = Elem<T>::mma(TL::column(lds, col_base + at, 16 * t, dt), x, dq[dt]);
+      for (int t = 0; t < 2; ++t) {
+        const Frag x = to_frag<T>(dp[u], t);
+#pragma unroll
+        for (int dt = 0; dt < kDt; ++dt) dq[dt] = Elem<T>::mma(TL::column(lds, col_base + at, 32 * u + 16 * t, dt), x, dq[dt]);
+      }
     }
     buffer ^= 1;
     if (more) {
@@ -726,10 +748,10 @@ template <typename T, int DP> hipError_t attn_backward_dp(AttnArgs a, int kv_spl
   hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
-  constexpr int kBytes = Tile<T, DP>::kBytes;
+  constexpr int kBytes = Tile<T, DP>::kBytes, tile_bytes = 2 * 32 * kBackwardSub<T, DP> * kBytes;
   if (a.Lk > 0) {
     static DeviceOnce once;
-    const int lds = (128 + 4 * 32) * kBytes + 1024;
+    const int lds = 128 * kBytes + 2 * tile_bytes + 1024;
     rc = allow_lds(once, (const void *)attn_backward_kv_kernel<T, DP>, lds);
     if (rc != hipSuccess) return rc;
     a.tiles = (a.Lk + 127) / 128;
@@ -742,7 +764,7 @@ template <typename T, int DP> hipError_t attn_backward_dp(AttnArgs a, int kv_spl
   }
   a.tiles = (a.Lq * a.G + 127) / 128;
   a.splits = q_splits;
-  hipLaunchKernelGGL((attn_backward_q_kernel<T, DP>), dim3((unsigned)a.tiles * a.splits * a.B * a.Hk), dim3(256), 4 * 32 * kBytes, st, a);
+  hipLaunchKernelGGL((attn_backward_q_kernel<T, DP>), dim3((unsigned)a.tiles * a.splits * a.B * a.Hk), dim3(256), 2 * tile_bytes, st, a);
   rc = hipGetLastError();
   if (rc == hipSuccess && a.splits > 1) rc = launch_sum<T, DP>(a.part_o, a.dq, a, a.Lq * a.G, a.G, st);
   return rc;
