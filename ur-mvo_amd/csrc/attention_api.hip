@@ -8,9 +8,9 @@ namespace urf {
 hipError_t attn_forward_f32(const AttnArgs &, int, hipStream_t);
 hipError_t attn_forward_f16(const AttnArgs &, int, hipStream_t);
 hipError_t attn_forward_bf16(const AttnArgs &, int, hipStream_t);
-hipError_t attn_backward_f32(const AttnArgs &, int, int, hipStream_t);
-hipError_t attn_backward_f16(const AttnArgs &, int, int, hipStream_t);
-hipError_t attn_backward_bf16(const AttnArgs &, int, int, hipStream_t);
+hipError_t attn_backward_f32(const AttnArgs &, hipStream_t);
+hipError_t attn_backward_f16(const AttnArgs &, hipStream_t);
+hipError_t attn_backward_bf16(const AttnArgs &, hipStream_t);
 }  // namespace urf
 using namespace urf;
 
@@ -30,35 +30,43 @@ Shape forward_shape(const urf_attn_config &c) {
   return {1, (int)(s < 1 ? 1 : s > 64 ? 64 : s)};
 }
 
+size_t padded_dim(const urf_attn_config &c) { return ((size_t)c.head_dim + 31) / 32 * 32; }
+
 size_t forward_bytes(const urf_attn_config &c) {
   const Shape sh = forward_shape(c);
   if (sh.splits == 1) return 0;
   const size_t rows = ((size_t)c.q_len * (c.q_heads / c.kv_heads) + 31) / 32 * 32 * c.batch * c.kv_heads * sh.splits;
-  return rows * ((c.head_dim <= 64 ? 64 : 128) + 2) * sizeof(float);
+  return rows * (padded_dim(c) + 2) * sizeof(float);
 }
 
-// How the backward kernels are cut: 128 keys (rows) a workgroup, and where that leaves less than two workgroups per CU, the rows
-// (keys) in ranges of at least 256, whose partial sums are added in fp32 afterwards.
-int backward_splits(long long own, long long other, long long groups, bool causal) {
-  const long long blocks = (own + 127) / 128 * groups, most = other / 256, want = ((causal ? 768 : 512) + blocks - 1) / (blocks > 0 ? blocks : 1);
-  const long long s = want < most ? want : most;
-  return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
-}
+// How the backward kernel is cut: 128 keys (or rows) a workgroup over all rows (keys), unless that is more than 0.6 of a workgroup
+// slot's average load -- few workgroups, or a causal mask's uneven ones; then over ranges of at least 256 rows (keys), whose
+// partial sums are added in fp32 afterwards.  A step costs four products for dk and dv, three for dq; two workgroups per CU.
 void backward_shape(const urf_attn_config &c, int *kv_splits, int *q_splits) {
-  const long long rows = (long long)c.q_len * (c.q_heads / c.kv_heads), groups = (long long)c.batch * c.kv_heads;
-  *kv_splits = backward_splits(c.k_len, rows, groups, c.causal);
-  *q_splits = backward_splits(rows, c.k_len, groups, c.causal);
+  const double rows = (double)c.q_len * (c.q_heads / c.kv_heads), keys = c.k_len, groups = (double)c.batch * c.kv_heads;
+  const double kv = 4 * rows, q = 3 * keys, blocks = ceil(keys / 128) * kv + ceil(rows / 128) * q;
+  const double load = groups * blocks * (c.causal ? 0.5 : 1.0) / 512;
+  auto splits = [&](double unit, double other) {
+    const double s = ceil(unit / (0.6 * load)), most = floor(other / 256);
+    return (int)fmax(1.0, fmin(fmin(s, most), 16.0));
+  };
+  *kv_splits = keys > 0 ? splits(kv, rows) : 1;
+  *q_splits = keys > 0 ? splits(q, keys) : 1;
 }
 
 size_t delta_bytes(const urf_attn_config &c) { return ((size_t)c.batch * c.q_heads * c.q_len * sizeof(float) + 15) / 16 * 16; }
 
-// delta, then the partial sums of dk and dv, and after them those of dq in the same place
+// delta, the parts of dk and dv, the parts of dq
+size_t part_kv_bytes(const urf_attn_config &c, int splits) {
+  return splits > 1 ? 2 * (size_t)splits * c.batch * c.kv_heads * c.k_len * padded_dim(c) * sizeof(float) : 0;
+}
+size_t part_q_bytes(const urf_attn_config &c, int splits) {
+  return splits > 1 ? (size_t)splits * c.batch * c.q_heads * c.q_len * padded_dim(c) * sizeof(float) : 0;
+}
 size_t backward_bytes(const urf_attn_config &c) {
   int kv, q;
   backward_shape(c, &kv, &q);
-  const size_t dp = (c.head_dim <= 64 ? 64 : 128) * sizeof(float);
-  const size_t a = kv > 1 ? 2 * (size_t)kv * c.batch * c.kv_heads * c.k_len * dp : 0, b = q > 1 ? (size_t)q * c.batch * c.q_heads * c.q_len * dp : 0;
-  return delta_bytes(c) + (a > b ? a : b);
+  return delta_bytes(c) + part_kv_bytes(c, kv) + part_q_bytes(c, q);
 }
 
 int check_config(const urf_attn_config *c, const char *who) {
@@ -132,7 +140,7 @@ extern "C" int urf_attn_forward(const urf_attn_config *cfg, const urf_attn_tenso
   if (sh.splits > 1) {
     const size_t rows = ((size_t)a.Lq * a.G + 31) / 32 * 32 * a.B * a.Hk * sh.splits;
     a.part_o = (float *)d_work;
-    a.part_ml = a.part_o + rows * (a.D <= 64 ? 64 : 128);
+    a.part_ml = a.part_o + rows * padded_dim(*cfg);
   }
   OnDevice on(cfg->device);
   URF_HIP(on.rc);
@@ -161,12 +169,12 @@ extern "C" int urf_attn_backward(const urf_attn_config *cfg, const urf_attn_tens
   a.o = view(o); a.dout = view(d_o); a.dq = view(dq); a.dk = view(dk); a.dv = view(dv);
   a.lse = (float *)d_lse;
   a.delta = (float *)d_work;
-  a.part_o = (float *)((char *)d_work + delta_bytes(*cfg));
-  int kv, qs;
-  backward_shape(*cfg, &kv, &qs);
+  backward_shape(*cfg, &a.kv_splits, &a.q_splits);
+  a.part_kv = (float *)((char *)d_work + delta_bytes(*cfg));
+  a.part_q = (float *)((char *)a.part_kv + part_kv_bytes(*cfg, a.kv_splits));
   OnDevice on(cfg->device);
   URF_HIP(on.rc);
   const hipStream_t st = (hipStream_t)stream;
-  URF_HIP(cfg->dtype == URF_F32 ? attn_backward_f32(a, kv, qs, st) : cfg->dtype == URF_F16 ? attn_backward_f16(a, kv, qs, st) : attn_backward_bf16(a, kv, qs, st));
+  URF_HIP(cfg->dtype == URF_F32 ? attn_backward_f32(a, st) : cfg->dtype == URF_F16 ? attn_backward_f16(a, st) : attn_backward_bf16(a, st));
   return 0;
 }

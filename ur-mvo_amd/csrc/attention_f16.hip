@@ -3,5 +3,5 @@
 
 namespace urf {
 hipError_t attn_forward_f16(const AttnArgs &a, int narrow, hipStream_t st) { return attn_forward_t<_Float16>(a, narrow, st); }
-hipError_t attn_backward_f16(const AttnArgs &a, int kv_splits, int q_splits, hipStream_t st) { return attn_backward_t<_Float16>(a, kv_splits, q_splits, st); }
+hipError_t attn_backward_f16(const AttnArgs &a, hipStream_t st) { return attn_backward_t<_Float16>(a, st); }
 }  // namespace urf

@@ -28,10 +28,12 @@ struct AttnArgs {
   float *lse;                    // [B][Hq][Lq], natural logarithm
   float *delta;                  // [B][Hq][Lq] (backward)
   float *part_o, *part_ml;       // forward over split keys: [split][B * Hk][rows padded to 32][DP] and (maximum, sum)
+  float *part_kv, *part_q;       // backward in parts: dk then dv [split][B * Hk][Lk][DP]; dq [split][B * Hk][Lq * G][DP]
   int B, Hq, Hk, G, Lq, Lk, D;
   int causal;
-  int splits;                    // key ranges of the forward kernel
-  int tiles;                     // row (key) tiles per (sequence, key head)
+  int splits;                    // forward: key ranges
+  int tiles;                     // its row tiles per (sequence, key head)
+  int kv_tiles, kv_splits, q_tiles, q_splits;   // backward: tiles of 128 keys / rows, and ranges of the other side
   float scale, scale2;           // scale, scale * log2(e)
 };
 
@@ -64,13 +66,15 @@ template <typename T> __device__ __forceinline__ typename Elem<T>::Frag to_frag(
 }
 
 // ------------------------------------------------------------------ LDS tiles
-// A tile is rows x DP elements, row r's 16-byte chunk c at chunk position c ^ swizzle(r).  16-bit types: eight consecutive
+// A tile is rows of 64 or 128 elements (head sizes padded to 32, 64, 96 or 128), row r's 16-byte chunk c at chunk position
+// c ^ swizzle(r).  16-bit types: eight consecutive
 // lanes of a row-wise fragment read (eight rows, one chunk) and the half wave of a transposed read (four rows, four chunks)
 // each fall into distinct banks.
 template <typename T, int DP> struct Tile {
   static constexpr int kPer = 16 / (int)sizeof(T);          // elements of a chunk
-  static constexpr int kChunks = DP / kPer;
-  static constexpr int kBytes = DP * (int)sizeof(T);        // of a row
+  static constexpr int kPitch = DP <= 64 ? 64 : 128;
+  static constexpr int kChunks = kPitch / kPer;
+  static constexpr int kBytes = kPitch * (int)sizeof(T);    // of a row
   static __device__ __forceinline__ int swizzle(int r) {
     if constexpr (sizeof(T) == 4) return (((r >> 2) & 1) << 3) | ((r & 3) << 1);
     else if constexpr (kBytes == 256) return ((r & 3) << 2) | ((r >> 2) & 3);
@@ -221,12 +225,14 @@ __device__ __forceinline__ int clamp_len(const int *lens, int b, int most) {
 }
 
 // ------------------------------------------------------------------ forward
+// workgroups of four waves per CU that the registers are kept for (fp32 rows of 128: twice the registers of everything)
+template <typename T, int DP> constexpr int kBlocksPerCu = sizeof(T) == 2 || DP <= 64 ? 2 : 1;
 constexpr float kSlack = 6.0f;      // log2: probabilities up to 64 before normalisation, in range of every type
 // One workgroup: SPLIT = 0: 128 rows, 32 per wave, over tiles of 64 keys; SPLIT = 1: 32 rows, each of the four waves a quarter of
 // a 128-key tile, joined through LDS at the end (few rows: more workgroups, more loads in flight).  The key range may be cut in
 // `splits` parts, joined by attn_join_kernel.
 template <typename T, int DP, int SPLIT>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, (kBlocksPerCu<T, DP>)) attn_forward_kernel(AttnArgs a) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::Frag Frag;
   constexpr int kKeys = SPLIT ? 128 : 64, kRows = SPLIT ? 32 : 128, kKc = DP / 16, kDt = DP / 32, kSub = SPLIT ? 1 : 2;
@@ -388,7 +394,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_forward_kern
   }
 }
 
-// Joins the key ranges: a wave per row, a lane for two columns; fixed order over the ranges.
+// Joins the key ranges: a wave per row; fixed order over the ranges.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
   const int lane = threadIdx.x & 63, rows = a.Lq * a.G;
@@ -401,21 +407,23 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 #pragma unroll
   for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
   const float mu = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f, o[DP / 64];
+  constexpr int kN = (DP + 63) / 64;       // columns lane and lane + 64
+  float l = 0.0f, o[kN];
 #pragma unroll
-  for (int e = 0; e < DP / 64; ++e) o[e] = 0.0f;
+  for (int e = 0; e < kN; ++e) o[e] = 0.0f;
   for (int s = 0; s < a.splits; ++s) {
     const long long p = base + s * step;
     const float f = exp2f(a.part_ml[p * 2] - mu);
     l += a.part_ml[p * 2 + 1] * f;
 #pragma unroll
-    for (int e = 0; e < DP / 64; ++e) o[e] += a.part_o[p * DP + lane * (DP / 64) + e] * f;
+    for (int e = 0; e < kN; ++e)
+      if (lane + 64 * e < DP) o[e] += a.part_o[p * DP + lane + 64 * e] * f;
   }
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
   T *orow = (T *)a.o.p + (long long)b * a.o.b + (long long)i * a.o.r + (long long)(hk * a.G + g) * a.o.h;
 #pragma unroll
-  for (int e = 0; e < DP / 64; ++e)
-    if (lane * (DP / 64) + e < a.D) orow[lane * (DP / 64) + e] = (T)(o[e] * inv);
+  for (int e = 0; e < kN; ++e)
+    if (lane + 64 * e < a.D) orow[lane + 64 * e] = (T)(o[e] * inv);
   if (lane == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
 }
 
@@ -452,21 +460,19 @@ template <typename T, int DP> constexpr int kBackwardSub = sizeof(T) == 2 && DP 
 // wave per SIMD only, and nothing runs beside its waits.  The query rows, cut in `splits` ranges of whole tiles, are walked
 // from the last one down, range by range over all key tiles: the workgroups that run together read the same rows at about the same
 // time, and the first of them brings a row into the XCD's L2 for the others, causal or not.
-template <typename T, int DP>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_kv_kernel(AttnArgs a) {
+template <typename T, int DP> __device__ __forceinline__ void attn_backward_kv(const AttnArgs &a, int id, char *lds) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::Frag Frag;
   constexpr int kSub = kBackwardSub<T, DP>, kRows = 32 * kSub, kKc = DP / 16, kDt = DP / 32;
-  extern __shared__ __align__(16) char lds[];
   constexpr int kTile = kRows * TL::kBytes, kBuffer = 2 * kTile + 512;         // q, do, lse (log2 units) and delta of the rows; two buffers
   char *const vt = lds + 2 * kBuffer;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
   const unsigned row_base = TL::row_base(col, half), v_base = row_base + 32 * wave * TL::kBytes;
   const typename TL::ColBase col_base = TL::col_base(lane);
   int tile, group;
-  xcd_group_map(blockIdx.x, a.tiles * a.splits, a.B * a.Hk, tile, group);
-  const int split = tile / a.tiles;                                           // 0: the last rows
-  tile -= split * a.tiles;
+  xcd_group_map(id, a.kv_tiles * a.kv_splits, a.B * a.Hk, tile, group);
+  const int split = tile / a.kv_tiles;                                           // 0: the last rows
+  tile -= split * a.kv_tiles;
   const int b = group / a.Hk, hk = group % a.Hk;
   const int nq = clamp_len(a.q_lens, b, a.Lq), nk = clamp_len(a.k_lens, b, a.Lk);
   const int key = tile * 128 + 32 * wave + col;
@@ -477,7 +483,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_kv_
   const int i_min = a.causal ? min(nq, max(0, tile * 128 - (nk - nq))) : 0, diagonal = a.causal ? min(nq, max(0, tile * 128 + 127 - (nk - nq))) * a.G : 0;
   int begin = min(i_min * a.G, rows) / kRows * kRows;
   {
-    const int t = (nq * a.G + kRows - 1) / kRows, per = (t + a.splits - 1) / a.splits * kRows, from = (t * kRows) - (split + 1) * per;
+    const int t = (nq * a.G + kRows - 1) / kRows, per = (t + a.kv_splits - 1) / a.kv_splits * kRows, from = (t * kRows) - (split + 1) * per;
     begin = max(begin, from);
     rows = min(rows, from + per);
   }
@@ -585,10 +591,10 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_kv_
 #pragma unroll
     for (int dt = 0; dt < kDt; ++dt) dk[dt] = dv[dt] = f32x16{};
   }
-  if (a.splits > 1) {
-    const long long at = ((long long)split * a.B * a.Hk + group) * a.Lk + key, other = (long long)a.splits * a.B * a.Hk * a.Lk * DP;
-    store_rows<float, DP>(a.part_o + at * DP, dk, a.scale, DP, half);
-    store_rows<float, DP>(a.part_o + other + at * DP, dv, 1.0f, DP, half);
+  if (a.kv_splits > 1) {
+    const long long at = ((long long)split * a.B * a.Hk + group) * a.Lk + key, other = (long long)a.kv_splits * a.B * a.Hk * a.Lk * DP;
+    store_rows<float, DP>(a.part_kv + at * DP, dk, a.scale, DP, half);
+    store_rows<float, DP>(a.part_kv + other + at * DP, dv, 1.0f, DP, half);
   } else {
     store_rows<T, DP>((T *)a.dk.p + (long long)b * a.dk.b + (long long)key * a.dk.r + (long long)hk * a.dk.h, dk, a.scale, a.D, half);
     store_rows<T, DP>((T *)a.dv.p + (long long)b * a.dv.b + (long long)key * a.dv.r + (long long)hk * a.dv.h, dv, 1.0f, a.D, half);
@@ -596,20 +602,18 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_kv_
 }
 
 // dq of 128 rows, 32 per wave, whose q and do rows stay in registers; walks the keys (or one of `splits` ranges).
-template <typename T, int DP>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_q_kernel(AttnArgs a) {
+template <typename T, int DP> __device__ __forceinline__ void attn_backward_q(const AttnArgs &a, int id, char *lds) {
   typedef Tile<T, DP> TL;
   typedef typename Elem<T>::Frag Frag;
   constexpr int kSub = kBackwardSub<T, DP>, kKeys = 32 * kSub, kKc = DP / 16, kDt = DP / 32;
-  extern __shared__ __align__(16) char lds[];
   constexpr int kTile = kKeys * TL::kBytes;                // k, then v; two buffers
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
   const unsigned row_base = TL::row_base(col, half);
   const typename TL::ColBase col_base = TL::col_base(lane);
   int tile, group;
-  xcd_group_map(blockIdx.x, a.tiles * a.splits, a.B * a.Hk, tile, group);
-  const int split = tile % a.splits;
-  tile = a.tiles - 1 - tile / a.splits;
+  xcd_group_map(id, a.q_tiles * a.q_splits, a.B * a.Hk, tile, group);
+  const int split = tile % a.q_splits;
+  tile = a.q_tiles - 1 - tile / a.q_splits;
   const int b = group / a.Hk, hk = group % a.Hk;
   const int nq = clamp_len(a.q_lens, b, a.Lq), nk = clamp_len(a.k_lens, b, a.Lk);
   const int row = tile * 128 + 32 * wave + col, i = row / a.G, g = row - i * a.G;
@@ -620,7 +624,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_q_k
   const int full_end = a.causal ? min(nk, max(0, i_first + 1 + nk - nq)) : nk;
   int begin = 0;
   {
-    const int n = (block_end + kKeys - 1) / kKeys, per = (n + a.splits - 1) / a.splits;
+    const int n = (block_end + kKeys - 1) / kKeys, per = (n + a.q_splits - 1) / a.q_splits;
     begin = min(block_end, split * per * kKeys);
     block_end = min(block_end, begin + per * kKeys);
   }
@@ -691,21 +695,38 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attn_backward_q_k
     }
   }
   if (!inside) return;
-  if (a.splits > 1)
-    store_rows<float, DP>(a.part_o + (((long long)split * a.B * a.Hk + group) * ((long long)a.Lq * a.G) + row) * DP, dq, a.scale, DP, half);
+  if (a.q_splits > 1)
+    store_rows<float, DP>(a.part_q + (((long long)split * a.B * a.Hk + group) * ((long long)a.Lq * a.G) + row) * DP, dq, a.scale, DP, half);
   else
     store_rows<T, DP>((T *)a.dq.p + (long long)b * a.dq.b + (long long)i * a.dq.r + (long long)h * a.dq.h, dq, a.scale, a.D, half);
 }
 
-// out = the sum of `splits` partial gradients, in their order; rows (group, row) of DP floats, row = i * per_i + g
+// Both in one launch: the first workgroups make dk and dv, the others dq, so that neither leaves CUs idle at its end.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) attn_sum_kernel(const float *part, AttnView out, int groups, int heads, int rows, int per_i, int splits, int D) {
-  const long long u = (long long)blockIdx.x * 256 + threadIdx.x, r = u / (DP / 4);
-  const int d = (int)(u % (DP / 4)) * 4;
-  if (r >= (long long)groups * rows || d >= D) return;
+__global__ void __launch_bounds__(256, (kBlocksPerCu<T, DP>)) attn_backward_kernel(AttnArgs a) {
+  extern __shared__ __align__(16) char lds[];
+  const int kv_blocks = a.kv_tiles * a.kv_splits * a.B * a.Hk;
+  if ((int)blockIdx.x < kv_blocks) attn_backward_kv<T, DP>(a, blockIdx.x, lds);
+  else attn_backward_q<T, DP>(a, blockIdx.x - kv_blocks, lds);
+}
+
+// The gradients that were made in parts: the sums of the parts, in their order.  Four elements a thread, over the rows of dk and dv
+// (group, key) and of dq (group, row = i * G + g) as far as they have parts.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) attn_sum_kernel(AttnArgs a) {
+  long long u = (long long)blockIdx.x * 256 + threadIdx.x, r = u / (DP / 4);
+  const int d = (int)(u % (DP / 4)) * 4, groups = a.B * a.Hk;
+  const long long kv_rows = a.kv_splits > 1 ? (long long)groups * a.Lk : 0, q_rows = a.q_splits > 1 ? (long long)groups * a.Lq * a.G : 0;
+  if (r >= 2 * kv_rows + q_rows || d >= a.D) return;
+  const bool is_q = r >= 2 * kv_rows, is_v = !is_q && r >= kv_rows;
+  const float *part = is_q ? a.part_q : a.part_kv + (is_v ? a.kv_splits * kv_rows * DP : 0);
+  const AttnView out = is_q ? a.dq : is_v ? a.dv : a.dk;
+  const long long all = is_q ? q_rows : kv_rows;
+  const int splits = is_q ? a.q_splits : a.kv_splits, rows = is_q ? a.Lq * a.G : a.Lk, per_i = is_q ? a.G : 1;
+  r -= is_q ? 2 * kv_rows : is_v ? kv_rows : 0;
   f32x4 s = *(const f32x4 *)(part + r * DP + d);
-  for (int n = 1; n < splits; ++n) s += *(const f32x4 *)(part + ((long long)n * groups * rows + r) * DP + d);
-  const int group = (int)(r / rows), row = (int)(r % rows), b = group / heads, hk = group % heads, i = row / per_i, g = row - i * per_i;
+  for (int n = 1; n < splits; ++n) s += *(const f32x4 *)(part + (n * all + r) * DP + d);
+  const int group = (int)(r / rows), row = (int)(r % rows), b = group / a.Hk, hk = group % a.Hk, i = row / per_i, g = row - i * per_i;
   store4<T>((T *)out.p + (long long)b * out.b + (long long)i * out.r + (long long)(hk * per_i + g) * out.h + d, s[0], s[1], s[2], s[3]);
 }
 
@@ -736,45 +757,34 @@ template <typename T, int DP> hipError_t attn_forward_dp(AttnArgs a, int narrow,
   return hipGetLastError();
 }
 
-template <typename T, int DP>
-hipError_t launch_sum(const float *part, const AttnView &out, const AttnArgs &a, int rows, int per_i, hipStream_t st) {
-  const long long n = (long long)a.B * a.Hk * rows * (DP / 4);
-  hipLaunchKernelGGL((attn_sum_kernel<T, DP>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, out, a.B * a.Hk, a.Hk, rows, per_i, a.splits, a.D);
-  return hipGetLastError();
-}
-
-template <typename T, int DP> hipError_t attn_backward_dp(AttnArgs a, int kv_splits, int q_splits, hipStream_t st) {
+template <typename T, int DP> hipError_t attn_backward_dp(AttnArgs a, hipStream_t st) {
   const long long rows = (long long)a.B * a.Lq * a.Hq;
   hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, a);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
-  constexpr int kBytes = Tile<T, DP>::kBytes, tile_bytes = 2 * 32 * kBackwardSub<T, DP> * kBytes;
-  if (a.Lk > 0) {
-    static DeviceOnce once;
-    const int lds = 128 * kBytes + 2 * tile_bytes + 1024;
-    rc = allow_lds(once, (const void *)attn_backward_kv_kernel<T, DP>, lds);
-    if (rc != hipSuccess) return rc;
-    a.tiles = (a.Lk + 127) / 128;
-    a.splits = kv_splits;
-    hipLaunchKernelGGL((attn_backward_kv_kernel<T, DP>), dim3((unsigned)a.tiles * a.splits * a.B * a.Hk), dim3(256), lds, st, a);
-    rc = hipGetLastError();
-    if (rc == hipSuccess && a.splits > 1) rc = launch_sum<T, DP>(a.part_o, a.dk, a, a.Lk, 1, st);
-    if (rc == hipSuccess && a.splits > 1) rc = launch_sum<T, DP>(a.part_o + (long long)a.splits * a.B * a.Hk * a.Lk * DP, a.dv, a, a.Lk, 1, st);
-    if (rc != hipSuccess) return rc;
-  }
-  a.tiles = (a.Lq * a.G + 127) / 128;
-  a.splits = q_splits;
-  hipLaunchKernelGGL((attn_backward_q_kernel<T, DP>), dim3((unsigned)a.tiles * a.splits * a.B * a.Hk), dim3(256), 2 * tile_bytes, st, a);
+  constexpr int kBytes = Tile<T, DP>::kBytes;
+  static DeviceOnce once;
+  const int lds = 128 * kBytes + 4 * 32 * kBackwardSub<T, DP> * kBytes + 1024;
+  rc = allow_lds(once, (const void *)attn_backward_kernel<T, DP>, lds);
+  if (rc != hipSuccess) return rc;
+  a.kv_tiles = (a.Lk + 127) / 128;
+  a.q_tiles = (a.Lq * a.G + 127) / 128;
+  const unsigned grid = (unsigned)(a.kv_tiles * a.kv_splits + a.q_tiles * a.q_splits) * a.B * a.Hk;
+  hipLaunchKernelGGL((attn_backward_kernel<T, DP>), dim3(grid), dim3(256), lds, st, a);
   rc = hipGetLastError();
-  if (rc == hipSuccess && a.splits > 1) rc = launch_sum<T, DP>(a.part_o, a.dq, a, a.Lq * a.G, a.G, st);
-  return rc;
+  const long long sums = (long long)a.B * a.Hk * ((a.kv_splits > 1 ? 2ll * a.Lk : 0) + (a.q_splits > 1 ? (long long)a.Lq * a.G : 0)) * (DP / 4);
+  if (rc != hipSuccess || sums == 0) return rc;
+  hipLaunchKernelGGL((attn_sum_kernel<T, DP>), dim3((unsigned)((sums + 255) / 256)), dim3(256), 0, st, a);
+  return hipGetLastError();
 }
 
 template <typename T> hipError_t attn_forward_t(const AttnArgs &a, int narrow, hipStream_t st) {
-  return a.D <= 64 ? attn_forward_dp<T, 64>(a, narrow, st) : attn_forward_dp<T, 128>(a, narrow, st);
+  return a.D <= 32 ? attn_forward_dp<T, 32>(a, narrow, st) : a.D <= 64 ? attn_forward_dp<T, 64>(a, narrow, st)
+       : a.D <= 96 ? attn_forward_dp<T, 96>(a, narrow, st) : attn_forward_dp<T, 128>(a, narrow, st);
 }
-template <typename T> hipError_t attn_backward_t(const AttnArgs &a, int kv_splits, int q_splits, hipStream_t st) {
-  return a.D <= 64 ? attn_backward_dp<T, 64>(a, kv_splits, q_splits, st) : attn_backward_dp<T, 128>(a, kv_splits, q_splits, st);
+template <typename T> hipError_t attn_backward_t(const AttnArgs &a, hipStream_t st) {
+  return a.D <= 32 ? attn_backward_dp<T, 32>(a, st) : a.D <= 64 ? attn_backward_dp<T, 64>(a, st)
+       : a.D <= 96 ? attn_backward_dp<T, 96>(a, st) : attn_backward_dp<T, 128>(a, st);
 }
 
 }  // namespace urf
