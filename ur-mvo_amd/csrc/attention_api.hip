@@ -19,13 +19,16 @@ namespace {
 struct Shape { int narrow, splits; };
 
 // How the forward pass is cut.  128-row workgroups read the keys least often; where they are fewer than the 256 CUs, 32-row
-// workgroups; where those are fewer as well, the keys are split until there are two workgroups per CU, at least 256 keys each.
+// workgroups whose waves share the keys; where those are fewer as well, the keys are split until there are two workgroups per CU, at
+// least 256 keys each.  Up to 32 rows (one token, some heads) the keys' bytes are all there is: eight workgroups per CU even out
+// lengths and keep loads in flight (32 sequences of up to 16384 keys, 8 key heads of 128, bf16: 427 us in 128-row workgroups, 344 in
+// 32-row ones, 320, 303 and 290 with 512, 1024 and 2048 of them).
 Shape forward_shape(const urf_attn_config &c) {
   const long long rows = (long long)c.q_len * (c.q_heads / c.kv_heads), groups = (long long)c.batch * c.kv_heads;
-  if ((rows + 127) / 128 * groups >= 256) return {0, 1};
+  if (rows > 32 && (rows + 127) / 128 * groups >= 256) return {0, 1};
   const long long blocks = (rows + 31) / 32 * groups;
-  if (blocks >= 256) return {1, 1};
-  const long long most = (c.k_len + 255) / 256, want = (512 + blocks - 1) / blocks;
+  if (rows > 32 && blocks >= 256) return {1, 1};
+  const long long most = (c.k_len + 255) / 256, want = ((rows > 32 ? 512 : 2048) + blocks - 1) / blocks;
   const long long s = want < most ? want : most;
   return {1, (int)(s < 1 ? 1 : s > 64 ? 64 : s)};
 }
@@ -35,23 +38,30 @@ size_t padded_dim(const urf_attn_config &c) { return ((size_t)c.head_dim + 31) /
 size_t forward_bytes(const urf_attn_config &c) {
   const Shape sh = forward_shape(c);
   if (sh.splits == 1) return 0;
-  const size_t rows = ((size_t)c.q_len * (c.q_heads / c.kv_heads) + 31) / 32 * 32 * c.batch * c.kv_heads * sh.splits;
+  const size_t rows = (size_t)c.q_len * c.q_heads * c.batch * sh.splits;
   return rows * (padded_dim(c) + 2) * sizeof(float);
 }
 
-// How the backward kernel is cut: 128 keys (or rows) a workgroup over all rows (keys), unless that is more than 0.6 of a workgroup
-// slot's average load -- few workgroups, or a causal mask's uneven ones; then over ranges of at least 256 rows (keys), whose
-// partial sums are added in fp32 afterwards.  A step costs four products for dk and dv, three for dq; two workgroups per CU.
+// How the backward kernel is cut: 128 keys (or rows) a workgroup, over all rows (keys) or over `splits` ranges of them whose partial
+// sums are added in fp32 afterwards.  Chosen by an estimate of its time, in ns: a workgroup's product of one row with its 128 keys
+// takes 0.17 (16 bits) or 1.4 (fp32) per element of the head with two workgroups on every CU (four products for dk and dv, three for
+// dq), a range costs two steps of 32 rows to begin with, and its partial sums are written and read at 4.7 TB/s.
 void backward_shape(const urf_attn_config &c, int *kv_splits, int *q_splits) {
   const double rows = (double)c.q_len * (c.q_heads / c.kv_heads), keys = c.k_len, groups = (double)c.batch * c.kv_heads;
-  const double kv = 4 * rows, q = 3 * keys, blocks = ceil(keys / 128) * kv + ceil(rows / 128) * q;
-  const double load = groups * blocks * (c.causal ? 0.5 : 1.0) / 512;
-  auto splits = [&](double unit, double other) {
-    const double s = ceil(unit / (0.6 * load)), most = floor(other / 256);
-    return (int)fmax(1.0, fmin(fmin(s, most), 16.0));
-  };
-  *kv_splits = keys > 0 ? splits(kv, rows) : 1;
-  *q_splits = keys > 0 ? splits(q, keys) : 1;
+  const double dim = (c.head_dim + 31) / 32 * 32, step = dim * (c.dtype == URF_F32 ? 1.4 : 0.17), part = dim * 8 / 4700.0;
+  const double kv_tiles = ceil(keys / 128), q_tiles = ceil(rows / 128), share = c.causal ? 0.5 : 1.0;
+  double best = INFINITY;
+  *kv_splits = *q_splits = 1;
+  for (int k = 1; k <= 16 && (k == 1 || rows / k >= 64); ++k)
+    for (int q = 1; q <= 16 && (q == 1 || keys / q >= 64); ++q) {
+      const double units = groups * (kv_tiles * k + q_tiles * q), largest = step * fmax(4 * (rows / k + 64), 3 * (keys / q + 64));
+      const double all = step * groups * (kv_tiles * 4 * (rows * share + 64 * k) + q_tiles * 3 * (keys * share + 64 * q));
+      // equal units fill whole rounds of the 512 places; uneven ones (a causal mask's) even out
+      const double rounds = c.causal ? all / 512 : ceil(units / 512) * (all / units);
+      const double parts = (k > 1 ? 2 * k * groups * keys * part : 0.0) + (q > 1 ? q * groups * rows * part : 0.0) + (k > 1 || q > 1 ? 3000.0 : 0.0);
+      const double t = fmax(largest, rounds) + parts;
+      if (t < best) { best = t; *kv_splits = k; *q_splits = q; }
+    }
 }
 
 size_t delta_bytes(const urf_attn_config &c) { return ((size_t)c.batch * c.q_heads * c.q_len * sizeof(float) + 15) / 16 * 16; }
@@ -138,7 +148,7 @@ extern "C" int urf_attn_forward(const urf_attn_config *cfg, const urf_attn_tenso
   a.lse = d_lse;
   a.splits = sh.splits;
   if (sh.splits > 1) {
-    const size_t rows = ((size_t)a.Lq * a.G + 31) / 32 * 32 * a.B * a.Hk * sh.splits;
+    const size_t rows = (size_t)a.Lq * a.Hq * a.B * sh.splits;
     a.part_o = (float *)d_work;
     a.part_ml = a.part_o + rows * padded_dim(*cfg);
   }
