@@ -243,6 +243,13 @@ int urf_sg_infer(urf_pm *h, const double *f0, int n0, const double *f1, int n1,
  * dustbin row and column (src/super_glue.cpp:466-474), (n0+1) x (n1+1) f32: the input of the Sinkhorn iterations */
 int urf_sg_debug_couplings(urf_pm *h, int n0, int n1, float *out);
 
+/* How decided the last urf_sg_infer call with Zout of this handle was: its log-assignment (still on the device) as a distribution of
+ * each of the n0 keypoints over the n1 keypoints of the other image and the dustbin (candidate n1).  log_prob[i] = of candidate
+ * targets[i] (NULL, or n0 ints; 0 for an entry outside [0, n1], e.g. -1), entropy[i] in nats, and the `top` (0 .. URF_TOP_MAX) best
+ * candidates with their log probabilities, descending, n0 x top.  Host arrays.  An error once the handle has matched another pair. */
+int urf_sg_match_log_probs(urf_pm *h, const int *targets, int top, float *log_prob, float *entropy, int *top_index,
+                           float *top_log_prob);
+
 /* PointMatching::MatchingPoints(features0, features1, matches,
  * outlier_rejection), src/point_matching.cc:14-61.  Returns the match count
  * (>=0) or <0 on error.  The cv::findFundamentalMat call (:50) is replaced by
@@ -635,13 +642,13 @@ typedef struct {
 } urf_rows_config;
 /* z = scale * logits of a row.  lse[row] = log sum exp z; entropy[row] of softmax(z), in nats; log_prob[row][n] = z[targets[row][n]]
  * - lse, 0 for a target outside [0, classes) (-1: none); top_index / top_log_prob[row][top]: the `top` largest scores, descending,
- * equal ones by index.  Scores may be -infinity (log probability -infinity); a row of nothing else has lse -infinity and entropy 0.
- * A row with a NaN or +infinity has NaN everywhere and -1 as its alternatives.  d_targets may be NULL with n_targets = 0. */
+ * equal ones by index.  Scores may be -infinity (log probability -infinity).  A row whose largest z is below -2^100 (masks of
+ * -infinity or of the lowest fp32 or bf16 value everywhere) allows nothing: lse and log probabilities -infinity, entropy 0.  A row with a NaN or +infinity has NaN everywhere and -1 as its alternatives.  d_targets may be NULL with n_targets = 0. */
 int urf_log_probs(const urf_rows_config *cfg, const void *logits, const int *d_targets, int n_targets, int top, float *d_log_prob,
                   float *d_entropy, float *d_lse, int *d_top_index, float *d_top_log_prob, void *stream);
 /* d_logits (rows of d_logits_stride elements) = the gradient of sum(log_prob * d_log_prob) + sum(entropy * d_entropy), from the
- * forward call's lse and entropy; d_entropy may be NULL.  A candidate that is a target twice gets both.  Rows without a score above
- * -infinity get 0. */
+ * forward call's lse and entropy; d_entropy may be NULL.  A candidate that is a target twice gets both.  Rows that allow
+ * nothing get 0. */
 int urf_log_probs_backward(const urf_rows_config *cfg, const void *logits, const int *d_targets, int n_targets, const float *d_lse,
                            const float *d_entropy, const float *d_d_log_prob, const float *d_d_entropy, void *d_logits,
                            long long d_logits_stride, void *stream);

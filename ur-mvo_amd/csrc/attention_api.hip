@@ -93,8 +93,9 @@ int check_config(const urf_attn_config *c, const char *who) {
   return 0;
 }
 
-int check_tensor(const urf_attn_tensor *t, const urf_attn_config *c, const char *who, const char *name) {
-  URF_CHECK(t && t->data, "%s: %s is null", who, name);
+// `len` rows; without any there is nothing to point to
+int check_tensor(const urf_attn_tensor *t, const urf_attn_config *c, int len, const char *who, const char *name) {
+  URF_CHECK(t && (t->data || len == 0), "%s: %s is null", who, name);
   const long long per = 16 / dtype_bytes(c->dtype);
   URF_CHECK(((uintptr_t)t->data & 15) == 0 && t->batch_stride % per == 0 && t->row_stride % per == 0 && t->head_stride % per == 0,
             "%s: %s: base and strides have to be multiples of 16 bytes", who, name);
@@ -102,7 +103,7 @@ int check_tensor(const urf_attn_tensor *t, const urf_attn_config *c, const char 
 }
 
 int check_out(const urf_attn_tensor *t, const urf_attn_config *c, int len, int heads, const char *who, const char *name) {
-  if (check_tensor(t, c, who, name)) return -2;
+  if (check_tensor(t, c, len, who, name)) return -2;
   // two elements of an output may not share memory: no stride of a dimension longer than one below the head size
   const long long D = c->head_dim;
   URF_CHECK((c->batch == 1 || llabs(t->batch_stride) >= D) && (len <= 1 || llabs(t->row_stride) >= D) && (heads == 1 || llabs(t->head_stride) >= D),
@@ -136,7 +137,7 @@ extern "C" int urf_attn_forward(const urf_attn_config *cfg, const urf_attn_tenso
                                 const int *d_q_lens, const int *d_k_lens, const urf_attn_tensor *o, float *d_lse, void *d_work,
                                 size_t work_bytes, void *stream) {
   const char *who = "urf_attn_forward";
-  if (check_config(cfg, who) || check_tensor(q, cfg, who, "q") || check_tensor(k, cfg, who, "k") || check_tensor(v, cfg, who, "v") ||
+  if (check_config(cfg, who) || check_tensor(q, cfg, cfg->q_len, who, "q") || check_tensor(k, cfg, cfg->k_len, who, "k") || check_tensor(v, cfg, cfg->k_len, who, "v") ||
       check_out(o, cfg, cfg->q_len, cfg->q_heads, who, "o")) return -2;
   URF_CHECK(d_lse, "%s: lse is null", who);
   URF_CHECK(o->data != q->data && o->data != k->data && o->data != v->data, "%s: o may not be an input", who);
@@ -164,14 +165,14 @@ extern "C" int urf_attn_backward(const urf_attn_config *cfg, const urf_attn_tens
                                  const int *d_k_lens, const urf_attn_tensor *dq, const urf_attn_tensor *dk, const urf_attn_tensor *dv,
                                  void *d_work, size_t work_bytes, void *stream) {
   const char *who = "urf_attn_backward";
-  if (check_config(cfg, who) || check_tensor(q, cfg, who, "q") || check_tensor(k, cfg, who, "k") || check_tensor(v, cfg, who, "v") ||
-      check_tensor(o, cfg, who, "o") || check_tensor(d_o, cfg, who, "the gradient of o") || check_out(dq, cfg, cfg->q_len, cfg->q_heads, who, "dq") ||
+  if (check_config(cfg, who) || check_tensor(q, cfg, cfg->q_len, who, "q") || check_tensor(k, cfg, cfg->k_len, who, "k") || check_tensor(v, cfg, cfg->k_len, who, "v") ||
+      check_tensor(o, cfg, cfg->q_len, who, "o") || check_tensor(d_o, cfg, cfg->q_len, who, "the gradient of o") || check_out(dq, cfg, cfg->q_len, cfg->q_heads, who, "dq") ||
       check_out(dk, cfg, cfg->k_len, cfg->kv_heads, who, "dk") || check_out(dv, cfg, cfg->k_len, cfg->kv_heads, who, "dv")) return -2;
   URF_CHECK(d_lse, "%s: lse is null", who);
   const void *in[5] = {q->data, k->data, v->data, o->data, d_o->data}, *out[3] = {dq->data, dk->data, dv->data};
   for (int x = 0; x < 3; ++x) {
-    for (int y = 0; y < 5; ++y) URF_CHECK(out[x] != in[y], "%s: an output may not be an input", who);
-    for (int y = 0; y < x; ++y) URF_CHECK(out[x] != out[y], "%s: two outputs share a base", who);
+    for (int y = 0; y < 5; ++y) URF_CHECK(!out[x] || out[x] != in[y], "%s: an output may not be an input", who);
+    for (int y = 0; y < x; ++y) URF_CHECK(!out[x] || out[x] != out[y], "%s: two outputs share a base", who);
   }
   const size_t need = backward_bytes(*cfg);
   URF_CHECK(d_work && work_bytes >= need && ((uintptr_t)d_work & 15) == 0, "%s: workspace of %zu bytes, %zu needed", who, work_bytes, need);

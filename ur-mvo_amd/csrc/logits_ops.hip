@@ -1,9 +1,10 @@
 // logits_ops.hip -- operators over rows of scores (logits, log-assignments) on caller-owned tensors: log probabilities of given
 // candidates with entropy and top alternatives, distillation from a teacher's top alternatives, and their gradients.
 //
-// With c = scale log2(e), x_v = c z_v and m = max x:  S = sum 2^(x_v - m),  lse = (m + log2 S) ln 2,  and the entropy is
-// (log2 S - A / S) ln 2 with A = sum 2^(x_v - m) (x_v - m): one pass over the row, every lane with a running maximum of its own
-// that rescales its sums when it grows.  The gradients need lse only and are one more pass: read a score, write its gradient.
+// With c = scale log2(e), m = max z and x_v = c (z_v - m):  S = sum 2^x_v,  lse = scale m + ln S,  and the entropy is
+// (log2 S - A / S) ln 2 with A = sum 2^x_v x_v: one pass over the row, every lane with a running maximum of its own that rescales its
+// sums when it grows.  (The difference comes before the product: scores at the lowest value of their type stay in range.)  The
+// gradients need lse only and are one more pass: read a score, write its gradient.
 // All of it is bound by memory: a score is read once per pass, 16 bytes a lane and load, four loads in flight per lane.
 //
 // A row belongs to W waves (1, 4 or 16, one workgroup): 1 where the rows are short, 16 where there are too few rows to fill the
@@ -22,14 +23,15 @@ namespace urf {
 
 static_assert(URF_TOP_MAX == 64, "one listed candidate per lane");
 constexpr int kUnroll = 4;               // 16-byte loads in flight per lane
-constexpr double kLog2eDouble = 1.4426950408889634, kLn2Double = 0.6931471805599453;
+constexpr double kLog2eDouble = 1.4426950408889634;
+constexpr float kNothing = -0x1p100f;    // a row whose largest scaled score is below it allows nothing (masks of -inf or the lowest value)
 constexpr float kFloor = -1.0e4f;        // 2^kFloor is 0: a masked score (-inf) adds 0 * kFloor to A, not 0 * inf
 
 struct RowsArgs {
   const void *z;                 // [R] rows of V scores
   long long stride;              // elements between rows
   int R, V;
-  float c, clo;                  // scale * log2(e), and what the float lacks of it
+  float c;                       // scale * log2(e)
   float scale;                   // 1 / temperature for the distillation
   // log probabilities
   const int *targets; int N;     // [R][N]
@@ -100,19 +102,19 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-// running maximum (of x) and sums of a lane, a wave, a row
+// running maximum (of the scores) and sums of a lane, a wave, a row
 struct Stat { float m, s, a; };
-__device__ __forceinline__ Stat join(Stat p, Stat q) {
+__device__ __forceinline__ Stat join(Stat p, Stat q, float c) {
   const float m = fmaxf(p.m, q.m), mu = m == -INFINITY ? 0.0f : m;
-  const float fp = exp2f(p.m - mu), fq = exp2f(q.m - mu), dp = fmaxf(p.m - mu, kFloor), dq = fmaxf(q.m - mu, kFloor);
-  // x - m = (x - p.m) + (p.m - m)
-  return {m, p.s * fp + q.s * fq, fmaf(p.s, dp, p.a) * fp + fmaf(q.s, dq, q.a) * fq};
+  const float xp = (p.m - mu) * c, xq = (q.m - mu) * c, fp = exp2f(xp), fq = exp2f(xq);
+  // c (z - m) = c (z - p.m) + c (p.m - m)
+  return {m, p.s * fp + q.s * fq, fmaf(p.s, fmaxf(xp, kFloor), p.a) * fp + fmaf(q.s, fmaxf(xq, kFloor), q.a) * fq};
 }
-__device__ __forceinline__ Stat wave_join(Stat v) {
+__device__ __forceinline__ Stat wave_join(Stat v, float c) {
 #pragma unroll
   for (int x = 32; x >= 1; x >>= 1) {
     const Stat o = {lane_xor(v.m, x), lane_xor(v.s, x), lane_xor(v.a, x)};
-    v = (threadIdx.x & x) ? join(o, v) : join(v, o);      // the same operand order on both sides: the same bits in every lane
+    v = (threadIdx.x & x) ? join(o, v, c) : join(v, o, c);      // the same operand order on both sides: the same bits in every lane
   }
   return v;
 }
@@ -180,10 +182,9 @@ struct Share {
 };
 
 // One pass of a wave over its share of a row.  TOP: notes the lanes' best scores; TAIL: leaves the listed candidates out, so that a
-// tail far below them keeps its own maximum.  `clo`: what c lacks of scale * log2(e) (fp32 scores only: their gradients are told
-// apart to the last bits; 16-bit scores have none to tell).
+// tail far below them keeps its own maximum.
 template <typename T, int W, bool ENTROPY, bool TOP, bool TAIL>
-__device__ __forceinline__ Stat row_pass(const T *z, int V, float c, float clo, int part, int lane, int mine, Share &sh) {
+__device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, int lane, int mine, Share &sh) {
   typedef Row<T> RW;
   constexpr int kPer = RW::kPer, kStep = 64 * kPer;
   Stat st = {-INFINITY, 0.0f, 0.0f};
@@ -191,16 +192,14 @@ __device__ __forceinline__ Stat row_pass(const T *z, int V, float c, float clo, 
     float top = f[0];
 #pragma unroll
     for (int e = 1; e < n; ++e) top = fmaxf(top, f[e]);
-    const float m = fmaxf(st.m, top * c), mu = m == -INFINITY ? 0.0f : m;
-    const float f0 = __builtin_amdgcn_exp2f(st.m - mu);
-    if (ENTROPY) st.a = fmaf(st.s, fmaxf(st.m - mu, kFloor), st.a) * f0;
+    const float m = fmaxf(st.m, top), mu = m == -INFINITY ? 0.0f : m;
+    const float x0 = (st.m - mu) * c, f0 = __builtin_amdgcn_exp2f(x0);
+    if (ENTROPY) st.a = fmaf(st.s, fmaxf(x0, kFloor), st.a) * f0;
     st.s *= f0;
     st.m = m;
 #pragma unroll
     for (int e = 0; e < n; ++e) {
-      float x = fmaf(f[e], c, -mu);
-      if (sizeof(T) == 4) x = f[e] == -INFINITY ? x : fmaf(f[e], clo, x);
-      const float p = __builtin_amdgcn_exp2f(x);
+      const float x = (f[e] - mu) * c, p = __builtin_amdgcn_exp2f(x);
       st.s += p;
       if (ENTROPY) st.a = fmaf(p, fmaxf(x, kFloor), st.a);
     }
@@ -326,14 +325,14 @@ __device__ __forceinline__ u64 top_alternatives(const T *z, int V, int K, const 
 }
 
 // joins the parts of a row, in every wave
-template <int W> __device__ __forceinline__ Stat row_join(Stat st, int wave, int lane, Stat *lds) {
-  st = wave_join(st);
+template <int W> __device__ __forceinline__ Stat row_join(Stat st, float c, int wave, int lane, Stat *lds) {
+  st = wave_join(st, c);
   if constexpr (W > 1) {
     if (lane == 0) lds[wave] = st;
     lds_barrier();
     st = lds[0];
 #pragma unroll
-    for (int w = 1; w < W; ++w) st = join(st, lds[w]);
+    for (int w = 1; w < W; ++w) st = join(st, lds[w], c);
   }
   return st;
 }
@@ -349,20 +348,20 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) log_probs_kernel(RowsArg
   if (r >= a.R) return;
   const T *z = (const T *)a.z + (long long)r * a.stride;
   Share sh;
-  Stat st = row_pass<T, W, true, TOP, false>(z, a.V, a.c, a.clo, wave, lane, -1, sh);
-  st = row_join<W>(st, wave, lane, stats);
+  Stat st = row_pass<T, W, true, TOP, false>(z, a.V, a.c, wave, lane, -1, sh);
+  st = row_join<W>(st, a.c, wave, lane, stats);
   u64 list = 0;
   if constexpr (TOP) list = top_alternatives<T, W>(z, a.V, a.K, sh, wave, lane, keys, keys + 64 * kWaves + 160 * (threadIdx.x >> 6));
   if (wave) return;
-  // a NaN or +inf score leaves no distribution: everything is NaN and the alternatives are -1.  A row without any score above
-  // -inf: lse -inf, entropy 0, every log probability -inf.
-  const bool broken = !(st.s >= 0.0f) || st.m == INFINITY, empty = st.m == -INFINITY && !broken;
-  const float ls = log2f(st.s), nan = __uint_as_float(0x7fc00000u);
+  // a NaN or +inf score leaves no distribution: everything is NaN and the alternatives are -1.  A row that allows nothing: lse
+  // -inf, entropy 0, every log probability -inf.
+  const bool broken = !(st.s >= 0.0f) || st.m == INFINITY, empty = st.m * a.scale < kNothing && !broken;
+  const float ls = logf(st.s), nan = __uint_as_float(0x7fc00000u);
   if (lane == 0) {
-    a.lse[r] = broken ? nan : empty ? -INFINITY : (float)(((double)st.m + log2((double)st.s)) * kLn2Double);
-    a.entropy[r] = broken ? nan : empty ? 0.0f : (ls - st.a / st.s) * kLn2;
+    a.lse[r] = broken ? nan : empty ? -INFINITY : (float)((double)st.m * a.scale + ls);
+    a.entropy[r] = broken ? nan : empty ? 0.0f : fmaf(-st.a / st.s, kLn2, ls);
   }
-  auto log_prob = [&](float x) { return broken ? nan : empty || x == -INFINITY ? -INFINITY : (fmaf(x, a.clo, fmaf(x, a.c, -st.m)) - ls) * kLn2; };
+  auto log_prob = [&](float x) { return broken ? nan : empty || x == -INFINITY ? -INFINITY : fmaf(x - st.m, a.scale, -ls); };
   if (lane < a.N) {
     const int t = a.targets[(long long)r * a.N + lane];
     a.log_prob[(long long)r * a.N + lane] = t >= 0 && t < a.V ? log_prob((float)z[t]) : 0.0f;
@@ -412,13 +411,12 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) distill_kernel(RowsArgs 
   const T *z = (const T *)a.z + (long long)r * a.stride;
   const Teacher t = teacher_of<TAIL>(a, r, lane);
   Share sh;
-  Stat st = row_pass<T, W, false, false, TAIL>(z, a.V, a.c, a.clo, wave, lane, t.index, sh);
-  st = row_join<W>(st, wave, lane, stats);
+  Stat st = row_pass<T, W, false, false, TAIL>(z, a.V, a.c, wave, lane, t.index, sh);
+  st = row_join<W>(st, a.c, wave, lane, stats);
   if (wave) return;
   // What follows is a few operations per row, in 64 bits: a divergence close to zero is a difference of far larger terms.
   const bool used = t.index >= 0;
   const float zk = used ? (float)z[t.index] : -INFINITY;
-  const double c = (double)a.c + a.clo;
   float m = st.m;                                         // of the whole row
   double sum = st.s, listed = 0.0;
   if (TAIL) {
@@ -428,25 +426,25 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) distill_kernel(RowsArgs 
       const int other = __shfl(t.index, k, 64);
       if (k < lane && other == t.index) first = false;
     }
-    m = fmaxf(m, wave_max(zk * a.c));
-    const double mu = m == -INFINITY ? 0.0 : m;
-    listed = wave_sum(first ? (double)exp2f((float)((double)zk * c - mu)) : 0.0);
-    sum = st.s * exp2f((float)(st.m - mu));
+    m = fmaxf(m, wave_max(zk));
+    const float mu = m == -INFINITY ? 0.0f : m;
+    listed = wave_sum(first ? (double)exp2f((zk - mu) * a.c) : 0.0);
+    sum = st.s * exp2f((st.m - mu) * a.c);
   }
   const double all = sum + listed;
   // the logarithms, each in a lane of its own: of the sum, of the unlisted share of it, of the teacher's rest.  Where the unlisted
   // share is too small for the sum's scale, its own maximum counts.
   const bool far = TAIL && sum < 0x1p-100 * all;
   const double logs = log(lane == 0 ? all : lane == 1 ? (far ? (double)st.s : listed < sum ? 1.0 - listed / all : sum / all) : t.rest);
-  const double log_all = __shfl(logs, 0, 64), lse = m * kLn2Double + log_all;
+  const double log_all = __shfl(logs, 0, 64), lse = (double)m * a.scale + log_all;
   const float nan = __uint_as_float(0x7fc00000u);
-  const bool broken = !(all >= 0.0) || m == INFINITY, empty = m == -INFINITY && !broken;
-  const double lq = zk == -INFINITY ? -INFINITY : ((double)zk * c - m) * kLn2Double - log_all;
+  const bool broken = !(all >= 0.0) || m == INFINITY, empty = m * a.scale < kNothing && !broken;
+  const double lq = zk == -INFINITY ? -INFINITY : ((double)zk - m) * a.scale - log_all;
   double loss = wave_sum(t.p != 0.0 ? t.p * (t.lp - lq) : 0.0), tail = 0.0;
   if (TAIL) {
     // log of the student's probability of everything unlisted
     tail = __shfl(logs, 1, 64);
-    if (far) tail += (st.m - (double)m) * kLn2Double - log_all;
+    if (far) tail += (st.m - (double)m) * a.scale - log_all;
     if (t.rest > 0.0) loss += t.rest * (__shfl(logs, 2, 64) - tail);
   }
   if (empty) loss = t.mass != 0.0 ? INFINITY : 0.0;       // the student allows nothing
@@ -458,9 +456,9 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) distill_kernel(RowsArgs 
 }
 
 // ------------------------------------------------------------------ gradients
-// dz = coefficient * 2^(x - shift) [ * (1 + ...) ] + what the listed candidates add; one read, one write per score
+// dz = coefficient * exp(scale z - shift) [ * (1 + ...) ] + what the listed candidates add; one read, one write per score
 struct GradRow {
-  float shift, slo;  // log2 units: of lse (or of lse and the tail's probability), and what the float lacks (fp32 scores)
+  float shift, slo;  // lse (or lse and the tail's log probability), and what the float lacks (fp32 scores)
   float coef;        // of the probability
   float h, ent2;     // ENTROPY: -h p (log2 p + ent2), in log2 units
   float lshift, lslo, lcoef;   // TAIL: of a listed candidate's probability
@@ -475,12 +473,12 @@ __device__ __forceinline__ void set_shift(float &hi, float &lo, double shift) {
 
 // STREAM: written past the caches (a template: the compiler joins two stores that differ in this only)
 template <typename T, bool ENTROPY, bool TAIL, bool STREAM>
-__device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float c, float clo, const GradRow &g, int part, int parts, int lane) {
+__device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float scale, const GradRow &g, int part, int parts, int lane) {
   typedef Row<T> RW;
   constexpr int kPer = RW::kPer, kStep = 64 * kPer;
   auto exponent = [&](float f, float shift, float slo) {
-    const float x = fmaf(f, c, -shift);
-    return sizeof(T) == 4 && f != -INFINITY ? x + fmaf(f, clo, -slo) : x;
+    const float d = fmaf(f, scale, -shift);
+    return (sizeof(T) == 4 ? d - slo : d) * kLog2e;
   };
   auto grad = [&](float f) {
     const float x = exponent(f, g.shift, g.slo), p = __builtin_amdgcn_exp2f(x);
@@ -558,13 +556,13 @@ __global__ void __launch_bounds__(256) log_probs_backward_kernel(RowsArgs a) {
     else own = a.g1[(long long)r * a.N + lane];
   }
   g.add = own * a.scale;
-  set_shift(g.shift, g.slo, empty ? 0.0 : lse * kLog2eDouble);
+  set_shift(g.shift, g.slo, empty ? 0.0 : lse);
   g.coef = empty ? 0.0f : -wave_sum(own) * a.scale;
   if (ENTROPY && !empty) {
     g.h = a.g2[r] * a.scale * kLn2;
     g.ent2 = a.entropy[r] * kLog2e;
   }
-  grad_pass<T, ENTROPY, false, STREAM>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.c, a.clo, g, part, a.per_row, lane);
+  grad_pass<T, ENTROPY, false, STREAM>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.scale, g, part, a.per_row, lane);
 }
 
 template <typename T, bool TAIL, bool STREAM>
@@ -580,21 +578,21 @@ __global__ void __launch_bounds__(256) distill_backward_kernel(RowsArgs a) {
   GradRow g = {};
   g.mine = empty ? -1 : t.index;
   g.add = (float)(-gs * t.p);
-  set_shift(g.shift, g.slo, empty ? 0.0 : lse * kLog2eDouble);
+  set_shift(g.shift, g.slo, empty ? 0.0 : lse);
   g.coef = empty ? 0.0f : (float)(gs * t.mass);
   if (TAIL) {
     g.lshift = g.shift;
     g.lslo = g.slo;
     g.lcoef = g.coef;
-    // unlisted v: mass q_v - rest q_v / q_tail = (mass q_tail - rest) 2^(x - shift) with the tail's probability in the shift,
+    // unlisted v: mass q_v - rest q_v / q_tail = (mass q_tail - rest) exp(scale z - shift) with the tail's probability in the shift,
     // a probability within the tail: nothing overflows however small q_tail is
     const float tail = a.log_tail[r];
     if (!empty && tail != -INFINITY) {
-      set_shift(g.shift, g.slo, ((double)lse + tail) * kLog2eDouble);
+      set_shift(g.shift, g.slo, (double)lse + tail);
       g.coef = (float)(gs * (t.mass * expf(tail) - t.rest));
     }
   }
-  grad_pass<T, false, TAIL, STREAM>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.c, a.clo, g, part, a.per_row, lane);
+  grad_pass<T, false, TAIL, STREAM>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.scale, g, part, a.per_row, lane);
 }
 
 // ------------------------------------------------------------------ launches
@@ -688,7 +686,6 @@ RowsArgs rows_of(const urf_rows_config *c, const void *logits) {
   a.V = c->classes;
   a.scale = c->scale;
   a.c = (float)((double)c->scale * kLog2eDouble);
-  a.clo = (float)((double)c->scale * kLog2eDouble - (double)a.c);
   return a;
 }
 

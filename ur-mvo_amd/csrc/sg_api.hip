@@ -137,6 +137,8 @@ struct urf_pm {
   int rs_fallbacks = 0;                       // launches that gave up and were redone with the streaming kernels
   int rs_backoff = 0, rs_backoff_next = 64;   // streaming batches left before the resident kernel is tried again / after the next give-up
   size_t rs_xin_bytes = 0, rs_xbc_bytes = 0;
+  int z_n0 = 0, z_n1 = 0;   // Z holds the log-assignment of an urf_sg_infer call of this size (0: it does not)
+  int *d_logp = nullptr;    // urf_sg_match_log_probs: targets and results (allocated by its first call)
   int last_P = 0; bool last_Z = false, last_ransac = false;   // what the last pm_pipeline ran (pm_check_resident redoes its tail)
   int *mi0 = nullptr, *mi1 = nullptr, *idx0 = nullptr, *idx1 = nullptr, *nmatch = nullptr, *nfinal = nullptr;
   float *mv0 = nullptr, *mv1 = nullptr;
@@ -695,7 +697,7 @@ extern "C" void urf_pm_destroy(urf_pm *h) {
                     h->Ct, h->Z, h->u, h->v, h->mi0, h->mi1, h->mv0, h->mv1, h->idx0, h->idx1, h->ms0, h->ms1,
                     h->matches, h->fm_set[0], h->fm_set[1], h->fm_set[2], h->nmatch, h->nf_set[0], h->nf_set[1], h->nf_set[2], h->pts0, h->pts1, h->ps0, h->ps1, h->pn0, h->pn1, h->T, h->F,
                     h->score, h->Fbest, h->best_score, h->inliers, h->cv_scratch, (void *)h->d_slotptrs, h->rs_xin, h->rs_xbc, h->rs_err, h->ninl, h->d_sets,
-                    h->g_flags, h->rs_resid, h->rs_resid_cols};
+                    h->g_flags, h->rs_resid, h->rs_resid_cols, h->d_logp};
     for (void *p : bufs) (void)hipFree(p);
     for (int k = 0; k < urf_pm::kBegun; ++k) {
       (void)hipFree(h->bq[k].counts); (void)hipFree(h->bq[k].kxy); (void)hipFree(h->bq[k].x);
@@ -858,6 +860,7 @@ static int pm_gnn_exact(urf_pm *h, int NI, bool prof) {
 // the whole matching pipeline for P pairs whose inputs (counts, kin, kxy, x) are in place
 static int pm_pipeline(urf_pm *h, int P, bool want_Z, bool ransac) {
   hipStream_t st = h->st;
+  h->z_n0 = h->z_n1 = 0;
   const int NI = 2 * P;
   const bool prof = urf::g_profiling != 0;
   auto mark = [&](int i) { if (prof) (void)hipEventRecord(h->ev[i], st); };
@@ -1455,6 +1458,32 @@ extern "C" int urf_sg_infer(urf_pm *h, const double *f0, int n0, const double *f
     if (redo < 0) return -3;
     if (redo == 0) break;
   }
+  if (Zout) { h->z_n0 = n0; h->z_n1 = n1; }
+  return 0;
+}
+
+extern "C" int urf_sg_match_log_probs(urf_pm *h, const int *targets, int top, float *log_prob, float *entropy, int *top_index,
+                                      float *top_log_prob) {
+  URF_CHECK(h && h->built, "urf_sg_match_log_probs: matcher not built");
+  URF_CHECK(h->z_n0 > 0, "urf_sg_match_log_probs: this handle holds no log-assignment (urf_sg_infer with Zout, and no call of it since)");
+  const int n = h->z_n0, classes = h->z_n1 + 1;
+  URF_CHECK(top >= 0 && top <= URF_TOP_MAX && top <= classes, "urf_sg_match_log_probs: %d alternatives (0 .. %d, at most %d)", top, URF_TOP_MAX, classes);
+  URF_CHECK(entropy && (!targets || log_prob) && (top == 0 || (top_index && top_log_prob)), "urf_sg_match_log_probs: null pointer");
+  URF_HIP(hipSetDevice(h->device));
+  if (!h->d_logp && dalloc(&h->d_logp, (size_t)NP * (4 + 2 * URF_TOP_MAX))) return -1;
+  int *d_targets = h->d_logp, *d_index = d_targets + NP;
+  float *d_lp = (float *)(d_index + (size_t)NP * URF_TOP_MAX), *d_entropy = d_lp + NP, *d_lse = d_entropy + NP, *d_tlp = d_lse + NP;
+  if (targets) URF_HIP(hipMemcpyAsync(d_targets, targets, (size_t)n * sizeof(int), hipMemcpyHostToDevice, h->st));
+  // the rows of Z are log probabilities up to what the Sinkhorn iterations left of the row marginals: the row's own sum norms them
+  const urf_rows_config rows = {URF_F32, n, classes, LDC, 1.0f, h->device};
+  if (urf_log_probs(&rows, h->Z, d_targets, targets ? 1 : 0, top, d_lp, d_entropy, d_lse, d_index, d_tlp, h->st)) return -1;
+  if (targets) URF_HIP(hipMemcpyAsync(log_prob, d_lp, (size_t)n * sizeof(float), hipMemcpyDeviceToHost, h->st));
+  URF_HIP(hipMemcpyAsync(entropy, d_entropy, (size_t)n * sizeof(float), hipMemcpyDeviceToHost, h->st));
+  if (top) {
+    URF_HIP(hipMemcpyAsync(top_index, d_index, (size_t)n * top * sizeof(int), hipMemcpyDeviceToHost, h->st));
+    URF_HIP(hipMemcpyAsync(top_log_prob, d_tlp, (size_t)n * top * sizeof(float), hipMemcpyDeviceToHost, h->st));
+  }
+  URF_HIP(hipStreamSynchronize(h->st));
   return 0;
 }
 

@@ -292,7 +292,23 @@ class SuperGlue(_PM):
         rc = _lib.lib().urf_sg_infer(self._h, _p(f0), n0, _p(f1), n1, _p(i0), _p(i1), _p(m0), _p(m1), _p(Z))
         if rc != 0:
             return None
+        self._n0 = n0 if want_scores else 0
         return (i0, i1, m0, m1, Z) if want_scores else (i0, i1, m0, m1)
+
+    def match_log_probs(self, targets=None, top=0):
+        """How decided the last infer(..., want_scores=True) was: each keypoint of image 0 as a distribution over the keypoints of
+        image 1 and the dustbin (candidate n1).  Returns (log_prob [n0] of `targets` or None, entropy [n0], top_index [n0, top],
+        top_log_prob [n0, top])."""
+        n = getattr(self, "_n0", 0)
+        if targets is not None:
+            targets = np.ascontiguousarray(targets, np.int32)
+            if targets.shape != (n,):
+                raise ValueError(f"match_log_probs: targets has to be [{n}], one per keypoint of image 0")
+        lp = None if targets is None else np.zeros(n, np.float32)
+        entropy, index, value = np.zeros(n, np.float32), np.zeros((n, max(top, 0)), np.int32), np.zeros((n, max(top, 0)), np.float32)
+        check(_lib.lib().urf_sg_match_log_probs(self._h, _p(targets), top, _p(lp), _p(entropy), _p(index), _p(value)),
+              "urf_sg_match_log_probs")
+        return lp, entropy, index, value
 
 
 class PointMatching(_PM):
