@@ -156,7 +156,7 @@ def test_attention_gradients_against_differences(O):
 
 
 # ------------------------------------------------------------------ rows of scores
-ROWS = [(1, 1, 0), (3, 2, 0), (5, 7, 3), (4, 64, 0), (9, 1025, 3), (3, 2049, 0), (2, 9001, 0), (1, 70001, 0), (530, 2501, 5), (7, 513, 0)]
+ROWS = [(1, 1, 0), (3, 2, 0), (5, 7, 3), (4, 64, 0), (9, 1025, 3), (3, 2049, 0), (2, 9001, 0), (1, 70001, 0), (530, 2501, 5), (7, 513, 0), (4100, 300, 3), (2051, 2047, 0)]
 
 
 def rows_of(R_, V, pad, dtype, seed, masked=0.0):
@@ -187,10 +187,10 @@ def test_log_probs_and_gradients(O, rows, classes, pad, dtype, masked):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("classes", [100, 1500, 5000, 20000])
-def test_log_probs_alternatives_of_awkward_rows(O, dtype, classes):
+@pytest.mark.parametrize("classes,copies", [(100, 1), (1500, 1), (5000, 1), (20000, 1), (100, 200), (1500, 180)])
+def test_log_probs_alternatives_of_awkward_rows(O, dtype, classes, copies):
     """ties, -0 and +0, ascending and descending rows, one value everywhere, few scores that are not masked, all that is large in one
-    lane's reach, NaN, +inf, nothing at all"""
+    lane's reach, NaN, +inf, nothing at all; copies: enough rows for two a wave, different kinds side by side"""
     i = torch.arange(classes, dtype=torch.float32)
     few = torch.full((classes,), -INF)
     few[[3, classes // 2, classes - 1]] = torch.tensor([1.0, 1.0, 2.0])
@@ -199,9 +199,9 @@ def test_log_probs_alternatives_of_awkward_rows(O, dtype, classes):
     near[512:520] = 5.0
     z = torch.stack([i / classes, -i / classes, torch.zeros(classes), torch.where(i % 2 == 0, -0.0, 0.0), i % 3, few, near,
                      torch.full((classes,), -INF), torch.where(i == 7, torch.nan, i % 5), torch.where(i == classes - 1, INF, i % 5),
-                     torch.full((classes,), torch.finfo(dtype).min), torch.full((classes,), INF)]).to(dtype)
+                     torch.full((classes,), torch.finfo(dtype).min), torch.full((classes,), INF)]).to(dtype).repeat(copies, 1)
     targets = torch.full((len(z), 1), 7, dtype=torch.int32)
-    for top in (1, 20, 64):
+    for top in (1, 20, 32, 64):
         got = O.log_probs(cuda(z), cuda(targets), top=top)
         R.check(got._asdict(), R.log_probs(z, targets, top), top)
     one = torch.ones(len(z), 1)

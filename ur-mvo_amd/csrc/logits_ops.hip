@@ -8,7 +8,8 @@
 // All of it is bound by memory: a score is read once per pass, 16 bytes a lane and load, four loads in flight per lane.
 //
 // A row belongs to W waves (1, 4 or 16, one workgroup): 1 where the rows are short, 16 where there are too few rows to fill the
-// chip with 4.  Sums are joined in a fixed order.  Rows may start at any element: the loads are declared with the elements' own
+// chip with 4.  Of many short rows a wave takes two, one per half (L = 32 lanes a row): what is done once per row -- joining the
+// lanes, sorting, the row's results -- is most of the work there.  Sums are joined in a fixed order.  Rows may start at any element: the loads are declared with the elements' own
 // alignment (this hardware takes a 16-byte access at any address).
 //
 // "Listed" candidates (targets, a teacher's alternatives): at most 64 a row, one per lane of every wave.  A wave asks by ballot
@@ -57,10 +58,10 @@ template <typename T> struct Row {
     for (int e = 0; e < kPer; ++e) f[e] = (float)v[e];
   }
   // kUnroll steps from step b on: the whole vectors below `end` steps and V scores; the others are -inf
-  static __device__ __forceinline__ void fetch(const T *z, int b, int end, int V, int lane, Vec (&v)[kUnroll]) {
+  template <int L> static __device__ __forceinline__ void fetch(const T *z, int b, int end, int V, int lane, Vec (&v)[kUnroll]) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int first = (b + u) * 64 * kPer + lane * kPer;
+      const int first = (b + u) * L * kPer + lane * kPer;
 #pragma unroll
       for (int e = 0; e < kPer; ++e) v[u][e] = (T)-INFINITY;
       if (b + u < end && first + kPer <= V) v[u] = *(const Vec *)(z + first);
@@ -68,6 +69,7 @@ template <typename T> struct Row {
   }
 };
 
+typedef unsigned long long u64;
 // the value of lane ^ x, x a power of two, in the vector pipe (the LDS crossbar's latency is several times that)
 __device__ __forceinline__ int lane_xor(int v, int x) {
   const int lane = threadIdx.x;
@@ -86,20 +88,21 @@ __device__ __forceinline__ double lane_xor(double v, int x) {
   return __longlong_as_double(((long long)lane_xor((int)(u >> 32), x) << 32) | (unsigned)lane_xor((int)u, x));
 }
 
-__device__ __forceinline__ float wave_max(float v) {
+// over the L lanes of a row
+template <int L> __device__ __forceinline__ float row_max(float v) {
 #pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) v = fmaxf(v, lane_xor(v, x));
+  for (int x = L / 2; x >= 1; x >>= 1) v = fmaxf(v, lane_xor(v, x));
   return v;
 }
-__device__ __forceinline__ float wave_sum(float v) {
+template <int L, typename F> __device__ __forceinline__ F row_sum(F v) {
 #pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) v += lane_xor(v, x);
+  for (int x = L / 2; x >= 1; x >>= 1) v += lane_xor(v, x);
   return v;
 }
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) v += lane_xor(v, x);
-  return v;
+// the lanes' votes on their row's question
+template <int L> __device__ __forceinline__ u64 row_ballot(bool v) {
+  const u64 all = __ballot(v);
+  return L == 64 ? all : (threadIdx.x & 32) ? all >> 32 : all & 0xffffffffu;
 }
 
 // running maximum (of the scores) and sums of a lane, a wave, a row
@@ -110,13 +113,9 @@ __device__ __forceinline__ Stat join(Stat p, Stat q, float c) {
   // c (z - m) = c (z - p.m) + c (p.m - m)
   return {m, p.s * fp + q.s * fq, fmaf(p.s, fmaxf(xp, kFloor), p.a) * fp + fmaf(q.s, fmaxf(xq, kFloor), q.a) * fq};
 }
-__device__ __forceinline__ Stat wave_join(Stat v, float c) {
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) {
-    const Stat o = {lane_xor(v.m, x), lane_xor(v.s, x), lane_xor(v.a, x)};
-    v = (threadIdx.x & x) ? join(o, v, c) : join(v, o, c);      // the same operand order on both sides: the same bits in every lane
-  }
-  return v;
+template <int L> __device__ __forceinline__ Stat lanes_join(Stat v, float c) {
+  const float m = row_max<L>(v.m), x = (v.m - (m == -INFINITY ? 0.0f : m)) * c, f = exp2f(x);
+  return {m, row_sum<L>(v.s * f), row_sum<L>(fmaf(v.s, fmaxf(x, kFloor), v.a) * f)};
 }
 
 // ------------------------------------------------------------------ top alternatives
@@ -126,7 +125,6 @@ __device__ __forceinline__ Stat wave_join(Stat v, float c) {
 // are candidates: about K again.  They are sorted 64 at a time.  (Keeping a list during the pass costs more than the pass: 190 us
 // for 2048 rows of 100003 bf16 scores, against 129 us without alternatives.)
 // Keys: the score as an ordered integer above, the complement of its index below (equal scores: the lower index wins); 0 = none.
-typedef unsigned long long u64;
 __device__ __forceinline__ u64 key_of(float z, int index) {
   const unsigned u = __float_as_uint(z + 0.0f);           // -0 counts as 0
   const unsigned o = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
@@ -136,45 +134,52 @@ __device__ __forceinline__ float key_score(u64 k) {
   const unsigned o = (unsigned)(k >> 32);
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
-__device__ __forceinline__ u64 exchange(u64 v, int x, bool keep_max) {
-  const u64 o = ((u64)(unsigned)lane_xor((int)(v >> 32), x) << 32) | (unsigned)lane_xor((int)(unsigned)v, x);
-  return (v > o) == keep_max ? v : o;
+__device__ __forceinline__ u64 shfl64(u64 v, int src, int width) {
+  return ((u64)(unsigned)__shfl((int)(v >> 32), src, width) << 32) | (unsigned)__shfl((int)(unsigned)v, src, width);
 }
-__device__ __forceinline__ u64 sort_desc(u64 v, int lane) {
-#pragma unroll
-  for (int n = 2; n <= 64; n <<= 1)
-#pragma unroll
-    for (int x = n >> 1; x >= 1; x >>= 1) v = exchange(v, x, ((lane & n) == 0) == ((lane & x) == 0));
+// the lanes (of 64) that keep the larger of themselves and their partner lane ^ x, in runs of n that alternate in direction
+constexpr u64 keepers(int n, int x) {
+  u64 mask = 0;
+  for (int l = 0; l < 64; ++l) mask |= (u64)(((l & n) == 0) == ((l & x) == 0)) << l;
+  return mask;
+}
+template <int N, int X> __device__ __forceinline__ u64 exchange(u64 v) {
+  constexpr u64 larger = keepers(N, X);
+  const u64 o = ((u64)(unsigned)lane_xor((int)(v >> 32), X) << 32) | (unsigned)lane_xor((int)(unsigned)v, X);
+  return __builtin_amdgcn_inverse_ballot_w64(__ballot(v > o) ^ ~larger) ? v : o;
+}
+template <int N, int X> __device__ __forceinline__ u64 merge_steps(u64 v) {
+  v = exchange<N, X>(v);
+  if constexpr (X > 1) v = merge_steps<N, X / 2>(v);
   return v;
 }
-__device__ __forceinline__ u64 shfl64(u64 v, int src) {
-  return ((u64)(unsigned)__shfl((int)(v >> 32), src, 64) << 32) | (unsigned)__shfl((int)(unsigned)v, src, 64);
-}
-// both descending: the 64 largest of the two, descending
-__device__ __forceinline__ u64 merge_desc(u64 a, u64 b, int lane) {
-  const u64 r = shfl64(b, 63 - lane);
-  u64 v = a > r ? a : r;
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) v = exchange(v, x, (lane & x) == 0);
+// over the L lanes of a row, descending (N = L at the end: every lane's bit L is taken as 0, all runs descend)
+template <int L, int N = 2> __device__ __forceinline__ u64 sort_desc(u64 v) {
+  v = merge_steps<N == L ? 64 : N, N / 2>(v);
+  if constexpr (N < L) v = sort_desc<L, 2 * N>(v);
   return v;
+}
+// both descending: the L largest of the two, descending
+template <int L> __device__ __forceinline__ u64 merge_desc(u64 a, u64 b, int lane) {
+  const u64 r = shfl64(b, L - 1 - lane, L);
+  return merge_steps<64, L / 2>(a > r ? a : r);
 }
 
 // ------------------------------------------------------------------ listed candidates
 // `mine` = this lane's listed index or -1, `hits` = the lanes whose index lies in the range at hand, f = elements first + 0 .. n - 1
-template <int n> __device__ __forceinline__ void hide_listed(float *f, int first, int mine, u64 hits) {
-  while (hits) {
-    const int src = (int)__ffsll((long long)hits) - 1;
+template <int L, int n> __device__ __forceinline__ void hide_listed(float *f, int first, int mine, u64 hits) {
+  while (__any(hits != 0)) {
+    const int src = hits ? (int)__ffsll((long long)hits) - 1 : 0, index = __shfl(mine, src, L), at = hits ? index - first : -1;
     hits &= hits - 1;
-    const int at = __shfl(mine, src, 64) - first;
 #pragma unroll
     for (int e = 0; e < n; ++e)
       if (e == at) f[e] = -INFINITY;
   }
 }
 
-// what the pass of a wave over its share of a row leaves in a lane, beside the sums
+// what the pass of a wave (or half of one) over its share of a row leaves in a lane, beside the sums
 struct Share {
-  int b0, b1;        // the share: steps of 64 vectors of 16 bytes
+  int b0, b1;        // the share: steps of L vectors of 16 bytes
   float best;        // the lane's largest score (whole vectors), and the first step it was in (-1: the lane has no vector)
   int best_at;
   float extra;       // what is left of the row behind the whole vectors: one score a lane of part 0, its index or -1
@@ -183,10 +188,10 @@ struct Share {
 
 // One pass of a wave over its share of a row.  TOP: notes the lanes' best scores; TAIL: leaves the listed candidates out, so that a
 // tail far below them keeps its own maximum.
-template <typename T, int W, bool ENTROPY, bool TOP, bool TAIL>
+template <typename T, int W, int L, bool ENTROPY, bool TOP, bool TAIL>
 __device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, int lane, int mine, Share &sh) {
   typedef Row<T> RW;
-  constexpr int kPer = RW::kPer, kStep = 64 * kPer;
+  constexpr int kPer = RW::kPer, kStep = L * kPer;
   Stat st = {-INFINITY, 0.0f, 0.0f};
   auto absorb = [&](const float *f, int n) {
     float top = f[0];
@@ -205,17 +210,17 @@ __device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, i
     }
     return top;
   };
-  const int steps = (V / kPer + 63) / 64;
+  const int steps = (V / kPer + L - 1) / L;
   sh.b0 = (int)((long long)steps * part / W);
   sh.b1 = (int)((long long)steps * (part + 1) / W);
   sh.best = -INFINITY;
   sh.best_at = sh.b0 < sh.b1 && sh.b0 * kStep + (lane + 1) * kPer <= V ? sh.b0 : -1;
   typename RW::Vec now[kUnroll], next[kUnroll];
-  if (W > 1) RW::fetch(z, sh.b0, sh.b1, V, lane, now);
+  if (W > 1) RW::template fetch<L>(z, sh.b0, sh.b1, V, lane, now);
   for (int b = sh.b0; b < sh.b1; b += kUnroll) {
     // long rows: the next scores are in flight while these are taken in; short ones are one or two steps
-    if (W > 1) RW::fetch(z, b + kUnroll, sh.b1, V, lane, next);
-    else RW::fetch(z, b, sh.b1, V, lane, now);
+    if (W > 1) RW::template fetch<L>(z, b + kUnroll, sh.b1, V, lane, next);
+    else RW::template fetch<L>(z, b, sh.b1, V, lane, now);
     float f[kUnroll][kPer];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
@@ -223,8 +228,8 @@ __device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, i
         const int base = (b + u) * kStep, first = base + lane * kPer;
         RW::spread(now[u], f[u]);
         if (TAIL) {
-          const u64 hits = __ballot(mine >= base && mine < base + kStep);
-          if (hits) hide_listed<kPer>(f[u], first, mine, hits);
+          const u64 hits = row_ballot<L>(mine >= base && mine < base + kStep);
+          if (__any(hits != 0)) hide_listed<L, kPer>(f[u], first, mine, hits);
         }
         const float top = absorb(f[u], kPer);
         if (TOP && top > sh.best) { sh.best = top; sh.best_at = b + u; }
@@ -238,8 +243,8 @@ __device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, i
   if (V % kPer && part == 0) {
     if (sh.extra_at >= 0) sh.extra = (float)z[sh.extra_at];
     if (TAIL) {
-      const u64 hits = __ballot(mine >= V - V % kPer);
-      if (hits) hide_listed<1>(&sh.extra, V - V % kPer + lane, mine, hits);
+      const u64 hits = row_ballot<L>(mine >= V - V % kPer);
+      if (__any(hits != 0)) hide_listed<L, 1>(&sh.extra, V - V % kPer + lane, mine, hits);
     }
     absorb(&sh.extra, 1);
   }
@@ -254,7 +259,7 @@ template <int W> __device__ __forceinline__ u64 lists_join(u64 list, int wave, i
     lds_barrier();
     for (int n = W / 2; n >= 1; n >>= 1) {
       if (wave < n) {
-        list = merge_desc(list, lds[(wave + n) * 64 + lane], lane);
+        list = merge_desc<64>(list, lds[(wave + n) * 64 + lane], lane);
         lds[wave * 64 + lane] = list;
       }
       lds_barrier();
@@ -263,11 +268,12 @@ template <int W> __device__ __forceinline__ u64 lists_join(u64 list, int wave, i
   return list;
 }
 
-// the alternatives of a row, descending, one key per lane, in wave 0.  LDS: 64 keys per wave to join, 160 of the wave's own
-template <typename T, int W>
+// The alternatives of a row, descending, one key per lane, in wave 0 (K <= L).  LDS: 64 keys per wave to join, 2.5 L keys of the
+// row's own lanes.  What loops, loops for both rows of a wave together.
+template <typename T, int W, int L>
 __device__ __forceinline__ u64 top_alternatives(const T *z, int V, int K, const Share &sh, int wave, int lane, u64 *lds, u64 *own_lds) {
   typedef Row<T> RW;
-  constexpr int kPer = RW::kPer, kStep = 64 * kPer;
+  constexpr int kPer = RW::kPer, kStep = L * kPer;
   float f[kPer];
   u64 best = sh.extra_at >= 0 ? key_of(sh.extra, sh.extra_at) : 0;
   if (sh.best_at >= 0) {
@@ -280,36 +286,36 @@ __device__ __forceinline__ u64 top_alternatives(const T *z, int V, int K, const 
     const u64 k = key_of(sh.best, first + at);
     best = k > best ? k : best;
   }
-  u64 list = lists_join<W>(sort_desc(best, lane), wave, lane, lds);
-  u64 bound = shfl64(list, K - 1);
+  u64 list = lists_join<W>(sort_desc<L>(best), wave, lane, lds);
+  u64 bound = shfl64(list, K - 1, L);
   if constexpr (W > 1) bound = lds[K - 1];                 // wave 0's list
   // the winners' scores, (winner, step) pairs spread over the lanes
-  const u64 winners = __ballot(sh.best_at >= 0 && best >= bound);
+  const u64 winners = row_ballot<L>(sh.best_at >= 0 && best >= bound), below = (1ull << lane) - 1;
   u64 *wait = own_lds;
-  int *who = (int *)(own_lds + 128);
-  if ((winners >> lane) & 1) who[__popcll(winners & ((1ull << lane) - 1))] = lane;
+  int *who = (int *)(own_lds + 2 * L);
+  if ((winners >> lane) & 1) who[__popcll(winners & below)] = lane;
   __builtin_amdgcn_wave_barrier();
   list = 0;
   int count = 0;
-  // takes in a candidate per lane (0 = none); sorts and merges whenever 64 wait, or what there is
+  // takes in a candidate per lane (0 = none); sorts and merges whenever L wait, or what there is
   auto take = [&](u64 key, bool all) {
-    const u64 pass = __ballot(key && key >= bound);
-    if ((pass >> lane) & 1) wait[count + __popcll(pass & ((1ull << lane) - 1))] = key;
+    const u64 pass = row_ballot<L>(key && key >= bound);
+    if ((pass >> lane) & 1) wait[count + __popcll(pass & below)] = key;
     count += __popcll(pass);
-    while (count >= 64 || (all && count > 0)) {
+    while (__any(count >= L || (all && count > 0))) {
       __builtin_amdgcn_wave_barrier();
-      list = merge_desc(list, sort_desc(lane < count ? wait[lane] : 0, lane), lane);
-      const u64 rest = lane + 64 < count ? wait[lane + 64] : 0;
+      list = merge_desc<L>(list, sort_desc<L>(lane < count ? wait[lane] : 0), lane);
+      const u64 rest = lane + L < count ? wait[lane + L] : 0;
       __builtin_amdgcn_wave_barrier();
       wait[lane] = rest;
       __builtin_amdgcn_wave_barrier();
-      count = max(0, count - 64);
-      const u64 kth = shfl64(list, K - 1);
+      count = max(0, count - L);
+      const u64 kth = shfl64(list, K - 1, L);
       bound = kth > bound ? kth : bound;
     }
   };
   const int ns = sh.b1 - sh.b0, pairs = __popcll(winners) * ns;
-  for (int i0 = 0; i0 < pairs; i0 += 64) {
+  for (int i0 = 0; __any(i0 < pairs); i0 += L) {
     const int i = i0 + lane, w = i / max(ns, 1), first = (sh.b0 + i - w * ns) * kStep + (i < pairs ? who[w] : 0) * kPer;
     const bool valid = i < pairs && first + kPer <= V;
     if (valid) RW::load(z + first, f);
@@ -325,8 +331,8 @@ __device__ __forceinline__ u64 top_alternatives(const T *z, int V, int K, const 
 }
 
 // joins the parts of a row, in every wave
-template <int W> __device__ __forceinline__ Stat row_join(Stat st, float c, int wave, int lane, Stat *lds) {
-  st = wave_join(st, c);
+template <int W, int L> __device__ __forceinline__ Stat row_join(Stat st, float c, int wave, int lane, Stat *lds) {
+  st = lanes_join<L>(st, c);
   if constexpr (W > 1) {
     if (lane == 0) lds[wave] = st;
     lds_barrier();
@@ -338,20 +344,27 @@ template <int W> __device__ __forceinline__ Stat row_join(Stat st, float c, int 
 }
 
 // ------------------------------------------------------------------ forward kernels
-template <typename T, int W, bool TOP>
+// which row, wave of the row and lane of the row a thread is
+template <int W, int L> struct Place {
+  static constexpr int kRows = W > 1 ? 1 : 256 / L;        // of a workgroup
+  const int lane = threadIdx.x & (L - 1), slot = W > 1 ? 0 : threadIdx.x / L, wave = W > 1 ? threadIdx.x >> 6 : 0;
+  const int row = blockIdx.x * kRows + slot;
+};
+
+template <typename T, int W, int L, bool TOP>
 __global__ void __launch_bounds__(W == 16 ? 1024 : 256) log_probs_kernel(RowsArgs a) {
   constexpr int kWaves = W == 16 ? 16 : 4;
   __shared__ Stat stats[kWaves];
   __shared__ u64 keys[TOP ? (64 + 160) * kWaves : 1];
-  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6;
-  const int r = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
-  if (r >= a.R) return;
+  const Place<W, L> place;
+  const int lane = place.lane, wave = place.wave, r = place.row;
+  if (r >= a.R) return;                                    // (of a wave with one row to do, the other half is gone)
   const T *z = (const T *)a.z + (long long)r * a.stride;
   Share sh;
-  Stat st = row_pass<T, W, true, TOP, false>(z, a.V, a.c, wave, lane, -1, sh);
-  st = row_join<W>(st, a.c, wave, lane, stats);
+  Stat st = row_pass<T, W, L, true, TOP, false>(z, a.V, a.c, wave, lane, -1, sh);
+  st = row_join<W, L>(st, a.c, wave, lane, stats);
   u64 list = 0;
-  if constexpr (TOP) list = top_alternatives<T, W>(z, a.V, a.K, sh, wave, lane, keys, keys + 64 * kWaves + 160 * (threadIdx.x >> 6));
+  if constexpr (TOP) list = top_alternatives<T, W, L>(z, a.V, a.K, sh, wave, lane, keys, keys + 64 * kWaves + 5 * L / 2 * (threadIdx.x / L));
   if (wave) return;
   // a NaN or +inf score leaves no distribution: everything is NaN and the alternatives are -1.  A row that allows nothing: lse
   // -inf, entropy 0, every log probability -inf.
@@ -375,7 +388,7 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) log_probs_kernel(RowsArg
 // the teacher's side of a row: lane k holds alternative k (index -1 where there is none), its probability and log probability
 // (in 64 bits: what is left of 1, and of teacher and student where they agree, is a difference)
 struct Teacher { int index; double p, lp, mass, rest; };
-template <bool TAIL>
+template <bool TAIL, int L>
 __device__ __forceinline__ Teacher teacher_of(const RowsArgs &a, int r, int lane) {
   Teacher t = {-1, 0.0, 0.0, 0.0, 0.0};
   double v = -INFINITY;
@@ -387,14 +400,14 @@ __device__ __forceinline__ Teacher teacher_of(const RowsArgs &a, int r, int lane
   if (TAIL) {
     t.lp = v;
     t.p = exp(v);
-    const double sum = wave_sum(t.p);
+    const double sum = row_sum<L>(t.p);
     t.rest = fmax(1.0 - sum, 0.0);
     if (t.rest < 0x1p-20) t.rest = 0.0;                   // below the rounding of the listed probabilities: there is no rest
     t.mass = sum + t.rest;
   } else {
     v *= (double)a.scale;
-    const float m = wave_max((float)v);
-    const float e = m == -INFINITY ? 0.0f : expf((float)(v - m)), sum = wave_sum(e);
+    const float m = row_max<L>((float)v);
+    const float e = m == -INFINITY ? 0.0f : expf((float)(v - m)), sum = row_sum<L>(e);
     t.p = sum == 0.0f ? 0.0f : e / sum;
     t.lp = v - m - logf(sum);
     t.mass = sum == 0.0f ? 0.0 : sum == sum ? 1.0 : sum;
@@ -402,17 +415,17 @@ __device__ __forceinline__ Teacher teacher_of(const RowsArgs &a, int r, int lane
   return t;
 }
 
-template <typename T, int W, bool TAIL>
+template <typename T, int W, int L, bool TAIL>
 __global__ void __launch_bounds__(W == 16 ? 1024 : 256) distill_kernel(RowsArgs a) {
   __shared__ Stat stats[W];
-  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6;
-  const int r = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  const Place<W, L> place;
+  const int lane = place.lane, wave = place.wave, r = place.row;
   if (r >= a.R) return;
   const T *z = (const T *)a.z + (long long)r * a.stride;
-  const Teacher t = teacher_of<TAIL>(a, r, lane);
+  const Teacher t = teacher_of<TAIL, L>(a, r, lane);
   Share sh;
-  Stat st = row_pass<T, W, false, false, TAIL>(z, a.V, a.c, wave, lane, t.index, sh);
-  st = row_join<W>(st, a.c, wave, lane, stats);
+  Stat st = row_pass<T, W, L, false, false, TAIL>(z, a.V, a.c, wave, lane, t.index, sh);
+  st = row_join<W, L>(st, a.c, wave, lane, stats);
   if (wave) return;
   // What follows is a few operations per row, in 64 bits: a divergence close to zero is a difference of far larger terms.
   const bool used = t.index >= 0;
@@ -423,12 +436,12 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) distill_kernel(RowsArgs 
     // the pass left the listed candidates out: add each of them once
     bool first = used;
     for (int k = 0; k < a.K; ++k) {
-      const int other = __shfl(t.index, k, 64);
+      const int other = __shfl(t.index, k, L);
       if (k < lane && other == t.index) first = false;
     }
-    m = fmaxf(m, wave_max(zk));
+    m = fmaxf(m, row_max<L>(zk));
     const float mu = m == -INFINITY ? 0.0f : m;
-    listed = wave_sum(first ? (double)exp2f((zk - mu) * a.c) : 0.0);
+    listed = row_sum<L>(first ? (double)exp2f((zk - mu) * a.c) : 0.0);
     sum = st.s * exp2f((st.m - mu) * a.c);
   }
   const double all = sum + listed;
@@ -436,16 +449,16 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) distill_kernel(RowsArgs 
   // share is too small for the sum's scale, its own maximum counts.
   const bool far = TAIL && sum < 0x1p-100 * all;
   const double logs = log(lane == 0 ? all : lane == 1 ? (far ? (double)st.s : listed < sum ? 1.0 - listed / all : sum / all) : t.rest);
-  const double log_all = __shfl(logs, 0, 64), lse = (double)m * a.scale + log_all;
+  const double log_all = __shfl(logs, 0, L), lse = (double)m * a.scale + log_all;
   const float nan = __uint_as_float(0x7fc00000u);
   const bool broken = !(all >= 0.0) || m == INFINITY, empty = m * a.scale < kNothing && !broken;
   const double lq = zk == -INFINITY ? -INFINITY : ((double)zk - m) * a.scale - log_all;
-  double loss = wave_sum(t.p != 0.0 ? t.p * (t.lp - lq) : 0.0), tail = 0.0;
+  double loss = row_sum<L>(t.p != 0.0 ? t.p * (t.lp - lq) : 0.0), tail = 0.0;
   if (TAIL) {
     // log of the student's probability of everything unlisted
-    tail = __shfl(logs, 1, 64);
+    tail = __shfl(logs, 1, L);
     if (far) tail += (st.m - (double)m) * a.scale - log_all;
-    if (t.rest > 0.0) loss += t.rest * (__shfl(logs, 2, 64) - tail);
+    if (t.rest > 0.0) loss += t.rest * (__shfl(logs, 2, L) - tail);
   }
   if (empty) loss = t.mass != 0.0 ? INFINITY : 0.0;       // the student allows nothing
   if (lane == 0) {
@@ -557,7 +570,7 @@ __global__ void __launch_bounds__(256) log_probs_backward_kernel(RowsArgs a) {
   }
   g.add = own * a.scale;
   set_shift(g.shift, g.slo, empty ? 0.0 : lse);
-  g.coef = empty ? 0.0f : -wave_sum(own) * a.scale;
+  g.coef = empty ? 0.0f : -row_sum<64>(own) * a.scale;
   if (ENTROPY && !empty) {
     g.h = a.g2[r] * a.scale * kLn2;
     g.ent2 = a.entropy[r] * kLog2e;
@@ -571,7 +584,7 @@ __global__ void __launch_bounds__(256) distill_backward_kernel(RowsArgs a) {
   const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int r = a.R - 1 - (int)(w / a.per_row), part = (int)(w % a.per_row);      // the last rows, read last by the forward pass, first
   if (r < 0) return;
-  const Teacher t = teacher_of<TAIL>(a, r, lane);
+  const Teacher t = teacher_of<TAIL, 64>(a, r, lane);
   const float lse = a.lse[r];
   const double gs = (double)a.g1[r] * a.scale;
   const bool empty = lse == -INFINITY;
@@ -609,21 +622,28 @@ inline int grad_waves(int R, int V, int bytes) {
 // next pass over scores reads, which then takes 130 us instead of 100 (2048 rows of 131072 bf16 scores; 538 MB).
 inline bool streams(const RowsArgs &a, int bytes) { return (long long)a.R * a.V * bytes > (128ll << 20); }
 
+// two rows a wave where they are short and many enough to fill the chip, and one lane is enough for each entry of their lists
+inline bool two_rows(int R, int V, int lists) { return V <= 2048 && R > 2048 && lists <= 32; }
+
 template <typename T> hipError_t launch_log_probs(const RowsArgs &a, hipStream_t st) {
   const int W = row_waves(a.R, a.V);
-  const dim3 grid(W == 1 ? (a.R + 3) / 4 : a.R), block(W == 16 ? 1024 : 256);
-  auto kernel = W == 1 ? (a.K ? log_probs_kernel<T, 1, true> : log_probs_kernel<T, 1, false>)
-              : W == 4 ? (a.K ? log_probs_kernel<T, 4, true> : log_probs_kernel<T, 4, false>)
-                       : (a.K ? log_probs_kernel<T, 16, true> : log_probs_kernel<T, 16, false>);
+  const bool two = two_rows(a.R, a.V, a.K > a.N ? a.K : a.N);
+  const dim3 grid(W > 1 ? a.R : two ? (a.R + 7) / 8 : (a.R + 3) / 4), block(W == 16 ? 1024 : 256);
+  auto kernel = two ? (a.K ? log_probs_kernel<T, 1, 32, true> : log_probs_kernel<T, 1, 32, false>)
+              : W == 1 ? (a.K ? log_probs_kernel<T, 1, 64, true> : log_probs_kernel<T, 1, 64, false>)
+              : W == 4 ? (a.K ? log_probs_kernel<T, 4, 64, true> : log_probs_kernel<T, 4, 64, false>)
+                       : (a.K ? log_probs_kernel<T, 16, 64, true> : log_probs_kernel<T, 16, 64, false>);
   hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
   return hipGetLastError();
 }
 template <typename T> hipError_t launch_distill(const RowsArgs &a, bool tail, hipStream_t st) {
   const int W = row_waves(a.R, a.V);
-  const dim3 grid(W == 1 ? (a.R + 3) / 4 : a.R), block(W == 16 ? 1024 : 256);
-  auto kernel = W == 1 ? (tail ? distill_kernel<T, 1, true> : distill_kernel<T, 1, false>)
-              : W == 4 ? (tail ? distill_kernel<T, 4, true> : distill_kernel<T, 4, false>)
-                       : (tail ? distill_kernel<T, 16, true> : distill_kernel<T, 16, false>);
+  const bool two = two_rows(a.R, a.V, a.K);
+  const dim3 grid(W > 1 ? a.R : two ? (a.R + 7) / 8 : (a.R + 3) / 4), block(W == 16 ? 1024 : 256);
+  auto kernel = two ? (tail ? distill_kernel<T, 1, 32, true> : distill_kernel<T, 1, 32, false>)
+              : W == 1 ? (tail ? distill_kernel<T, 1, 64, true> : distill_kernel<T, 1, 64, false>)
+              : W == 4 ? (tail ? distill_kernel<T, 4, 64, true> : distill_kernel<T, 4, 64, false>)
+                       : (tail ? distill_kernel<T, 16, 64, true> : distill_kernel<T, 16, 64, false>);
   hipLaunchKernelGGL(kernel, grid, block, 0, st, a);
   return hipGetLastError();
 }
