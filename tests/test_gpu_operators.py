@@ -160,11 +160,13 @@ ROWS = [(1, 1, 0), (3, 2, 0), (5, 7, 3), (4, 64, 0), (9, 1025, 3), (3, 2049, 0),
 
 
 def rows_of(R_, V, pad, dtype, seed, masked=0.0):
+    """scores of rows V + pad elements apart, the first one (pad + 1) / 2 elements behind a boundary"""
     z = normal((R_, V + pad), torch.float32, seed) * 3
+    at = (pad + 1) // 2
     if masked:
         z[torch.rand(z.shape, generator=torch.Generator().manual_seed(seed + 1)) < masked] = -INF
-        z[:, 0] = 0.25
-    return z.to(dtype)[:, :V], cuda(z.to(dtype))[:, :V]
+        z[:, at] = 0.25
+    return z.to(dtype)[:, at:at + V], cuda(z.to(dtype))[:, at:at + V]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)

@@ -51,13 +51,20 @@ struct RowsArgs {
 // ------------------------------------------------------------------ rows
 template <typename T> struct Row {
   static constexpr int kPer = 16 / (int)sizeof(T);
-  typedef T Vec __attribute__((ext_vector_type(kPer), aligned(sizeof(T))));
+  typedef T Vec __attribute__((ext_vector_type(kPer)));
+  typedef T LooseVec __attribute__((ext_vector_type(kPer), aligned(sizeof(T))));      // gradients whose rows begin elsewhere
+  // scores before the first boundary: of 64 bytes, what the memory pipeline takes four lanes' vectors as, or of 16 where the lanes of a
+  // row are too few to take up to 31 scores before it and 7 behind the last vector
+  template <int L> static __device__ __forceinline__ int head(const T *z, int V) {
+    constexpr int kTo = L == 64 ? 63 : 15;
+    return min(V, (int)(-(uintptr_t)z & kTo) / (int)sizeof(T));
+  }
   static __device__ __forceinline__ void load(const T *p, float (&f)[kPer]) { spread(*(const Vec *)p, f); }
   static __device__ __forceinline__ void spread(const Vec &v, float (&f)[kPer]) {
 #pragma unroll
     for (int e = 0; e < kPer; ++e) f[e] = (float)v[e];
   }
-  // kUnroll steps from step b on: the whole vectors below `end` steps and V scores; the others are -inf
+  // kUnroll steps from step b on: the vectors below `end` steps and V scores; the others are -inf.  (z, V: from the first boundary on)
   template <int L> static __device__ __forceinline__ void fetch(const T *z, int b, int end, int V, int lane, Vec (&v)[kUnroll]) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -179,10 +186,11 @@ template <int L, int n> __device__ __forceinline__ void hide_listed(float *f, in
 
 // what the pass of a wave (or half of one) over its share of a row leaves in a lane, beside the sums
 struct Share {
+  int head;          // scores before the first vector: the vectors' scores are counted from there
   int b0, b1;        // the share: steps of L vectors of 16 bytes
   float best;        // the lane's largest score (whole vectors), and the first step it was in (-1: the lane has no vector)
   int best_at;
-  float extra;       // what is left of the row behind the whole vectors: one score a lane of part 0, its index or -1
+  float extra;       // what is left of the row before and behind the vectors: one score a lane of part 0, its index or -1
   int extra_at;
 };
 
@@ -210,6 +218,11 @@ __device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, i
     }
     return top;
   };
+  const int head = RW::template head<L>(z, V), tail = (V - head) % kPer, all = V;
+  const T *row = z;
+  z += head;
+  V -= head;
+  sh.head = head;
   const int steps = (V / kPer + L - 1) / L;
   sh.b0 = (int)((long long)steps * part / W);
   sh.b1 = (int)((long long)steps * (part + 1) / W);
@@ -225,7 +238,7 @@ __device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, i
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
       if (b + u < sh.b1) {
-        const int base = (b + u) * kStep, first = base + lane * kPer;
+        const int base = head + (b + u) * kStep, first = base + lane * kPer;
         RW::spread(now[u], f[u]);
         if (TAIL) {
           const u64 hits = row_ballot<L>(mine >= base && mine < base + kStep);
@@ -239,12 +252,12 @@ __device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, i
       for (int u = 0; u < kUnroll; ++u) now[u] = next[u];
   }
   sh.extra = -INFINITY;
-  sh.extra_at = part == 0 && lane < V % kPer ? V - V % kPer + lane : -1;
-  if (V % kPer && part == 0) {
-    if (sh.extra_at >= 0) sh.extra = (float)z[sh.extra_at];
+  sh.extra_at = part || lane >= head + tail ? -1 : lane < head ? lane : all - tail + lane - head;
+  if (part == 0 && head + tail) {
+    if (sh.extra_at >= 0) sh.extra = (float)row[sh.extra_at];
     if (TAIL) {
-      const u64 hits = row_ballot<L>(mine >= V - V % kPer);
-      if (__any(hits != 0)) hide_listed<L, 1>(&sh.extra, V - V % kPer + lane, mine, hits);
+      const u64 hits = row_ballot<L>(mine >= 0 && (mine < head || mine >= all - tail));
+      if (__any(hits != 0)) hide_listed<L, 1>(&sh.extra, sh.extra_at, mine, hits);
     }
     absorb(&sh.extra, 1);
   }
@@ -274,6 +287,9 @@ template <typename T, int W, int L>
 __device__ __forceinline__ u64 top_alternatives(const T *z, int V, int K, const Share &sh, int wave, int lane, u64 *lds, u64 *own_lds) {
   typedef Row<T> RW;
   constexpr int kPer = RW::kPer, kStep = L * kPer;
+  const int head = sh.head;
+  z += head;
+  V -= head;
   float f[kPer];
   u64 best = sh.extra_at >= 0 ? key_of(sh.extra, sh.extra_at) : 0;
   if (sh.best_at >= 0) {
@@ -283,7 +299,7 @@ __device__ __forceinline__ u64 top_alternatives(const T *z, int V, int K, const 
 #pragma unroll
     for (int e = kPer - 1; e >= 0; --e)
       if (f[e] == sh.best) at = e;
-    const u64 k = key_of(sh.best, first + at);
+    const u64 k = key_of(sh.best, head + first + at);
     best = k > best ? k : best;
   }
   u64 list = lists_join<W>(sort_desc<L>(best), wave, lane, lds);
@@ -321,7 +337,7 @@ __device__ __forceinline__ u64 top_alternatives(const T *z, int V, int K, const 
     if (valid) RW::load(z + first, f);
 #pragma unroll 1
     for (int e = 0; e < kPer; ++e) {
-      take(valid ? key_of(f[0], first + e) : 0, false);
+      take(valid ? key_of(f[0], head + first + e) : 0, false);
 #pragma unroll
       for (int x = 0; x + 1 < kPer; ++x) f[x] = f[x + 1];
     }
@@ -515,6 +531,13 @@ __device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float scale,
         if (e == at) d[e] += add;
     }
   };
+  const int head = RW::template head<64>(z, V), tail = (V - head) % kPer, all = V;
+  const T *row = z;
+  T *drow = dz;
+  z += head;
+  dz += head;
+  V -= head;
+  const bool loose = (uintptr_t)dz & 15;
   const int steps = (V / kPer + 63) / 64;
   const int b0 = (int)((long long)steps * part / parts), b1 = (int)((long long)steps * (part + 1) / parts);
   for (int b = b0; b < b1; b += kUnroll) {
@@ -527,28 +550,29 @@ __device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float scale,
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
       if (b + u < b1) {
-        const int base = (b + u) * kStep, first = base + lane * kPer;
+        const int base = head + (b + u) * kStep, first = (b + u) * kStep + lane * kPer;
         float d[kPer];
 #pragma unroll
         for (int e = 0; e < kPer; ++e) d[e] = grad(f[u][e]);
         const u64 hits = __ballot(g.mine >= base && g.mine < base + kStep);
-        if (hits) listed(f[u], d, kPer, first, hits);
+        if (hits) listed(f[u], d, kPer, head + first, hits);
         if (first + kPer <= V) {
           typename RW::Vec o;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) o[e] = (T)d[e];
-          if constexpr (STREAM) __builtin_nontemporal_store(o, (typename RW::Vec *)(dz + first));
+          if (loose) *(typename RW::LooseVec *)(dz + first) = o;
+          else if constexpr (STREAM) __builtin_nontemporal_store(o, (typename RW::Vec *)(dz + first));
           else *(typename RW::Vec *)(dz + first) = o;
         }
       }
   }
-  if (part == 0 && V % kPer) {
-    const int v = V - V % kPer + lane;
-    const float f[1] = {v < V ? (float)z[v] : -INFINITY};
+  if (part == 0 && head + tail) {
+    const int at = lane >= head + tail ? -1 : lane < head ? lane : all - tail + lane - head;
+    const float f[1] = {at >= 0 ? (float)row[at] : -INFINITY};
     float d[1] = {grad(f[0])};
-    const u64 hits = __ballot(g.mine >= V - V % kPer);
-    if (hits) listed(f, d, 1, v, hits);
-    if (v < V) dz[v] = (T)d[0];
+    const u64 hits = __ballot(g.mine >= 0 && (g.mine < head || g.mine >= all - tail));
+    if (hits) listed(f, d, 1, at, hits);
+    if (at >= 0) drow[at] = (T)d[0];
   }
 }
 
