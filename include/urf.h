@@ -608,25 +608,31 @@ typedef struct {
   int dtype;                  /* URF_F32, URF_F16, URF_BF16: of q, k, v, o and their gradients */
   int batch, q_heads, kv_heads, head_dim;   /* q_heads a multiple of kv_heads (query head h reads key head h / (q_heads / kv_heads));
                                * head_dim a multiple of 8, 8 .. 128 */
-  int q_len, k_len;           /* rows of the tensors per sequence; k_len may be 0 */
+  int q_len, k_len;           /* rows of the tensors per sequence; k_len may be 0.  With ceil32(n) = (n + 31) / 32: fewer than 2^23
+                               * batch * kv_heads * ceil32(q_len * q_heads / kv_heads) and batch * kv_heads * ceil32(k_len), and
+                               * fewer than 2^27 batch * q_heads * q_len */
   int causal;                 /* non-zero: row i of a sequence sees key j iff j <= i + (its keys - its rows), the last row the last key */
   float scale;                /* of q . k; 0 -> 1 / sqrt(head_dim) */
   int device;
 } urf_attn_config;
 /* element (b, row, head, d) at data[b * batch_stride + row * row_stride + head * head_stride + d], strides in elements, any order
- * of the dimensions; data and strides multiples of 16 bytes.  Inputs may be broadcast (stride 0). */
+ * of the dimensions; data and strides multiples of 16 bytes.  Inputs may be broadcast (stride 0); in an output every dimension
+ * steps over all of the dimensions with smaller strides. */
 typedef struct { void *data; long long batch_stride, row_stride, head_stride; } urf_attn_tensor;
 /* bytes of d_work for urf_attn_forward (backward = 0) / urf_attn_backward (1) */
 int urf_attn_workspace(const urf_attn_config *cfg, int backward, size_t *bytes);
 /* o = softmax(scale q k^T) v per head, lse[b][head][row] = log of the row's sum of exponentials (f32, contiguous).
  * d_q_lens / d_k_lens: device ints, rows / keys in use per sequence (NULL = all; values are clamped to the tensors).  What lies
- * behind them is never used, whatever it holds; o is 0 and lse -infinity in rows behind q_lens and in rows that see no key.
+ * behind them is never used, whatever it holds; o is 0 and lse -infinity in rows behind q_lens and in rows that see no key.  (A
+ * NaN or infinity among the keys in use of a causal call may reach rows before it too: a probability of 0 times it is NaN.)
  * Scores, maxima, sums and accumulators are fp32; 16-bit types round the probabilities once, for the second product. */
 int urf_attn_forward(const urf_attn_config *cfg, const urf_attn_tensor *q, const urf_attn_tensor *k, const urf_attn_tensor *v,
                      const int *d_q_lens, const int *d_k_lens, const urf_attn_tensor *o, float *d_lse, void *d_work,
                      size_t work_bytes, void *stream);
 /* gradients of sum(o * d_o) with respect to q, k and v; o and d_lse are the forward call's, the probabilities are recomputed from
- * them.  Heads that share a key head are summed into its dk and dv.  Rows behind q_lens / k_lens get 0. */
+ * them.  Heads that share a key head are summed into its dk and dv.  Rows behind q_lens / k_lens and rows that see no key get 0, and
+ * what they hold is not used.  16-bit types round the probabilities and the gradients of the scores once: of f16, d_o . v has to stay
+ * below 65504 (a scaled loss). */
 int urf_attn_backward(const urf_attn_config *cfg, const urf_attn_tensor *q, const urf_attn_tensor *k, const urf_attn_tensor *v,
                       const urf_attn_tensor *o, const float *d_lse, const urf_attn_tensor *d_o, const int *d_q_lens,
                       const int *d_k_lens, const urf_attn_tensor *dq, const urf_attn_tensor *dk, const urf_attn_tensor *dv,
@@ -635,7 +641,7 @@ int urf_attn_backward(const urf_attn_config *cfg, const urf_attn_tensor *q, cons
 #define URF_TOP_MAX 64        /* targets, alternatives or listed entries per row */
 typedef struct {
   int dtype;                  /* URF_F32, URF_F16, URF_BF16: of the scores and their gradient; everything else is f32 */
-  int rows, classes;          /* rows may be 0 */
+  int rows, classes;          /* 0 .. 2^24 - 1 rows */
   long long row_stride;       /* elements between rows of the scores (any, also 0 or less than `classes`: they are only read) */
   float scale;                /* the scores are multiplied by it first: 1 / temperature; positive */
   int device;
@@ -643,7 +649,8 @@ typedef struct {
 /* z = scale * logits of a row.  lse[row] = log sum exp z; entropy[row] of softmax(z), in nats; log_prob[row][n] = z[targets[row][n]]
  * - lse, 0 for a target outside [0, classes) (-1: none); top_index / top_log_prob[row][top]: the `top` largest scores, descending,
  * equal ones by index.  Scores may be -infinity (log probability -infinity).  A row whose largest z is below -2^100 (masks of
- * -infinity or of the lowest fp32 or bf16 value everywhere) allows nothing: lse and log probabilities -infinity, entropy 0.  A row with a NaN or +infinity has NaN everywhere and -1 as its alternatives.  d_targets may be NULL with n_targets = 0. */
+ * -infinity or of the lowest fp32 or bf16 value everywhere) allows nothing: lse and log probabilities -infinity, entropy 0.  A row
+ * with a NaN or +infinity has NaN everywhere and -1 as its alternatives.  d_targets may be NULL with n_targets = 0. */
 int urf_log_probs(const urf_rows_config *cfg, const void *logits, const int *d_targets, int n_targets, int top, float *d_log_prob,
                   float *d_entropy, float *d_lse, int *d_top_index, float *d_top_log_prob, void *stream);
 /* d_logits (rows of d_logits_stride elements) = the gradient of sum(log_prob * d_log_prob) + sum(entropy * d_entropy), from the

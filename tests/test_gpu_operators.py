@@ -108,6 +108,20 @@ def test_attention_lengths_beyond_the_tensors_are_clamped(O):
             R.attention(q, k, v, False, None, [20, 20, 0], [20, 20, 0], do))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("group", [1, 3])
+def test_attention_rows_that_see_nothing_may_hold_anything(O, dtype, group):
+    """causal with more rows than keys: the first rows' q and do are not used, in their own gradient or in the keys'"""
+    nq, nk = [150, 90, 41], [60, 0, 70]
+    q, do = (normal((3, 150, 2 * group, 64), dtype, s) for s in (1, 2))
+    k, v = (normal((3, 70, 2, 64), dtype, s) for s in (3, 4))
+    want = R.attention(q, k, v, True, None, nq, nk, do)
+    for b in range(3):
+        blind = max(0, nq[b] - nk[b])
+        q[b, :blind], do[b, :blind] = torch.nan, INF
+    R.check(run_attention(O, cuda(q), cuda(k), cuda(v), cuda(do), True, None, cuda(lens(nq)), cuda(lens(nk))), want)
+
+
 def test_attention_offsets_beyond_32_bits(O):
     """rows 2^26 elements apart: the last ones lie 5 GB behind the first"""
     L, D, step = 40, 64, 1 << 26
@@ -382,6 +396,8 @@ def test_refusals(O):
     three = torch.zeros((1, 4, 3, 64), dtype=torch.bfloat16, device="cuda")
     with pytest.raises(RuntimeError):
         O.attention(three, q, q)
+    with pytest.raises(RuntimeError):
+        O.attention(q[..., :0], q[..., :0], q[..., :0])
     none = O.log_probs(z[:0], t[:0], top=3)
     assert none.lse.shape == (0,) and none.top_index.shape == (0, 3)
     assert O.attention(q[:, :0], q, q)[0].shape == (1, 0, 2, 64)

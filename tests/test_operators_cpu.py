@@ -43,11 +43,13 @@ class Attn:
 BOTH = [dict(dtype=3), dict(dtype=-1), dict(batch=0), dict(q_len=0), dict(k_len=-1), dict(kv_heads=0), dict(kv_heads=3), dict(q_heads=0),
         dict(head_dim=0), dict(head_dim=12), dict(head_dim=136), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf),
         dict(q_p=None), dict(v_p=0), dict(q_p=(1 << 20) + 8), dict(k_sr=130), dict(v_sh=4), dict(q_sb=1), dict(lse=None),
-        dict(q_len=1 << 30, q_heads=8, kv_heads=1), dict(batch=1 << 30)]
-FORWARD = [dict(o_p=None), dict(o_p=1 << 20), dict(o_sr=0), dict(o_sh=32), dict(o_sb=0), dict(work=None, q_len=1, k_len=5000),
+        dict(q_len=1 << 30, q_heads=8, kv_heads=1), dict(batch=1 << 30), dict(batch=1 << 22, kv_heads=4), dict(q_len=1 << 27), dict(k_len=1 << 28),
+        dict(batch=1 << 15, q_len=1 << 10), dict(batch=1 << 30, q_heads=1 << 30, kv_heads=1 << 30), dict(k_len=(1 << 31) - 1)]
+FORWARD = [dict(o_p=None), dict(o_p=1 << 20), dict(o_sr=0), dict(o_sh=32), dict(o_sb=0), dict(o_sr=64), dict(o_sb=64 * 4 * 9), dict(o_sr=128, o_sh=64), dict(o_sr=64, o_sh=64 * 9),
+           dict(o_sb=-64), dict(o_sb=1 << 61), dict(work=None, q_len=1, k_len=5000),
            dict(bytes=16, q_len=1, k_len=5000), dict(work=(1 << 25) + 4, q_len=1, k_len=5000)]
 BACKWARD = [dict(do_p=None), dict(o_p=None), dict(dq_p=None), dict(dk_p=2 << 20), dict(dq_p=5 << 20), dict(dv_p=7 << 20), dict(dk_sr=0),
-            dict(dv_sb=0), dict(work=None), dict(bytes=0), dict(work=(1 << 25) + 8)]
+            dict(dv_sb=0), dict(dk_sr=64), dict(dq_sb=64 * 39), dict(work=None), dict(bytes=0), dict(work=(1 << 25) + 8)]
 
 
 @pytest.mark.parametrize("change", BOTH, ids=str)
@@ -116,7 +118,7 @@ GRAD = ["log_probs_backward", "distill_backward"]
 
 
 @pytest.mark.parametrize("calls,change", [
-    (ALL, dict(cfg=None)), (ALL, dict(dtype=7)), (ALL, dict(rows=-1)), (ALL, dict(classes=0)), (ALL, dict(classes=(1 << 31) - 1)), (ALL, dict(scale=0.0)),
+    (ALL, dict(cfg=None)), (ALL, dict(dtype=7)), (ALL, dict(rows=-1)), (ALL, dict(classes=0)), (ALL, dict(classes=(1 << 31) - 1)), (ALL, dict(scale=0.0)), (ALL, dict(rows=1 << 24, row_stride=0)),
     (ALL, dict(scale=-2.0)), (ALL, dict(scale=math.nan)), (ALL, dict(z=None)), (ALL, dict(z=4098)), (ALL, dict(lse=None)),
     (["log_probs", "log_probs_backward"], dict(n=65)), (["log_probs", "log_probs_backward"], dict(n=-1)), (["log_probs", "log_probs_backward"], dict(t=None)),
     (["log_probs"], dict(top=65)), (["log_probs"], dict(top=-1)), (["log_probs"], dict(top=51)), (["log_probs"], dict(lp=None)),
@@ -208,7 +210,7 @@ def test_reference_rows_are_autograds():
             if tail and rest >= 2.0 ** -20:
                 others = [i for i in range(30) if i not in {j for j, _ in use}]
                 loss = loss + rest * (math.log(rest) - torch.logsumexp(lq[r, others], 0))
-            assert abs(float(loss) - float(want["loss"][0][r])) < 1e-9
+            assert abs(float(torch.as_tensor(loss).detach()) - float(want["loss"][0][r])) < 1e-9
             total = total + loss * float(gh[r])
         total.backward()
         assert torch.allclose(x.grad, want["d_logits"][0], atol=1e-9)

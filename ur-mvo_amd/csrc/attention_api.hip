@@ -4,6 +4,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 namespace urf {
 hipError_t attn_forward_f32(const AttnArgs &, int, hipStream_t);
 hipError_t attn_forward_f16(const AttnArgs &, int, hipStream_t);
@@ -86,10 +88,12 @@ int check_config(const urf_attn_config *c, const char *who) {
   URF_CHECK(c->kv_heads >= 1 && c->q_heads >= 1 && c->q_heads % c->kv_heads == 0, "%s: %d query heads over %d key heads", who, c->q_heads, c->kv_heads);
   URF_CHECK(c->head_dim >= 8 && c->head_dim <= 128 && c->head_dim % 8 == 0, "%s: head size %d (a multiple of 8 up to 128)", who, c->head_dim);
   URF_CHECK(isfinite(c->scale) && c->scale >= 0.0f, "%s: scale %g", who, (double)c->scale);
-  // row and key indices and the grid are 32-bit; element offsets are 64-bit
-  const long long rows = (long long)c->q_len * (c->q_heads / c->kv_heads), groups = (long long)c->batch * c->kv_heads;
-  URF_CHECK(rows <= (1ll << 30) && c->k_len <= (1 << 30) && groups * ((rows + 31) / 32) <= (1ll << 24) * 64 && groups * ((c->k_len + 31) / 32) <= (1ll << 24) * 64 &&
-            (long long)c->batch * c->q_heads <= (1ll << 30), "%s: too many rows, keys or heads", who);
+  // row and key indices are 32-bit, element offsets 64-bit; a launch takes fewer than 2^24 workgroups of 256 threads
+  const long long most = 1ll << 23, rows = (long long)c->q_len * (c->q_heads / c->kv_heads);
+  const bool few = (long long)c->batch * c->q_heads < most;
+  const long long groups = few ? (long long)c->batch * c->kv_heads : most;
+  URF_CHECK(few && rows < most * 32 && groups * ((rows + 31) / 32) < most && groups * (((long long)c->k_len + 31) / 32) < most &&
+            (long long)c->batch * c->q_heads * c->q_len < most * 16, "%s: too many rows, keys or heads", who);
   return 0;
 }
 
@@ -104,10 +108,15 @@ int check_tensor(const urf_attn_tensor *t, const urf_attn_config *c, int len, co
 
 int check_out(const urf_attn_tensor *t, const urf_attn_config *c, int len, int heads, const char *who, const char *name) {
   if (check_tensor(t, c, len, who, name)) return -2;
-  // two elements of an output may not share memory: no stride of a dimension longer than one below the head size
-  const long long D = c->head_dim;
-  URF_CHECK((c->batch == 1 || llabs(t->batch_stride) >= D) && (len <= 1 || llabs(t->row_stride) >= D) && (heads == 1 || llabs(t->head_stride) >= D),
-            "%s: the rows of output %s overlap", who, name);
+  // two elements of an output may not share memory: each dimension, from the smallest stride up, steps over all that is below it
+  struct { long long stride, n; } dim[3] = {{llabs(t->batch_stride), c->batch}, {llabs(t->row_stride), len}, {llabs(t->head_stride), heads}};
+  std::sort(dim, dim + 3, [](const auto &x, const auto &y) { return x.stride < y.stride; });
+  long long extent = c->head_dim;
+  for (const auto &d : dim) {
+    if (d.n <= 1) continue;
+    URF_CHECK(d.stride >= extent && d.stride < (1ll << 60) / d.n, "%s: the rows of output %s overlap", who, name);
+    extent += d.stride * (d.n - 1);
+  }
   return 0;
 }
 

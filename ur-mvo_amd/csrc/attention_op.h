@@ -138,8 +138,8 @@ template <typename T, int DP> struct Tile {
 };
 
 // Copies tiles of R consecutive rows into LDS, one after the other, through registers: load() fetches the next tile, store() writes
-// it.  Rows at or behind `end` and chunks beyond the head size become zero -- what lies behind a sequence's end may be anything,
-// NaN included, and never enters a product.  Every thread walks pointers of its own: an (i, g) row advances by R rows without a
+// it.  Rows outside [low, end) and chunks beyond the head size become zero -- what lies behind a
+// sequence's end may be anything, NaN included, and never enters a product.  Every thread walks pointers of its own: an (i, g) row advances by R rows without a
 // division.
 template <typename T, int DP, int R> struct Stage {
   typedef Tile<T, DP> TL;
@@ -147,10 +147,10 @@ template <typename T, int DP, int R> struct Stage {
   static_assert(R * TL::kChunks % 256 == 0, "whole chunks per thread");
   u32x4 x[kN];
   const T *p[kN];
-  int g[kN], row, group;            // row of chunk 0; chunk n is 256 / kChunks * n rows further
+  int g[kN], row, group;            // row of chunk 0, from `low` on; chunk n is 256 / kChunks * n rows further
   long long step, wrap;
   bool inner;                       // the chunk lies within the head size
-  __device__ __forceinline__ void start(const T *head, long long srow, long long shead, int grp, int first, int D, int tid) {
+  __device__ __forceinline__ void start(const T *head, long long srow, long long shead, int grp, int first, int D, int tid, int low = 0) {
     group = grp;
     row = first + tid / TL::kChunks;
     const int c = tid % TL::kChunks;
@@ -163,13 +163,14 @@ template <typename T, int DP, int R> struct Stage {
       g[n] = r - i * grp;
       p[n] = head + (long long)i * srow + (long long)g[n] * shead + c * TL::kPer;
     }
+    row -= low;
   }
-  // DOWN: the tiles are walked towards the first row
-  template <bool DOWN = false> __device__ __forceinline__ void load(int end) {
+  // count = end - low, not negative.  DOWN: the tiles are walked towards the first row
+  template <bool DOWN = false> __device__ __forceinline__ void load(int count) {
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       x[n] = u32x4{0, 0, 0, 0};
-      if (inner && row + 256 / TL::kChunks * n < end) x[n] = *(const u32x4 *)p[n];
+      if (inner && (unsigned)(row + 256 / TL::kChunks * n) < (unsigned)count) x[n] = *(const u32x4 *)p[n];
       p[n] += DOWN ? -step : step;
       if (group > 1) {
         g[n] += DOWN ? -(R % group) : R % group;
@@ -488,6 +489,7 @@ template <typename T, int DP> __device__ __forceinline__ void attn_backward_kv(c
   int rows = tile * 128 < nk ? nq * a.G : 0;
   const int first_row = a.causal ? min(nq, max(0, key - (nk - nq))) * a.G : 0;
   const int i_min = a.causal ? min(nq, max(0, tile * 128 - (nk - nq))) : 0, diagonal = a.causal ? min(nq, max(0, tile * 128 + 127 - (nk - nq))) * a.G : 0;
+  const int low = a.causal ? max(0, nq - nk) * a.G : 0;      // rows below it see no key at all: as if they were not there
   int begin = min(i_min * a.G, rows) / kRows * kRows;
   {
     const int t = (nq * a.G + kRows - 1) / kRows, per = (t + a.kv_splits - 1) / a.kv_splits * kRows, from = (t * kRows) - (split + 1) * per;
@@ -512,19 +514,19 @@ template <typename T, int DP> __device__ __forceinline__ void attn_backward_kv(c
     }
     int r0 = (rows - 1) / kRows * kRows;
     Stage<T, DP, kRows> qs, ds;
-    qs.start((const T *)a.q.p + (long long)b * a.q.b + (long long)hk * a.G * a.q.h, a.q.r, a.q.h, a.G, r0, a.D, tid);
-    ds.start((const T *)a.dout.p + (long long)b * a.dout.b + (long long)hk * a.G * a.dout.h, a.dout.r, a.dout.h, a.G, r0, a.D, tid);
+    qs.start((const T *)a.q.p + (long long)b * a.q.b + (long long)hk * a.G * a.q.h, a.q.r, a.q.h, a.G, r0, a.D, tid, low);
+    ds.start((const T *)a.dout.p + (long long)b * a.dout.b + (long long)hk * a.G * a.dout.h, a.dout.r, a.dout.h, a.G, r0, a.D, tid, low);
     // threads 0 .. kRows - 1 carry the rows' lse, the next kRows their delta
     int stat_row = r0 + (tid & (kRows - 1)), stat_i = stat_row / a.G, stat_g = stat_row - stat_i * a.G;
     const float *stat = (tid < kRows ? a.lse : a.delta) + ((long long)b * a.Hq + hk * a.G) * a.Lq;
     float stat_next = 0.0f;
     auto load = [&]() {
-      qs.template load<true>(rows);
-      ds.template load<true>(rows);
+      qs.template load<true>(max(0, rows - low));
+      ds.template load<true>(max(0, rows - low));
       if (tid < 2 * kRows) {
         // no such row, or one that sees nothing: probabilities 0
         stat_next = tid < kRows ? INFINITY : 0.0f;
-        if (stat_row < rows) {
+        if (stat_row < rows && stat_row >= low) {
           const float x = stat[(long long)stat_g * a.Lq + stat_i];
           stat_next = tid < kRows ? (x == -INFINITY ? INFINITY : x * kLog2e) : x;
         }
@@ -624,8 +626,9 @@ template <typename T, int DP> __device__ __forceinline__ void attn_backward_q(co
   const int b = group / a.Hk, hk = group % a.Hk;
   const int nq = clamp_len(a.q_lens, b, a.Lq), nk = clamp_len(a.k_lens, b, a.Lk);
   const int row = tile * 128 + 32 * wave + col, i = row / a.G, g = row - i * a.G;
-  const bool inside = row < a.Lq * a.G, active = i < nq;
-  const int seen = !active ? 0 : a.causal ? min(nk, max(0, i + 1 + nk - nq)) : nk;
+  const bool inside = row < a.Lq * a.G;
+  const int seen = i >= nq ? 0 : a.causal ? min(nk, max(0, i + 1 + nk - nq)) : nk;
+  const bool active = seen > 0;
   const int i_last = min(nq, (min((tile + 1) * 128, a.Lq * a.G) - 1) / a.G + 1) - 1, i_first = tile * 128 / a.G;
   int block_end = i_first >= nq ? 0 : a.causal ? min(nk, max(0, i_last + 1 + nk - nq)) : nk;
   const int full_end = a.causal ? min(nk, max(0, i_first + 1 + nk - nq)) : nk;
@@ -644,7 +647,7 @@ template <typename T, int DP> __device__ __forceinline__ void attn_backward_q(co
 #pragma unroll
   for (int kc = 0; kc < kKc; ++kc) { q[kc] = load_frag<T>(qrow, active, kc, half, a.D); d[kc] = load_frag<T>(drow, active, kc, half, a.D); }
   const long long at = ((long long)b * a.Hq + h) * a.Lq + i;
-  // no such row, or one that sees nothing: probabilities 0
+  // a row that sees nothing: probabilities 0
   const float lse = active ? a.lse[at] : -INFINITY, ls = lse == -INFINITY ? INFINITY : lse * kLog2e, de = active ? a.delta[at] : 0.0f;
   f32x16 dq[kDt];
 #pragma unroll

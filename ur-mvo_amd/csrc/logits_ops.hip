@@ -701,7 +701,8 @@ namespace {
 int check_rows(const urf_rows_config *c, const void *logits, const char *who) {
   URF_CHECK(c, "%s: null configuration", who);
   URF_CHECK(dtype_bytes(c->dtype), "%s: element type %d (URF_F32, URF_F16 or URF_BF16)", who, c->dtype);
-  URF_CHECK(c->rows >= 0 && c->classes >= 1 && c->classes <= (1 << 30), "%s: %d rows of %d classes", who, c->rows, c->classes);
+  // a workgroup per row, and a launch takes fewer than 2^24 of them (of 256 threads)
+  URF_CHECK(c->rows >= 0 && c->rows < (1 << 24) && c->classes >= 1 && c->classes <= (1 << 30), "%s: %d rows of %d classes", who, c->rows, c->classes);
   URF_CHECK(isfinite(c->scale) && c->scale > 0.0f, "%s: scale %g (positive)", who, (double)c->scale);
   URF_CHECK(c->rows == 0 || logits, "%s: logits is null", who);
   URF_CHECK(((uintptr_t)logits & (dtype_bytes(c->dtype) - 1)) == 0, "%s: logits is not aligned to its elements", who);

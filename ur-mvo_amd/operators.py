@@ -112,7 +112,7 @@ def attention(q, k, v, *, causal=False, scale=None, q_lens=None, k_lens=None):
     B, Lq, Hq, _ = q.shape
     o = torch.empty(q.shape, dtype=q.dtype, device=device)
     lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=device)
-    if not q.numel():
+    if not B * Lq * Hq:
         return o, lse
     n = _workspace_bytes(cfg, 0)
     work = torch.empty(n, dtype=torch.uint8, device=device) if n else None
@@ -126,12 +126,12 @@ def attention_backward(do, q, k, v, o, lse, *, causal=False, scale=None, q_lens=
     who = "attention_backward"
     device, cfg, views, lens = _attn_config(who, q, k, v, causal, scale, q_lens, k_lens)
     B, Lq, Hq, _ = q.shape
-    if do.shape != q.shape or o.shape != q.shape:
+    if not isinstance(do, torch.Tensor) or not isinstance(o, torch.Tensor) or do.shape != q.shape or o.shape != q.shape:
         _refuse(who, "do and o have to be of q's shape")
     o_view, do_view = _head_view(who, "o", o, q.dtype, device), _head_view(who, "do", do, q.dtype, device)
     lse = _plain(who, "lse", lse, torch.float32, (B, Hq, Lq), device)
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
-    if not q.numel():
+    if not B * Lq * Hq:
         return dq, dk.zero_(), dv.zero_()
     n = _workspace_bytes(cfg, 1)
     work = torch.empty(n, dtype=torch.uint8, device=device)
