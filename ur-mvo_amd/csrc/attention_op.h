@@ -406,9 +406,9 @@ __global__ void __launch_bounds__(256, (kBlocksPerCu<T, DP>)) attn_forward_kerne
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
   const int lane = threadIdx.x & 63, rows = a.Lq * a.G;
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (w >= (long long)a.B * a.Hk * rows) return;
-  const int group = (int)(w / rows), row = (int)(w % rows), b = group / a.Hk, hk = group % a.Hk, i = row / a.G, g = row - i * a.G;
+  const unsigned w = blockIdx.x * 4 + (threadIdx.x >> 6);       // (rows of all heads: below 2^28)
+  if (w >= (unsigned)(a.B * a.Hk * rows)) return;
+  const int group = w / rows, row = w - group * rows, b = group / a.Hk, hk = group % a.Hk, i = row / a.G, g = row - i * a.G;
   const long long step = (long long)a.B * a.Hk * rows, base = w;
   float m = -INFINITY;
   for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, a.part_ml[(base + s * step) * 2]);
@@ -440,10 +440,10 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 template <typename T>
 __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a) {
   constexpr int kPer = 16 / (int)sizeof(T);
-  const long long u = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);      // row (b, i, h)
+  const unsigned u = blockIdx.x * 16 + (threadIdx.x >> 4), uh = u / a.Hq;      // row (b, i, h), (b, i)
   const int c = threadIdx.x & 15;
-  const bool inside = u < (long long)a.B * a.Lq * a.Hq;
-  const int h = (int)(u % a.Hq), i = (int)(u / a.Hq % a.Lq), b = inside ? (int)(u / a.Hq / a.Lq) : 0;
+  const bool inside = u < (unsigned)(a.B * a.Lq * a.Hq);
+  const int h = u - uh * a.Hq, b = inside ? uh / a.Lq : 0, i = uh - b * a.Lq;
   float s = 0.0f;
   if (inside && i < clamp_len(a.q_lens, b, a.Lq)) {
     const T *o = (const T *)a.o.p + (long long)b * a.o.b + (long long)i * a.o.r + (long long)h * a.o.h;
@@ -724,8 +724,9 @@ __global__ void __launch_bounds__(256, (kBlocksPerCu<T, DP>)) attn_backward_kern
 // (group, key) and of dq (group, row = i * G + g) as far as they have parts.
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) attn_sum_kernel(AttnArgs a) {
-  long long u = (long long)blockIdx.x * 256 + threadIdx.x, r = u / (DP / 4);
-  const int d = (int)(u % (DP / 4)) * 4, groups = a.B * a.Hk;
+  const long long u = (long long)blockIdx.x * 256 + threadIdx.x;
+  long long r = u / (DP / 4);
+  const int d = (int)(u - r * (DP / 4)) * 4, groups = a.B * a.Hk;
   const long long kv_rows = a.kv_splits > 1 ? (long long)groups * a.Lk : 0, q_rows = a.q_splits > 1 ? (long long)groups * a.Lq * a.G : 0;
   if (r >= 2 * kv_rows + q_rows || d >= a.D) return;
   const bool is_q = r >= 2 * kv_rows, is_v = !is_q && r >= kv_rows;
@@ -735,8 +736,15 @@ __global__ void __launch_bounds__(256) attn_sum_kernel(AttnArgs a) {
   const int splits = is_q ? a.q_splits : a.kv_splits, rows = is_q ? a.Lq * a.G : a.Lk, per_i = is_q ? a.G : 1;
   r -= is_q ? 2 * kv_rows : is_v ? kv_rows : 0;
   f32x4 s = *(const f32x4 *)(part + r * DP + d);
-  for (int n = 1; n < splits; ++n) s += *(const f32x4 *)(part + (n * all + r) * DP + d);
-  const int group = (int)(r / rows), row = (int)(r % rows), b = group / a.Hk, hk = group % a.Hk, i = row / per_i, g = row - i * per_i;
+  for (int n = 1; n < splits; n += 3) {        // three loads in flight (8.4 million sums of three parts: 19.7 -> 18.4 us)
+    f32x4 x[3];
+#pragma unroll
+    for (int e = 0; e < 3; ++e) x[e] = *(const f32x4 *)(part + (min(n + e, splits - 1) * all + r) * DP + d);
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (n + e < splits) s += x[e];
+  }
+  const int group = (unsigned)r / (unsigned)rows, row = (int)r - group * rows, b = group / a.Hk, hk = group % a.Hk, i = row / per_i, g = row - i * per_i;
   store4<T>((T *)out.p + (long long)b * out.b + (long long)i * out.r + (long long)(hk * per_i + g) * out.h + d, s[0], s[1], s[2], s[3]);
 }
 
