@@ -652,7 +652,10 @@ typedef struct {
  * -infinity or of the lowest fp32 or bf16 value everywhere) allows nothing: lse and log probabilities -infinity, entropy 0.  A row
  * with a NaN or +infinity has NaN everywhere and -1 as its alternatives.  d_targets may be NULL with n_targets = 0. */
 int urf_log_probs(const urf_rows_config *cfg, const void *logits, const int *d_targets, int n_targets, int top, float *d_log_prob,
-                  float *d_entropy, float *d_lse, int *d_top_index, float *d_top_log_prob, void *stream);
+                  float *d_entropy, float *d_lse, int *d_top_index, float *d_top_log_prob, void *d_work, size_t work_bytes,
+                  void *stream);
+/* bytes of d_work for urf_log_probs (0 for all but a few long rows) */
+int urf_log_probs_workspace(const urf_rows_config *cfg, int top, size_t *bytes);
 /* d_logits (rows of d_logits_stride elements) = the gradient of sum(log_prob * d_log_prob) + sum(entropy * d_entropy), from the
  * forward call's lse and entropy; d_entropy may be NULL.  A candidate that is a target twice gets both.  Rows that allow
  * nothing get 0. */

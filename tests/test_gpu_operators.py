@@ -170,7 +170,8 @@ def test_attention_gradients_against_differences(O):
 
 
 # ------------------------------------------------------------------ rows of scores
-ROWS = [(1, 1, 0), (3, 2, 0), (5, 7, 3), (4, 64, 0), (9, 1025, 3), (3, 2049, 0), (2, 9001, 0), (1, 70001, 0), (530, 2501, 5), (7, 513, 0), (4100, 300, 3), (2051, 2047, 0)]
+ROWS = [(1, 1, 0), (3, 2, 0), (5, 7, 3), (4, 64, 0), (9, 1025, 3), (3, 2049, 0), (2, 9001, 0), (1, 70001, 0), (530, 2501, 5), (7, 513, 0), (4100, 300, 3), (2051, 2047, 0),
+        (3, 40001, 3), (128, 32771, 1), (2, 300007, 0)]
 
 
 def rows_of(R_, V, pad, dtype, seed, masked=0.0):
@@ -203,7 +204,7 @@ def test_log_probs_and_gradients(O, rows, classes, pad, dtype, masked):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-@pytest.mark.parametrize("classes,copies", [(100, 1), (1500, 1), (5000, 1), (20000, 1), (100, 200), (1500, 180)])
+@pytest.mark.parametrize("classes,copies", [(100, 1), (1500, 1), (5000, 1), (20000, 1), (50000, 1), (100, 200), (1500, 180)])
 def test_log_probs_alternatives_of_awkward_rows(O, dtype, classes, copies):
     """ties, -0 and +0, ascending and descending rows, one value everywhere, few scores that are not masked, all that is large in one
     lane's reach, NaN, +inf, nothing at all; copies: enough rows for two a wave, different kinds side by side"""

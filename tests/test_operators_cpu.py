@@ -97,7 +97,8 @@ class Rows:
 
     def log_probs(self):
         return self.L.urf_log_probs(self.a("cfg", self.cfg), self.a("z", 4096), self.a("t", 1 << 16), self.a("n", 1), self.a("top", 3),
-                                    self.a("lp", 1 << 17), self.a("h", 1 << 18), self.a("lse", 1 << 19), self.a("ti", 1 << 20), self.a("tp", 1 << 21), None)
+                                    self.a("lp", 1 << 17), self.a("h", 1 << 18), self.a("lse", 1 << 19), self.a("ti", 1 << 20), self.a("tp", 1 << 21),
+                                    self.a("work", 1 << 25), self.a("bytes", 1 << 30), None)
 
     def log_probs_backward(self):
         return self.L.urf_log_probs_backward(self.a("cfg", self.cfg), self.a("z", 4096), self.a("t", 1 << 16), self.a("n", 1), self.a("lse", 1 << 19),
@@ -122,7 +123,8 @@ GRAD = ["log_probs_backward", "distill_backward"]
     (ALL, dict(scale=-2.0)), (ALL, dict(scale=math.nan)), (ALL, dict(z=None)), (ALL, dict(z=4098)), (ALL, dict(lse=None)),
     (["log_probs", "log_probs_backward"], dict(n=65)), (["log_probs", "log_probs_backward"], dict(n=-1)), (["log_probs", "log_probs_backward"], dict(t=None)),
     (["log_probs"], dict(top=65)), (["log_probs"], dict(top=-1)), (["log_probs"], dict(top=51)), (["log_probs"], dict(lp=None)),
-    (["log_probs"], dict(h=None)), (["log_probs"], dict(ti=None)), (["log_probs"], dict(tp=None)),
+    (["log_probs"], dict(h=None)), (["log_probs"], dict(ti=None)), (["log_probs"], dict(classes=100000, row_stride=0, work=None)),
+    (["log_probs"], dict(classes=100000, row_stride=0, bytes=1000)), (["log_probs"], dict(classes=100000, row_stride=0, work=(1 << 25) + 8)), (["log_probs"], dict(tp=None)),
     (["log_probs_backward"], dict(h=None)), (["log_probs_backward"], dict(g=None)),
     (["distill", "distill_backward"], dict(k=0)), (["distill", "distill_backward"], dict(k=65)), (["distill", "distill_backward"], dict(ix=None)),
     (["distill", "distill_backward"], dict(v=None)), (["distill", "distill_backward"], dict(lt=None)), (["distill"], dict(loss=None)),
@@ -132,6 +134,20 @@ GRAD = ["log_probs_backward", "distill_backward"]
 def test_rows_refuse(U, calls, change):
     for call in calls:
         assert getattr(Rows(U, **change), call)() == -2, call
+
+
+def test_log_probs_workspace(U):
+    L, n = U._lib.lib(), C.c_size_t()
+
+    def size(top, **c):
+        assert L.urf_log_probs_workspace(Rows(U, **c).cfg, top, C.byref(n)) == 0
+        return n.value
+
+    assert size(3) == 0 and size(3, rows=5000, classes=100000) == 0 and size(0, rows=0, classes=100000) == 0
+    assert size(5, rows=1, classes=100000) >= 2 * (5 * 8 + 12)                       # two parts at least
+    for c, top in ((dict(dtype=9), 0), (dict(), 51), (dict(), -1), (dict(), 65)):
+        assert L.urf_log_probs_workspace(Rows(U, **c).cfg, top, C.byref(n)) == -2
+    assert L.urf_log_probs_workspace(None, 0, C.byref(n)) == -2 and L.urf_log_probs_workspace(Rows(U).cfg, 0, None) == -2
 
 
 def test_rows_of_no_rows_are_nothing_to_do(U):

@@ -18,7 +18,7 @@ SYMBOLS = [
     "urf_sp_infer_device", "urf_sp_sync", "urf_slot_to_host", "urf_sp_debug_tensor", "urf_pm_create",
     "urf_pm_build", "urf_pm_build_file", "urf_pm_destroy", "urf_normalize_keypoints", "urf_sg_infer",
     "urf_match", "urf_match_device", "urf_match_device_async", "urf_pm_fetch", "urf_pm_fetch_begin", "urf_pm_fetch_ready", "urf_pm_fetch_end", "urf_pm_sync",
-    "urf_ransac_find_F", "urf_sp_stage_ms", "urf_pm_stage_ms", "urf_set_profiling", "urf_sg_match_log_probs", "urf_attn_workspace", "urf_attn_forward", "urf_attn_backward", "urf_log_probs", "urf_log_probs_backward", "urf_distill", "urf_distill_backward", "urf_probe_fma_gemm",
+    "urf_ransac_find_F", "urf_sp_stage_ms", "urf_pm_stage_ms", "urf_set_profiling", "urf_sg_match_log_probs", "urf_attn_workspace", "urf_attn_forward", "urf_attn_backward", "urf_log_probs", "urf_log_probs_workspace", "urf_log_probs_backward", "urf_distill", "urf_distill_backward", "urf_probe_fma_gemm",
     "urf_probe_math", "urf_probe_divsqrt", "urf_pm_share_stream", "urf_sp_stream", "urf_sp_result_stream", "urf_epipolar_reconstruct", "urf_probe_h2gemm", "urf_pm_wait_for_sp", "urf_pm_wait_event", "urf_sp_stage_ms_age", "urf_sp_wait_for_sinkhorn",
     "urf_cam_create", "urf_cam_create_from_maps", "urf_cam_destroy", "urf_cam_maps", "urf_cam_undistort",
     "urf_cam_undistort_device", "urf_cam_sync", "urf_cam_size",
@@ -142,7 +142,8 @@ def lib():
         L.urf_attn_workspace.argtypes = [B, I, P]
         L.urf_attn_forward.argtypes = [B] * 4 + [P, P, B, P, P, Z, P]
         L.urf_attn_backward.argtypes = [B] * 5 + [P, B, P, P, B, B, B, P, Z, P]
-        L.urf_log_probs.argtypes = [B, P, P, I, I, P, P, P, P, P, P]
+        L.urf_log_probs.argtypes = [B, P, P, I, I, P, P, P, P, P, P, Z, P]
+        L.urf_log_probs_workspace.argtypes = [B, I, P]
         L.urf_log_probs_backward.argtypes = [B, P, P, I, P, P, P, P, P, C.c_longlong, P]
         L.urf_distill.argtypes = [B, P, P, P, I, I, P, P, P, P]
         L.urf_distill_backward.argtypes = [B, P, P, P, I, I, P, P, P, P, C.c_longlong, P]

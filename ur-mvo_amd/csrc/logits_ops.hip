@@ -8,7 +8,8 @@
 // All of it is bound by memory: a score is read once per pass, 16 bytes a lane and load, four loads in flight per lane.
 //
 // A row belongs to W waves (1, 4 or 16, one workgroup): 1 where the rows are short, 16 where there are too few rows to fill the
-// chip with 4.  Of many short rows a wave takes two, one per half (L = 32 lanes a row): what is done once per row -- joining the
+// chip with 4.  A few long rows (the next token of some sequences) are cut in parts, a workgroup of 4 each, whose sums and
+// alternatives a second kernel joins.  Of many short rows a wave takes two, one per half (L = 32 lanes a row): what is done once per row -- joining the
 // lanes, sorting, the row's results -- is most of the work there.  Sums are joined in a fixed order.  Rows may start at any element: the loads are declared with the elements' own
 // alignment (this hardware takes a 16-byte access at any address).
 //
@@ -25,6 +26,7 @@ namespace urf {
 static_assert(URF_TOP_MAX == 64, "one listed candidate per lane");
 constexpr int kUnroll = 4;               // 16-byte loads in flight per lane
 constexpr double kLog2eDouble = 1.4426950408889634;
+constexpr int kMostParts = 64;           // of a row
 constexpr float kNothing = -0x1p100f;    // a row whose largest scaled score is below it allows nothing (masks of -inf or the lowest value)
 constexpr float kFloor = -1.0e4f;        // 2^kFloor is 0: a masked score (-inf) adds 0 * kFloor to A, not 0 * inf
 
@@ -46,6 +48,9 @@ struct RowsArgs {
   const float *g1, *g2;          // d_log_prob [R][N] (or d_loss [R]); d_entropy [R]
   void *dz; long long dz_stride;
   int per_row;                   // gradients: waves per row
+  // log probabilities of rows in parts: per row and part K keys, then a Stat
+  int parts;
+  unsigned long long *part_keys; struct Stat *part_stats;
 };
 
 // ------------------------------------------------------------------ rows
@@ -197,7 +202,7 @@ struct Share {
 // One pass of a wave over its share of a row.  TOP: notes the lanes' best scores; TAIL: leaves the listed candidates out, so that a
 // tail far below them keeps its own maximum.
 template <typename T, int W, int L, bool ENTROPY, bool TOP, bool TAIL>
-__device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, int lane, int mine, Share &sh) {
+__device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, int parts, int lane, int mine, Share &sh) {
   typedef Row<T> RW;
   constexpr int kPer = RW::kPer, kStep = L * kPer;
   Stat st = {-INFINITY, 0.0f, 0.0f};
@@ -224,8 +229,8 @@ __device__ __forceinline__ Stat row_pass(const T *z, int V, float c, int part, i
   V -= head;
   sh.head = head;
   const int steps = (V / kPer + L - 1) / L;
-  sh.b0 = (int)((long long)steps * part / W);
-  sh.b1 = (int)((long long)steps * (part + 1) / W);
+  sh.b0 = (int)((long long)steps * part / parts);
+  sh.b1 = (int)((long long)steps * (part + 1) / parts);
   sh.best = -INFINITY;
   sh.best_at = sh.b0 < sh.b1 && sh.b0 * kStep + (lane + 1) * kPer <= V ? sh.b0 : -1;
   typename RW::Vec now[kUnroll], next[kUnroll];
@@ -367,21 +372,9 @@ template <int W, int L> struct Place {
   const int row = blockIdx.x * kRows + slot;
 };
 
-template <typename T, int W, int L, bool TOP>
-__global__ void __launch_bounds__(W == 16 ? 1024 : 256) log_probs_kernel(RowsArgs a) {
-  constexpr int kWaves = W == 16 ? 16 : 4;
-  __shared__ Stat stats[kWaves];
-  __shared__ u64 keys[TOP ? (64 + 160) * kWaves : 1];
-  const Place<W, L> place;
-  const int lane = place.lane, wave = place.wave, r = place.row;
-  if (r >= a.R) return;                                    // (of a wave with one row to do, the other half is gone)
+// what is done once per row, by its first wave; `list`: its alternatives
+template <typename T, bool TOP> __device__ __forceinline__ void finish_log_probs(const RowsArgs &a, int r, const Stat &st, u64 list, int lane) {
   const T *z = (const T *)a.z + (long long)r * a.stride;
-  Share sh;
-  Stat st = row_pass<T, W, L, true, TOP, false>(z, a.V, a.c, wave, lane, -1, sh);
-  st = row_join<W, L>(st, a.c, wave, lane, stats);
-  u64 list = 0;
-  if constexpr (TOP) list = top_alternatives<T, W, L>(z, a.V, a.K, sh, wave, lane, keys, keys + 64 * kWaves + 5 * L / 2 * (threadIdx.x / L));
-  if (wave) return;
   // a NaN or +inf score leaves no distribution: everything is NaN and the alternatives are -1.  A row that allows nothing: lse
   // -inf, entropy 0, every log probability -inf.
   const bool broken = !(st.s >= 0.0f) || st.m == INFINITY, empty = st.m * a.scale < kNothing && !broken;
@@ -399,6 +392,66 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) log_probs_kernel(RowsArg
     a.top_index[(long long)r * a.K + lane] = broken ? -1 : (int)~(unsigned)list;
     a.top_log_prob[(long long)r * a.K + lane] = log_prob(key_score(list));
   }
+}
+
+template <typename T, int W, int L, bool TOP>
+__global__ void __launch_bounds__(W == 16 ? 1024 : 256) log_probs_kernel(RowsArgs a) {
+  constexpr int kWaves = W == 16 ? 16 : 4;
+  __shared__ Stat stats[kWaves];
+  __shared__ u64 keys[TOP ? (64 + 160) * kWaves : 1];
+  const Place<W, L> place;
+  const int lane = place.lane, wave = place.wave, r = place.row;
+  if (r >= a.R) return;                                    // (of a wave with one row to do, the other half is gone)
+  const T *z = (const T *)a.z + (long long)r * a.stride;
+  Share sh;
+  Stat st = row_pass<T, W, L, true, TOP, false>(z, a.V, a.c, wave, W, lane, -1, sh);
+  st = row_join<W, L>(st, a.c, wave, lane, stats);
+  u64 list = 0;
+  if constexpr (TOP) list = top_alternatives<T, W, L>(z, a.V, a.K, sh, wave, lane, keys, keys + 64 * kWaves + 5 * L / 2 * (threadIdx.x / L));
+  if (wave) return;
+  finish_log_probs<T, TOP>(a, r, st, list, lane);
+}
+
+// A row in parts, and their join: a workgroup per row, lane p of a wave holds part p's sums, a wave merges the lists of every
+// fourth part.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(256) log_probs_part_kernel(RowsArgs a) {
+  __shared__ Stat stats[4];
+  __shared__ u64 keys[TOP ? (64 + 160) * 4 : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x / a.parts, part = blockIdx.x - r * a.parts;
+  const T *z = (const T *)a.z + (long long)r * a.stride;
+  Share sh;
+  Stat st = row_pass<T, 4, 64, true, TOP, false>(z, a.V, a.c, 4 * part + wave, 4 * a.parts, lane, -1, sh);
+  st = row_join<4, 64>(st, a.c, wave, lane, stats);
+  u64 list = 0;
+  if constexpr (TOP) list = top_alternatives<T, 4, 64>(z, a.V, a.K, sh, wave, lane, keys, keys + 64 * 4 + 160 * wave);
+  if (wave) return;
+  if (lane == 0) a.part_stats[blockIdx.x] = st;
+  if (TOP && lane < a.K) a.part_keys[(long long)blockIdx.x * a.K + lane] = list;
+}
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(256) log_probs_join_kernel(RowsArgs a) {
+  __shared__ u64 keys[TOP ? 64 * 4 : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x;
+  Stat st = {-INFINITY, 0.0f, 0.0f};
+  if (lane < a.parts) st = a.part_stats[r * a.parts + lane];
+  u64 list = 0;
+  if constexpr (TOP) {
+    u64 lists[kMostParts / 4];                              // parts wave, wave + 4, ...
+#pragma unroll
+    for (int i = 0; i < kMostParts / 4; ++i) {
+      const int p = wave + 4 * i;
+      lists[i] = p < a.parts && lane < a.K ? a.part_keys[((long long)r * a.parts + p) * a.K + lane] : 0;
+    }
+#pragma unroll
+    for (int n = kMostParts / 8; n >= 1; n >>= 1)
+#pragma unroll
+      for (int i = 0; i < n; ++i)
+        if (wave + 4 * (i + n) < a.parts) lists[i] = merge_desc<64>(lists[i], lists[i + n], lane);
+    list = lists_join<4>(lists[0], wave, lane, keys);
+  }
+  if (wave) return;
+  finish_log_probs<T, TOP>(a, r, lanes_join<64>(st, a.c), list, lane);
 }
 
 // the teacher's side of a row: lane k holds alternative k (index -1 where there is none), its probability and log probability
@@ -440,7 +493,7 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) distill_kernel(RowsArgs 
   const T *z = (const T *)a.z + (long long)r * a.stride;
   const Teacher t = teacher_of<TAIL, L>(a, r, lane);
   Share sh;
-  Stat st = row_pass<T, W, L, false, false, TAIL>(z, a.V, a.c, wave, lane, t.index, sh);
+  Stat st = row_pass<T, W, L, false, false, TAIL>(z, a.V, a.c, wave, W, lane, t.index, sh);
   st = row_join<W, L>(st, a.c, wave, lane, stats);
   if (wave) return;
   // What follows is a few operations per row, in 64 bits: a divergence close to zero is a difference of far larger terms.
@@ -635,6 +688,17 @@ __global__ void __launch_bounds__(256) distill_backward_kernel(RowsArgs a) {
 // ------------------------------------------------------------------ launches
 // waves per row: one for short rows; sixteen where four per row would leave the 256 CUs with less than two workgroups each
 inline int row_waves(int R, int V) { return V <= 2048 ? 1 : R <= 512 && V > 8192 ? 16 : 4; }
+// Parts per row, two workgroups per CU and at least 4096 scores each; 0 = one workgroup does a row.  One launch against two, bf16, us
+// without / with 20 alternatives: 1 row of 131072: 13.1 / 22.5 -> 5.1 / 13.0 (parts of 2048: 5.0 / 14.8); 64: 13.9 / 23.7 -> 8.2 / 16.7;
+// 128: 14.5 / 24.2 -> 11.9 / 22.8; 256: 21.0 / 27.8 -> 19.6 / 34.0; rows of 20001: 1: 5.4 / 13.3 -> 5.1 / 11.3, 128: 6.0 / 14.6 -> 6.3 /
+// 13.2; rows of 10001: 128: 5.4 / 13.9 -> 6.1 / 12.8.
+inline int row_parts(int R, int V) {
+  if (V < 16384 || R > 128) return 0;
+  const int by_size = V / 4096, fill = 512 / R, n = by_size < fill ? by_size : fill;
+  return n > kMostParts ? kMostParts : n;
+}
+inline size_t log_probs_bytes(int R, int V, int K) { return (size_t)R * row_parts(R, V) * (K * sizeof(u64) + sizeof(Stat)); }
+
 // gradients: a wave takes about 16 KiB of scores, less where that leaves waves to spare
 inline int grad_waves(int R, int V, int bytes) {
   const long long by_size = ((long long)V * bytes + 16383) / 16384, steps = (long long)V * bytes / 1024;
@@ -650,6 +714,15 @@ inline bool streams(const RowsArgs &a, int bytes) { return (long long)a.R * a.V 
 inline bool two_rows(int R, int V, int lists) { return V <= 2048 && R > 2048 && lists <= 32; }
 
 template <typename T> hipError_t launch_log_probs(const RowsArgs &a, hipStream_t st) {
+  if (a.parts) {
+    auto part = a.K ? log_probs_part_kernel<T, true> : log_probs_part_kernel<T, false>;
+    auto join = a.K ? log_probs_join_kernel<T, true> : log_probs_join_kernel<T, false>;
+    hipLaunchKernelGGL(part, dim3(a.R * a.parts), dim3(256), 0, st, a);
+    const hipError_t rc = hipGetLastError();
+    if (rc != hipSuccess) return rc;
+    hipLaunchKernelGGL(join, dim3(a.R), dim3(256), 0, st, a);
+    return hipGetLastError();
+  }
   const int W = row_waves(a.R, a.V);
   const bool two = two_rows(a.R, a.V, a.K > a.N ? a.K : a.N);
   const dim3 grid(W > 1 ? a.R : two ? (a.R + 7) / 8 : (a.R + 3) / 4), block(W == 16 ? 1024 : 256);
@@ -698,12 +771,17 @@ namespace {
 #define URF_BY_TYPE(dtype, f, ...) \
   ((dtype) == URF_F32 ? f<float>(__VA_ARGS__) : (dtype) == URF_F16 ? f<_Float16>(__VA_ARGS__) : f<__bf16>(__VA_ARGS__))
 
-int check_rows(const urf_rows_config *c, const void *logits, const char *who) {
+int check_config(const urf_rows_config *c, const char *who) {
   URF_CHECK(c, "%s: null configuration", who);
   URF_CHECK(dtype_bytes(c->dtype), "%s: element type %d (URF_F32, URF_F16 or URF_BF16)", who, c->dtype);
   // a workgroup per row, and a launch takes fewer than 2^24 of them (of 256 threads)
   URF_CHECK(c->rows >= 0 && c->rows < (1 << 24) && c->classes >= 1 && c->classes <= (1 << 30), "%s: %d rows of %d classes", who, c->rows, c->classes);
   URF_CHECK(isfinite(c->scale) && c->scale > 0.0f, "%s: scale %g (positive)", who, (double)c->scale);
+  return 0;
+}
+
+int check_rows(const urf_rows_config *c, const void *logits, const char *who) {
+  if (check_config(c, who)) return -2;
   URF_CHECK(c->rows == 0 || logits, "%s: logits is null", who);
   URF_CHECK(((uintptr_t)logits & (dtype_bytes(c->dtype) - 1)) == 0, "%s: logits is not aligned to its elements", who);
   return 0;
@@ -736,17 +814,35 @@ RowsArgs rows_of(const urf_rows_config *c, const void *logits) {
 
 }  // namespace
 
-extern "C" int urf_log_probs(const urf_rows_config *cfg, const void *logits, const int *d_targets, int n_targets, int top,
-                             float *d_log_prob, float *d_entropy, float *d_lse, int *d_top_index, float *d_top_log_prob, void *stream) {
-  const char *who = "urf_log_probs";
-  if (check_rows(cfg, logits, who)) return -2;
-  URF_CHECK(n_targets >= 0 && n_targets <= URF_TOP_MAX, "%s: %d targets per row (0 .. %d)", who, n_targets, URF_TOP_MAX);
+static int check_top(const urf_rows_config *cfg, int top, const char *who) {
   URF_CHECK(top >= 0 && top <= URF_TOP_MAX && top <= cfg->classes, "%s: %d alternatives (0 .. %d, at most the %d classes)", who, top, URF_TOP_MAX, cfg->classes);
+  return 0;
+}
+
+extern "C" int urf_log_probs_workspace(const urf_rows_config *cfg, int top, size_t *bytes) {
+  const char *who = "urf_log_probs_workspace";
+  if (check_config(cfg, who) || check_top(cfg, top, who)) return -2;
+  URF_CHECK(bytes, "%s: null pointer", who);
+  *bytes = cfg->rows ? log_probs_bytes(cfg->rows, cfg->classes, top) : 0;
+  return 0;
+}
+
+extern "C" int urf_log_probs(const urf_rows_config *cfg, const void *logits, const int *d_targets, int n_targets, int top,
+                             float *d_log_prob, float *d_entropy, float *d_lse, int *d_top_index, float *d_top_log_prob, void *d_work,
+                             size_t work_bytes, void *stream) {
+  const char *who = "urf_log_probs";
+  if (check_rows(cfg, logits, who) || check_top(cfg, top, who)) return -2;
+  URF_CHECK(n_targets >= 0 && n_targets <= URF_TOP_MAX, "%s: %d targets per row (0 .. %d)", who, n_targets, URF_TOP_MAX);
   if (cfg->rows == 0) return 0;
+  const size_t need = log_probs_bytes(cfg->rows, cfg->classes, top);
+  URF_CHECK(need == 0 || (d_work && work_bytes >= need && ((uintptr_t)d_work & 15) == 0), "%s: workspace of %zu bytes, %zu needed", who, work_bytes, need);
   URF_CHECK(d_entropy && d_lse && (n_targets == 0 || (d_targets && d_log_prob)) && (top == 0 || (d_top_index && d_top_log_prob)), "%s: null pointer", who);
   RowsArgs a = rows_of(cfg, logits);
   a.targets = d_targets; a.N = n_targets; a.K = top;
   a.log_prob = d_log_prob; a.entropy = d_entropy; a.lse = d_lse; a.top_index = d_top_index; a.top_log_prob = d_top_log_prob;
+  a.parts = row_parts(cfg->rows, cfg->classes);
+  a.part_keys = (u64 *)d_work;
+  a.part_stats = (Stat *)(a.part_keys + (size_t)cfg->rows * a.parts * top);
   OnDevice on(cfg->device);
   URF_HIP(on.rc);
   URF_HIP(URF_BY_TYPE(cfg->dtype, launch_log_probs, a, (hipStream_t)stream));

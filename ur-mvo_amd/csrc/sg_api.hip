@@ -1476,7 +1476,7 @@ extern "C" int urf_sg_match_log_probs(urf_pm *h, const int *targets, int top, fl
   if (targets) URF_HIP(hipMemcpyAsync(d_targets, targets, (size_t)n * sizeof(int), hipMemcpyHostToDevice, h->st));
   // the rows of Z are log probabilities up to what the Sinkhorn iterations left of the row marginals: the row's own sum norms them
   const urf_rows_config rows = {URF_F32, n, classes, LDC, 1.0f, h->device};
-  if (urf_log_probs(&rows, h->Z, d_targets, targets ? 1 : 0, top, d_lp, d_entropy, d_lse, d_index, d_tlp, h->st)) return -1;
+  if (urf_log_probs(&rows, h->Z, d_targets, targets ? 1 : 0, top, d_lp, d_entropy, d_lse, d_index, d_tlp, nullptr, 0, h->st)) return -1;      // (1024 rows at most and short: no workspace)
   if (targets) URF_HIP(hipMemcpyAsync(log_prob, d_lp, (size_t)n * sizeof(float), hipMemcpyDeviceToHost, h->st));
   URF_HIP(hipMemcpyAsync(entropy, d_entropy, (size_t)n * sizeof(float), hipMemcpyDeviceToHost, h->st));
   if (top) {

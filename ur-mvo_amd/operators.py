@@ -154,6 +154,13 @@ def _rows_config(who, logits, scale):
     return device, R, V, _ROWS_CONFIG.pack(DTYPES[logits.dtype], R, V, sr, scale, device.index)
 
 
+@functools.lru_cache(maxsize=1024)
+def _log_probs_workspace(cfg, top):
+    n = _lib.C.c_size_t()
+    check(_lib.lib().urf_log_probs_workspace(cfg, top, _lib.C.byref(n)), "urf_log_probs_workspace")
+    return n.value
+
+
 def _targets(who, targets, R, device):
     """how many per row, and their address"""
     if targets is None:
@@ -179,9 +186,11 @@ def log_probs(logits, targets=None, *, top=0, scale=1.0):
     log_prob = None if targets is None else torch.empty(targets.shape, dtype=torch.float32, device=device)
     top_index = torch.empty((R, top), dtype=torch.int32, device=device) if top else None
     top_log_prob = torch.empty((R, top), dtype=torch.float32, device=device) if top else None
+    size = _log_probs_workspace(cfg, top)
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     check(_lib.lib().urf_log_probs(cfg, logits.data_ptr(), at, n, top, log_prob.data_ptr() if n else None, entropy.data_ptr(),
                                    lse.data_ptr(), top_index.data_ptr() if top else None, top_log_prob.data_ptr() if top else None,
-                                   _stream(device)), "urf_log_probs")
+                                   work.data_ptr() if size else None, size, _stream(device)), "urf_log_probs")
     return LogProbs(log_prob, entropy, lse, top_index, top_log_prob)
 
 
