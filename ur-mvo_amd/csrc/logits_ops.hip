@@ -26,7 +26,7 @@ namespace urf {
 static_assert(URF_TOP_MAX == 64, "one listed candidate per lane");
 constexpr int kUnroll = 4;               // 16-byte loads in flight per lane
 constexpr double kLog2eDouble = 1.4426950408889634;
-constexpr int kMostParts = 64;           // of a row
+constexpr int kMostParts = 32;           // of a row
 constexpr float kNothing = -0x1p100f;    // a row whose largest scaled score is below it allows nothing (masks of -inf or the lowest value)
 constexpr float kFloor = -1.0e4f;        // 2^kFloor is 0: a masked score (-inf) adds 0 * kFloor to A, not 0 * inf
 
@@ -686,32 +686,48 @@ __global__ void __launch_bounds__(256) distill_backward_kernel(RowsArgs a) {
 }
 
 // ------------------------------------------------------------------ launches
-// waves per row: one for short rows; sixteen where four per row would leave the 256 CUs with less than two workgroups each
-inline int row_waves(int R, int V) { return V <= 2048 ? 1 : R <= 512 && V > 8192 ? 16 : 4; }
-// Parts per row, two workgroups per CU and at least 4096 scores each; 0 = one workgroup does a row.  One launch against two, bf16, us
-// without / with 20 alternatives: 1 row of 131072: 13.1 / 22.5 -> 5.1 / 13.0 (parts of 2048: 5.0 / 14.8); 64: 13.9 / 23.7 -> 8.2 / 16.7;
-// 128: 14.5 / 24.2 -> 11.9 / 22.8; 256: 21.0 / 27.8 -> 19.6 / 34.0; rows of 20001: 1: 5.4 / 13.3 -> 5.1 / 11.3, 128: 6.0 / 14.6 -> 6.3 /
-// 13.2; rows of 10001: 128: 5.4 / 13.9 -> 6.1 / 12.8.
-inline int row_parts(int R, int V) {
-  if (V < 16384 || R > 128) return 0;
-  const int by_size = V / 4096, fill = 512 / R, n = by_size < fill ? by_size : fill;
-  return n > kMostParts ? kMostParts : n;
+// Waves per row.  One for short rows and, the more rows there are, for longer ones (what is done once per row, the alternatives most of
+// all, costs every wave); sixteen for long rows where four would leave CUs with less than two workgroups.  bf16, us for the
+// sums / with 8 alternatives / distillation: 512 rows of 3000: 4.5 / 8.5 / 4.8 with one wave, 4.3 / 9.9 / 4.9 with four, 8.5 / 23.8 / 7.8
+// with sixteen; 8192 rows of 12000: 35 / 61 / 35, 39 / 76 / 40, 131 / 382 / 97; 1024 rows of 24000: 17.6 / 31 / 16.3, 13.9 / 22 / 13.8,
+// 22 / 53 / 17; 256 rows of 131072: 73 / 109 / 65, 23 / 32 / 22, 20 / 27 / 19; 256 rows of 24000: 14 / 26 / 13, 6.1 / 12.4 / 6.4, 6.4 / 15 / 6.9.
+inline int row_waves(int R, int V, int bytes) {
+  const long long size = (long long)V * bytes, one = 16ll * R < 6144 ? 6144 : 16ll * R < 32768 ? 16ll * R : 32768;
+  return size <= one ? 1 : R <= 256 && size > 96 * 1024 ? 16 : 4;
 }
-inline size_t log_probs_bytes(int R, int V, int K) { return (size_t)R * row_parts(R, V) * (K * sizeof(u64) + sizeof(Stat)); }
+// Parts per row, two workgroups per CU and at least 8 KiB each; 0 = one workgroup does a row.  One launch against two, bf16, us
+// without / with 20 alternatives: 1 row of 131072: 13.1 / 22.5 -> 5.1 / 13.0; 64: 13.9 / 23.7 -> 8.2 / 16.7; 128: 14.5 / 24.2 -> 11.9 / 22.8;
+// 256: 21.0 / 27.8 -> 19.6 / 34.0; with 8 alternatives 32 rows of 48000: 9.3 / 15.6 -> 6.7 / 13.5; 128 of 24000: 6.0 / 11.2 -> 6.7 / 13.2.
+// More parts cost their joining: 1 row of 131072 in 64 of 4 KiB: 5.0 / 14.8.
+inline int row_parts(int R, int V, int bytes) {
+  const long long size = (long long)V * bytes;
+  if (size < 64 * 1024 || R > 128) return 0;
+  const long long by_size = size / 8192, fill = 512 / R, n = by_size < fill ? by_size : fill;
+  return n > kMostParts ? kMostParts : (int)n;
+}
+inline size_t log_probs_bytes(int R, int V, int bytes, int K) { return (size_t)R * row_parts(R, V, bytes) * (K * sizeof(u64) + sizeof(Stat)); }
 
-// gradients: a wave takes about 16 KiB of scores, less where that leaves waves to spare
+// Gradients: a wave takes about 8 KiB of scores, less where that leaves waves to spare.  (2048 rows of 131072, bf16, log probabilities:
+// 195 us with 4 KiB, 181 with 8, 193 with 16, 222 with 64; 8192 rows of 2500: 18.4, 16.9, 16.9, 16.9; one row of 131072: 3.0, 8.4 without the
+// second rule.)
 inline int grad_waves(int R, int V, int bytes) {
-  const long long by_size = ((long long)V * bytes + 16383) / 16384, steps = (long long)V * bytes / 1024;
+  const long long by_size = ((long long)V * bytes + 8191) / 8192, steps = (long long)V * bytes / 1024;
   const long long fill = (4096 + R - 1) / R, n = by_size > fill ? by_size : fill;
   return (int)(n < 1 || steps < 1 ? 1 : n > steps ? steps : n);
 }
 
 // A gradient beyond half of the 256 MB of the last-level cache is written past it: left there, its lines are written back while the
-// next pass over scores reads, which then takes 130 us instead of 100 (2048 rows of 131072 bf16 scores; 538 MB).
+// next pass over scores reads (distillation and its gradient, 2048 rows of 131072 bf16 scores, 538 MB: 310 us instead of 281).
 inline bool streams(const RowsArgs &a, int bytes) { return (long long)a.R * a.V * bytes > (128ll << 20); }
 
-// two rows a wave where they are short and many enough to fill the chip, and one lane is enough for each entry of their lists
-inline bool two_rows(int R, int V, int lists) { return V <= 2048 && R > 2048 && lists <= 32; }
+// Two rows a wave where they are short and many enough to fill the chip, and one lane is enough for each entry of their lists.  fp32, us
+// for the sums / with 8 alternatives / distillation: 8192 rows of 1000: 7.5 / 13.4 / 8.2 against 8.2 / 17.3 / 10.0 with one; 30000 of 200:
+// 7.9 / 21 / 12.8 against 13.0 / 39 / 22.6; 3000 of 2047: 8.0 / 14.9 / 8.2 against 5.8 / 10.5 / 6.2; bf16, 2048 of 1000: 3.8 / 7.3 / 4.3 against
+// 4.1 / 8.0 / 4.5.
+inline bool two_rows(int R, int V, int lists, int bytes) {
+  const long long size = (long long)V * bytes;
+  return R >= 2048 && size <= 6144 && 2 * size <= 3ll * R && lists <= 32;
+}
 
 template <typename T> hipError_t launch_log_probs(const RowsArgs &a, hipStream_t st) {
   if (a.parts) {
@@ -723,8 +739,8 @@ template <typename T> hipError_t launch_log_probs(const RowsArgs &a, hipStream_t
     hipLaunchKernelGGL(join, dim3(a.R), dim3(256), 0, st, a);
     return hipGetLastError();
   }
-  const int W = row_waves(a.R, a.V);
-  const bool two = two_rows(a.R, a.V, a.K > a.N ? a.K : a.N);
+  const int W = row_waves(a.R, a.V, sizeof(T));
+  const bool two = two_rows(a.R, a.V, a.K > a.N ? a.K : a.N, sizeof(T));
   const dim3 grid(W > 1 ? a.R : two ? (a.R + 7) / 8 : (a.R + 3) / 4), block(W == 16 ? 1024 : 256);
   auto kernel = two ? (a.K ? log_probs_kernel<T, 1, 32, true> : log_probs_kernel<T, 1, 32, false>)
               : W == 1 ? (a.K ? log_probs_kernel<T, 1, 64, true> : log_probs_kernel<T, 1, 64, false>)
@@ -734,8 +750,8 @@ template <typename T> hipError_t launch_log_probs(const RowsArgs &a, hipStream_t
   return hipGetLastError();
 }
 template <typename T> hipError_t launch_distill(const RowsArgs &a, bool tail, hipStream_t st) {
-  const int W = row_waves(a.R, a.V);
-  const bool two = two_rows(a.R, a.V, a.K);
+  const int W = row_waves(a.R, a.V, sizeof(T));
+  const bool two = two_rows(a.R, a.V, a.K, sizeof(T));
   const dim3 grid(W > 1 ? a.R : two ? (a.R + 7) / 8 : (a.R + 3) / 4), block(W == 16 ? 1024 : 256);
   auto kernel = two ? (tail ? distill_kernel<T, 1, 32, true> : distill_kernel<T, 1, 32, false>)
               : W == 1 ? (tail ? distill_kernel<T, 1, 64, true> : distill_kernel<T, 1, 64, false>)
@@ -823,7 +839,7 @@ extern "C" int urf_log_probs_workspace(const urf_rows_config *cfg, int top, size
   const char *who = "urf_log_probs_workspace";
   if (check_config(cfg, who) || check_top(cfg, top, who)) return -2;
   URF_CHECK(bytes, "%s: null pointer", who);
-  *bytes = cfg->rows ? log_probs_bytes(cfg->rows, cfg->classes, top) : 0;
+  *bytes = cfg->rows ? log_probs_bytes(cfg->rows, cfg->classes, dtype_bytes(cfg->dtype), top) : 0;
   return 0;
 }
 
@@ -834,13 +850,13 @@ extern "C" int urf_log_probs(const urf_rows_config *cfg, const void *logits, con
   if (check_rows(cfg, logits, who) || check_top(cfg, top, who)) return -2;
   URF_CHECK(n_targets >= 0 && n_targets <= URF_TOP_MAX, "%s: %d targets per row (0 .. %d)", who, n_targets, URF_TOP_MAX);
   if (cfg->rows == 0) return 0;
-  const size_t need = log_probs_bytes(cfg->rows, cfg->classes, top);
+  const size_t need = log_probs_bytes(cfg->rows, cfg->classes, dtype_bytes(cfg->dtype), top);
   URF_CHECK(need == 0 || (d_work && work_bytes >= need && ((uintptr_t)d_work & 15) == 0), "%s: workspace of %zu bytes, %zu needed", who, work_bytes, need);
   URF_CHECK(d_entropy && d_lse && (n_targets == 0 || (d_targets && d_log_prob)) && (top == 0 || (d_top_index && d_top_log_prob)), "%s: null pointer", who);
   RowsArgs a = rows_of(cfg, logits);
   a.targets = d_targets; a.N = n_targets; a.K = top;
   a.log_prob = d_log_prob; a.entropy = d_entropy; a.lse = d_lse; a.top_index = d_top_index; a.top_log_prob = d_top_log_prob;
-  a.parts = row_parts(cfg->rows, cfg->classes);
+  a.parts = row_parts(cfg->rows, cfg->classes, dtype_bytes(cfg->dtype));
   a.part_keys = (u64 *)d_work;
   a.part_stats = (Stat *)(a.part_keys + (size_t)cfg->rows * a.parts * top);
   OnDevice on(cfg->device);
