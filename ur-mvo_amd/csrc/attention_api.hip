@@ -21,18 +21,22 @@ namespace {
 struct Shape { int narrow, splits; };
 
 // How the forward pass is cut.  128-row workgroups read the keys least often; where they are fewer than the 256 CUs, 32-row
-// workgroups whose waves share the keys; where those are fewer as well, the keys are split until there are two workgroups per CU, at
-// least 256 keys each.  Up to 32 rows (one token, some heads) the keys' bytes are all there is: eight workgroups per CU even out
-// lengths and keep loads in flight (32 sequences of up to 16384 keys, 8 key heads of 128, bf16: 427 us in 128-row workgroups, 344 in
-// 32-row ones, 320, 303 and 290 with 512, 1024 and 2048 of them).
+// workgroups whose waves share the keys (8 x 4 heads of 1024 x 1024 x 64, bf16: 23 us with 256 of the former, 30 with 1024 of the latter; 2 x 4
+// heads: 21 and 12.4); where those are fewer as well, the keys are split until there are two workgroups per CU, at least 256 keys each.  The
+// join costs some 3 us and grows with the rows, so that short keys are left whole (1 x 4 heads of 1000 x 1000 x 64: 13.8 us in four ranges, 12.7
+// whole; 512 x 512: 11.0 and 8.4; one row of 1 x 32 heads over 1000 keys: 9.2 and 12.8; fp32, whose products take longer, 512 x 512: 15.3 and
+// 17.4).  Up to 32 rows (one token, some heads) over many keys their bytes are all there is: eight workgroups per CU even out lengths and
+// keep loads in flight, at least 1024 keys each (32 sequences of up to 16384 keys, 8 key heads of 128, bf16: 427 us in 128-row workgroups, 344
+// in 32-row ones, 320, 303 and 290 with 512, 1024 and 2048 of them; 64 sequences of 1000: 30 us with 2048, 18 with 512).
 Shape forward_shape(const urf_attn_config &c) {
   const long long rows = (long long)c.q_len * (c.q_heads / c.kv_heads), groups = (long long)c.batch * c.kv_heads;
-  if (rows > 32 && (rows + 127) / 128 * groups >= 256) return {0, 1};
+  const bool few = rows <= 32;
+  if (!few && (rows + 127) / 128 * groups >= 256) return {0, 1};
   const long long blocks = (rows + 31) / 32 * groups;
-  if (rows > 32 && blocks >= 256) return {1, 1};
-  const long long most = (c.k_len + 255) / 256, want = ((rows > 32 ? 512 : 2048) + blocks - 1) / blocks;
-  const long long s = want < most ? want : most;
-  return {1, (int)(s < 1 ? 1 : s > 64 ? 64 : s)};
+  if ((!few && blocks >= 256) || c.k_len < (few || c.dtype == URF_F32 ? 512 : 1024)) return {1, 1};
+  long long s = std::min<long long>((c.k_len + 255) / 256, (512 + blocks - 1) / blocks);
+  if (few) s = std::max(s, std::min<long long>(c.k_len / 1024, (2048 + blocks - 1) / blocks));
+  return {1, (int)std::min<long long>(std::max<long long>(s, 1), 64)};
 }
 
 size_t padded_dim(const urf_attn_config &c) { return ((size_t)c.head_dim + 31) / 32 * 32; }
