@@ -5,13 +5,15 @@
 // (log2 S - A / S) ln 2 with A = sum 2^x_v x_v: one pass over the row, every lane with a running maximum of its own that rescales its
 // sums when it grows.  (The difference comes before the product: scores at the lowest value of their type stay in range.)  The
 // gradients need lse only and are one more pass: read a score, write its gradient.
-// All of it is bound by memory: a score is read once per pass, 16 bytes a lane and load, four loads in flight per lane.
+// All of it is bound by memory: a score is read once per pass, 16 bytes a lane and load, four loads in flight per lane.  bf16: 2048 rows of
+// 131072, 537 MB: log probabilities 121 us (4.4 TB/s, the entropy's operations beside it; fp32, 819 MB: 144 us, 5.7 TB/s), distillation 104
+// (5.2 TB/s), a gradient 181 (1.07 GB, 5.9 TB/s); a large copy reaches 4.8 TB/s, a large sum 4.0.
 //
 // A row belongs to W waves (1, 4 or 16, one workgroup): 1 where the rows are short, 16 where there are too few rows to fill the
 // chip with 4.  A few long rows (the next token of some sequences) are cut in parts, a workgroup of 4 each, whose sums and
-// alternatives a second kernel joins.  Of many short rows a wave takes two, one per half (L = 32 lanes a row): what is done once per row -- joining the
-// lanes, sorting, the row's results -- is most of the work there.  Sums are joined in a fixed order.  Rows may start at any element: the loads are declared with the elements' own
-// alignment (this hardware takes a 16-byte access at any address).
+// alternatives a second kernel joins.  Of many short rows a wave takes two, one per half (L = 32 lanes a row): what is done once per row
+// -- joining the lanes, sorting, the row's results -- is most of the work there.  Sums are joined in a fixed order.  Rows may start at any
+// element: the vectors begin at the row's first boundary, and the scores before and behind them are one more step.
 //
 // "Listed" candidates (targets, a teacher's alternatives): at most 64 a row, one per lane of every wave.  A wave asks by ballot
 // whether any lies among the elements it is about to handle, which is rare in a long row, and only then looks whose they are.
@@ -58,8 +60,9 @@ template <typename T> struct Row {
   static constexpr int kPer = 16 / (int)sizeof(T);
   typedef T Vec __attribute__((ext_vector_type(kPer)));
   typedef T LooseVec __attribute__((ext_vector_type(kPer), aligned(sizeof(T))));      // gradients whose rows begin elsewhere
-  // scores before the first boundary: of 64 bytes, what the memory pipeline takes four lanes' vectors as, or of 16 where the lanes of a
-  // row are too few to take up to 31 scores before it and 7 behind the last vector
+  // scores before the first boundary: of 64 bytes, what the memory pipeline takes four lanes' vectors as (2048 rows of 100003 bf16
+  // scores: 98 us, 104 from the rows' first elements on), or of 16 where the lanes of a row are too few to take up to 31 scores before it
+  // and 7 behind the last vector
   template <int L> static __device__ __forceinline__ int head(const T *z, int V) {
     constexpr int kTo = L == 64 ? 63 : 15;
     return min(V, (int)(-(uintptr_t)z & kTo) / (int)sizeof(T));
@@ -134,8 +137,8 @@ template <int L> __device__ __forceinline__ Stat lanes_join(Stat v, float c) {
 // The pass over a row only notes, per lane, its largest score and where it was (three instructions per 16 bytes).  The K-th largest
 // of the lanes' best scores bounds the K-th largest of the row from below, so that afterwards only lanes whose best is not below it
 // -- about K of the row's 64, 256 or 1024 -- have their scores read again, cooperatively, and only scores that are not below it
-// are candidates: about K again.  They are sorted 64 at a time.  (Keeping a list during the pass costs more than the pass: 190 us
-// for 2048 rows of 100003 bf16 scores, against 129 us without alternatives.)
+// are candidates: about K again.  They are sorted 64 at a time.  (2048 rows of 100003 bf16 scores: 88 us without alternatives, 96 with 4,
+// 116 with 20, 161 with 64.  Keeping a list during the pass costs more than the pass: 129 -> 190 us at the time.)
 // Keys: the score as an ordered integer above, the complement of its index below (equal scores: the lower index wins); 0 = none.
 __device__ __forceinline__ u64 key_of(float z, int index) {
   const unsigned u = __float_as_uint(z + 0.0f);           // -0 counts as 0
