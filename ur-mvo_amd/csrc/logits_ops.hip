@@ -29,6 +29,7 @@ static_assert(URF_TOP_MAX == 64, "one listed candidate per lane");
 constexpr int kUnroll = 4;               // 16-byte loads in flight per lane
 constexpr double kLog2eDouble = 1.4426950408889634;
 constexpr int kMostParts = 32;           // of a row
+constexpr int kShort = 8 * URF_TOP_MAX;  // classes of a row that the listed candidates may be a large part of
 constexpr float kNothing = -0x1p100f;    // a row whose largest scaled score is below it allows nothing (masks of -inf or the lowest value)
 constexpr float kFloor = -1.0e4f;        // 2^kFloor is 0: a masked score (-inf) adds 0 * kFloor to A, not 0 * inf
 
@@ -487,6 +488,45 @@ __device__ __forceinline__ Teacher teacher_of(const RowsArgs &a, int r, int lane
   return t;
 }
 
+// the student's side of a row: its largest score, the sum of the exponentials from there and its logarithm, the logarithm of the
+// unlisted share, the score in this lane's listed place and the logarithm of the teacher's rest
+struct Student { float m, zk; double all, log_all, tail, log_rest; };
+// `st`: of the row, TAIL: without the listed candidates.  A few operations per row, in 64 bits: a divergence close to zero, and a
+// gradient, are differences of far larger terms.
+template <typename T, bool TAIL, int L>
+__device__ __forceinline__ Student student_of(const RowsArgs &a, const T *z, const Teacher &t, const Stat &st, int lane) {
+  Student q;
+  const bool used = t.index >= 0;
+  q.zk = used ? (float)z[t.index] : -INFINITY;
+  q.m = st.m;                                             // of the whole row
+  double sum = st.s, listed = 0.0;
+  if (TAIL) {
+    // the pass left the listed candidates out: add each of them once
+    bool first = used;
+    for (int k = 0; k < a.K; ++k) {
+      const int other = __shfl(t.index, k, L);
+      if (k < lane && other == t.index) first = false;
+    }
+    q.m = fmaxf(q.m, row_max<L>(q.zk));
+    const float mu = q.m == -INFINITY ? 0.0f : q.m;
+    listed = row_sum<L>(first ? (double)exp2f((q.zk - mu) * a.c) : 0.0);
+    sum = st.s * exp2f((st.m - mu) * a.c);
+  }
+  q.all = sum + listed;
+  // the logarithms, each in a lane of its own: of the sum, of the unlisted share of it, of the teacher's rest.  Where the unlisted
+  // share is too small for the sum's scale, its own maximum counts.
+  const bool far = TAIL && sum < 0x1p-100 * q.all;
+  const double logs = log(lane == 0 ? q.all : lane == 1 ? (far ? (double)st.s : listed < sum ? 1.0 - listed / q.all : sum / q.all) : t.rest);
+  q.log_all = __shfl(logs, 0, L);
+  q.tail = q.log_rest = 0.0;
+  if (TAIL) {
+    q.tail = __shfl(logs, 1, L);
+    if (far) q.tail += (st.m - (double)q.m) * a.scale - q.log_all;
+    q.log_rest = __shfl(logs, 2, L);
+  }
+  return q;
+}
+
 template <typename T, int W, int L, bool TAIL>
 __global__ void __launch_bounds__(W == 16 ? 1024 : 256) distill_kernel(RowsArgs a) {
   __shared__ Stat stats[W];
@@ -499,44 +539,17 @@ __global__ void __launch_bounds__(W == 16 ? 1024 : 256) distill_kernel(RowsArgs 
   Stat st = row_pass<T, W, L, false, false, TAIL>(z, a.V, a.c, wave, W, lane, t.index, sh);
   st = row_join<W, L>(st, a.c, wave, lane, stats);
   if (wave) return;
-  // What follows is a few operations per row, in 64 bits: a divergence close to zero is a difference of far larger terms.
-  const bool used = t.index >= 0;
-  const float zk = used ? (float)z[t.index] : -INFINITY;
-  float m = st.m;                                         // of the whole row
-  double sum = st.s, listed = 0.0;
-  if (TAIL) {
-    // the pass left the listed candidates out: add each of them once
-    bool first = used;
-    for (int k = 0; k < a.K; ++k) {
-      const int other = __shfl(t.index, k, L);
-      if (k < lane && other == t.index) first = false;
-    }
-    m = fmaxf(m, row_max<L>(zk));
-    const float mu = m == -INFINITY ? 0.0f : m;
-    listed = row_sum<L>(first ? (double)exp2f((zk - mu) * a.c) : 0.0);
-    sum = st.s * exp2f((st.m - mu) * a.c);
-  }
-  const double all = sum + listed;
-  // the logarithms, each in a lane of its own: of the sum, of the unlisted share of it, of the teacher's rest.  Where the unlisted
-  // share is too small for the sum's scale, its own maximum counts.
-  const bool far = TAIL && sum < 0x1p-100 * all;
-  const double logs = log(lane == 0 ? all : lane == 1 ? (far ? (double)st.s : listed < sum ? 1.0 - listed / all : sum / all) : t.rest);
-  const double log_all = __shfl(logs, 0, L), lse = (double)m * a.scale + log_all;
+  const Student q = student_of<T, TAIL, L>(a, z, t, st, lane);
   const float nan = __uint_as_float(0x7fc00000u);
-  const bool broken = !(all >= 0.0) || m == INFINITY, empty = m * a.scale < kNothing && !broken;
-  const double lq = zk == -INFINITY ? -INFINITY : ((double)zk - m) * a.scale - log_all;
-  double loss = row_sum<L>(t.p != 0.0 ? t.p * (t.lp - lq) : 0.0), tail = 0.0;
-  if (TAIL) {
-    // log of the student's probability of everything unlisted
-    tail = __shfl(logs, 1, L);
-    if (far) tail += (st.m - (double)m) * a.scale - log_all;
-    if (t.rest > 0.0) loss += t.rest * (__shfl(logs, 2, L) - tail);
-  }
+  const bool broken = !(q.all >= 0.0) || q.m == INFINITY, empty = q.m * a.scale < kNothing && !broken;
+  const double lq = q.zk == -INFINITY ? -INFINITY : ((double)q.zk - q.m) * a.scale - q.log_all;
+  double loss = row_sum<L>(t.p != 0.0 ? t.p * (t.lp - lq) : 0.0);
+  if (TAIL && t.rest > 0.0) loss += t.rest * (q.log_rest - q.tail);
   if (empty) loss = t.mass != 0.0 ? INFINITY : 0.0;       // the student allows nothing
   if (lane == 0) {
     a.loss[r] = broken ? nan : (float)loss;
-    a.lse[r] = broken ? nan : empty ? -INFINITY : (float)lse;
-    if (TAIL) a.log_tail[r] = broken ? nan : empty ? -INFINITY : (float)tail;
+    a.lse[r] = broken ? nan : empty ? -INFINITY : (float)((double)q.m * a.scale + q.log_all);
+    if (TAIL) a.log_tail[r] = broken ? nan : empty ? -INFINITY : (float)q.tail;
   }
 }
 
@@ -632,6 +645,27 @@ __device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float scale,
   }
 }
 
+// A row's lse from the one that was rounded to 32 bits.  Where probability and what is subtracted from it are close, that rounding is
+// all that would be left of a gradient (rows of five classes, all of them listed, fp32: 1.7e-6 of its norm, 3e-7 so).  The sum of
+// the probabilities says how far it is off; rows that the listed candidates may be a large part of are short and summed again (8192 rows
+// of 200: 5.8 -> 6.8 us; up to 4096 classes it would cost 8192 rows of 4000 43 -> 58).  16-bit gradients are rounded coarser than that.
+template <typename T> __device__ __forceinline__ double exact_lse(const T *z, int V, float scale, float lse, int lane) {
+  if constexpr (sizeof(T) == 4) {
+    if (V <= kShort) {
+      float sum = 0.0f;
+      for (int v = lane; v < V; v += 256) {
+        float f[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) f[u] = v + 64 * u < V ? z[v + 64 * u] : -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sum += __builtin_amdgcn_exp2f(fmaf(f[u], scale, -lse) * kLog2e);
+      }
+      return (double)lse + logf(row_sum<64>(sum));
+    }
+  }
+  return lse;
+}
+
 template <typename T, bool ENTROPY, bool STREAM>
 __global__ void __launch_bounds__(256) log_probs_backward_kernel(RowsArgs a) {
   const int lane = threadIdx.x & 63;
@@ -649,7 +683,7 @@ __global__ void __launch_bounds__(256) log_probs_backward_kernel(RowsArgs a) {
     else own = a.g1[(long long)r * a.N + lane];
   }
   g.add = own * a.scale;
-  set_shift(g.shift, g.slo, empty ? 0.0 : lse);
+  set_shift(g.shift, g.slo, empty ? 0.0 : exact_lse((const T *)a.z + (long long)r * a.stride, a.V, a.scale, lse, lane));
   g.coef = empty ? 0.0f : -row_sum<64>(own) * a.scale;
   if (ENTROPY && !empty) {
     g.h = a.g2[r] * a.scale * kLn2;
@@ -665,13 +699,13 @@ __global__ void __launch_bounds__(256) distill_backward_kernel(RowsArgs a) {
   const int r = a.R - 1 - (int)(w / a.per_row), part = (int)(w % a.per_row);      // the last rows, read last by the forward pass, first
   if (r < 0) return;
   const Teacher t = teacher_of<TAIL, 64>(a, r, lane);
-  const float lse = a.lse[r];
   const double gs = (double)a.g1[r] * a.scale;
-  const bool empty = lse == -INFINITY;
+  const bool empty = a.lse[r] == -INFINITY;
+  const double lse = empty ? 0.0 : exact_lse((const T *)a.z + (long long)r * a.stride, a.V, a.scale, a.lse[r], lane);
   GradRow g = {};
   g.mine = empty ? -1 : t.index;
   g.add = (float)(-gs * t.p);
-  set_shift(g.shift, g.slo, empty ? 0.0 : lse);
+  set_shift(g.shift, g.slo, lse);
   g.coef = empty ? 0.0f : (float)(gs * t.mass);
   if (TAIL) {
     g.lshift = g.shift;
@@ -681,7 +715,7 @@ __global__ void __launch_bounds__(256) distill_backward_kernel(RowsArgs a) {
     // a probability within the tail: nothing overflows however small q_tail is
     const float tail = a.log_tail[r];
     if (!empty && tail != -INFINITY) {
-      set_shift(g.shift, g.slo, (double)lse + tail);
+      set_shift(g.shift, g.slo, lse + tail);
       g.coef = (float)(gs * (t.mass * expf(tail) - t.rest));
     }
   }
