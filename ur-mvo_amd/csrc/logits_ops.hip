@@ -491,8 +491,8 @@ __device__ __forceinline__ Teacher teacher_of(const RowsArgs &a, int r, int lane
 // the student's side of a row: its largest score, the sum of the exponentials from there and its logarithm, the logarithm of the
 // unlisted share, the score in this lane's listed place and the logarithm of the teacher's rest
 struct Student { float m, zk; double all, log_all, tail, log_rest; };
-// `st`: of the row, TAIL: without the listed candidates.  A few operations per row, in 64 bits: a divergence close to zero, and a
-// gradient, are differences of far larger terms.
+// `st`: of the row, TAIL: without the listed candidates.  A few operations per row, in 64 bits: a divergence close to zero is a
+// difference of far larger terms.
 template <typename T, bool TAIL, int L>
 __device__ __forceinline__ Student student_of(const RowsArgs &a, const T *z, const Teacher &t, const Stat &st, int lane) {
   Student q;
