@@ -365,6 +365,44 @@ def test_two_streams_at_once(O):
             assert all(torch.equal(g[n], want[i][n]) for n in g), i
 
 
+def test_few_rows_in_parts_captured_and_on_two_streams(O):
+    """single tokens over long keys and a few long rows of scores: two graphs, each with the workspaces of its own capture, replayed at
+    the same time, and the same calls eagerly on two streams"""
+    def inputs(seed):
+        return {"q": cuda(normal((2, 1, 8, 64), torch.bfloat16, seed)), "k": cuda(normal((2, 5000, 2, 64), torch.bfloat16, seed + 1)),
+                "v": cuda(normal((2, 5000, 2, 64), torch.bfloat16, seed + 2)), "z": cuda(normal((3, 60001), torch.bfloat16, seed + 3))}
+
+    def calls(s):
+        o, lse = O.attention(s["q"], s["k"], s["v"], causal=True)
+        return {"o": o, "lse": lse, **{n: t for n, t in O.log_probs(s["z"], top=9)._asdict().items() if t is not None and n != "lse"}}
+
+    sets = [inputs(1), inputs(50)]
+    for s in sets:
+        calls(s)
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(calls(s))
+    for seed in (7, 90, 1):
+        for i, s in enumerate(sets):
+            for n, t in inputs(seed + 400 * i).items():
+                s[n].copy_(t)
+        want = [calls(s) for s in sets]
+        torch.cuda.synchronize()
+        eager = [None, None]
+        for _ in range(4):
+            for i, st in enumerate(streams):
+                with torch.cuda.stream(st):
+                    graphs[i].replay()
+                    eager[i] = calls(sets[i])
+        torch.cuda.synchronize()
+        for i in range(2):
+            for n in want[i]:
+                assert torch.equal(outs[i][n], want[i][n]) and torch.equal(eager[i][n], want[i][n]), (seed, i, n)
+
+
 def test_refusals(O):
     q = torch.zeros((1, 4, 2, 64), dtype=torch.bfloat16, device="cuda")
     z, t, f = torch.zeros((2, 50), device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(2, device="cuda")
