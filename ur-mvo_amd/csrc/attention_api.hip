@@ -114,6 +114,7 @@ int check_tensor(const urf_attn_tensor *t, const urf_attn_config *c, int len, co
 
 int check_out(const urf_attn_tensor *t, const urf_attn_config *c, int len, int heads, const char *who, const char *name) {
   if (check_tensor(t, c, len, who, name)) return -2;
+  if (len == 0) return 0;
   // two elements of an output may not share memory: each dimension, from the smallest stride up, steps over all that is below it
   struct { long long stride, n; } dim[3] = {{llabs(t->batch_stride), c->batch}, {llabs(t->row_stride), len}, {llabs(t->head_stride), heads}};
   std::sort(dim, dim + 3, [](const auto &x, const auto &y) { return x.stride < y.stride; });

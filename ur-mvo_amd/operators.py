@@ -65,7 +65,7 @@ def _head_view(who, name, t, dtype, device):
     if t.dtype is not dtype:
         _refuse(who, f"{name} is {t.dtype}, not {dtype}")
     (B, L, H, D), (sb, sr, sh, sd), p = t.shape, t.stride(), t.data_ptr()
-    per = 16 // t.element_size()
+    per = 4 if dtype is torch.float32 else 8
     if sd != 1 and D != 1:
         _refuse(who, f"the last dimension of {name} has to be contiguous")
     # the stride of a dimension of one says nothing
@@ -96,9 +96,17 @@ def _workspace_bytes(cfg, backward):
     return n.value
 
 
-def _out_view(t):
-    sb, sr, sh, _ = t.stride()
-    return _ATTN_TENSOR.pack(t.data_ptr(), sb, sr, sh)
+def _head_output(like, device):
+    """a contiguous tensor of the shape and type of `like`, and its view"""
+    B, L, H, D = like.shape
+    sr = H * D
+    sb = max(L, 1) * sr
+    t = torch.empty_strided((B, L, H, D), (sb, sr, D, 1), dtype=like.dtype, device=device)
+    return t, _ATTN_TENSOR.pack(t.data_ptr(), sb, sr, D)
+
+
+def _floats(n, device):
+    return torch.empty_strided((n,), (1,), dtype=torch.float32, device=device)
 
 
 def attention(q, k, v, *, causal=False, scale=None, q_lens=None, k_lens=None):
@@ -110,13 +118,13 @@ def attention(q, k, v, *, causal=False, scale=None, q_lens=None, k_lens=None):
     who = "attention"
     device, cfg, views, lens = _attn_config(who, q, k, v, causal, scale, q_lens, k_lens)
     B, Lq, Hq, _ = q.shape
-    o = torch.empty(q.shape, dtype=q.dtype, device=device)
-    lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=device)
+    o, o_view = _head_output(q, device)
+    lse = torch.empty_strided((B, Hq, Lq), (Hq * Lq, Lq, 1), dtype=torch.float32, device=device)
     if not B * Lq * Hq:
         return o, lse
     n = _workspace_bytes(cfg, 0)
     work = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-    check(_lib.lib().urf_attn_forward(cfg, *views, *lens, _out_view(o), lse.data_ptr(), work.data_ptr() if n else None, n,
+    check(_lib.lib().urf_attn_forward(cfg, *views, *lens, o_view, lse.data_ptr(), work.data_ptr() if n else None, n,
                                       _stream(device)), "urf_attn_forward")
     return o, lse
 
@@ -130,12 +138,12 @@ def attention_backward(do, q, k, v, o, lse, *, causal=False, scale=None, q_lens=
         _refuse(who, "do and o have to be of q's shape")
     o_view, do_view = _head_view(who, "o", o, q.dtype, device), _head_view(who, "do", do, q.dtype, device)
     lse = _plain(who, "lse", lse, torch.float32, (B, Hq, Lq), device)
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=device) for t in (q, k, v))
+    (dq, dq_view), (dk, dk_view), (dv, dv_view) = (_head_output(t, device) for t in (q, k, v))
     if not B * Lq * Hq:
         return dq, dk.zero_(), dv.zero_()
     n = _workspace_bytes(cfg, 1)
     work = torch.empty(n, dtype=torch.uint8, device=device)
-    check(_lib.lib().urf_attn_backward(cfg, *views, o_view, lse, do_view, *lens, _out_view(dq), _out_view(dk), _out_view(dv),
+    check(_lib.lib().urf_attn_backward(cfg, *views, o_view, lse, do_view, *lens, dq_view, dk_view, dv_view,
                                        work.data_ptr(), n, _stream(device)), "urf_attn_backward")
     return dq, dk, dv
 
@@ -182,10 +190,10 @@ def log_probs(logits, targets=None, *, top=0, scale=1.0):
     n, at = _targets(who, targets, R, device)
     if not 0 <= top <= min(TOP_MAX, V):
         _refuse(who, f"top {top} (0 .. {TOP_MAX}, at most the {V} classes)")
-    entropy, lse = torch.empty(R, dtype=torch.float32, device=device), torch.empty(R, dtype=torch.float32, device=device)
+    entropy, lse = _floats(R, device), _floats(R, device)
     log_prob = None if targets is None else torch.empty(targets.shape, dtype=torch.float32, device=device)
-    top_index = torch.empty((R, top), dtype=torch.int32, device=device) if top else None
-    top_log_prob = torch.empty((R, top), dtype=torch.float32, device=device) if top else None
+    top_index = torch.empty_strided((R, top), (top, 1), dtype=torch.int32, device=device) if top else None
+    top_log_prob = torch.empty_strided((R, top), (top, 1), dtype=torch.float32, device=device) if top else None
     size = _log_probs_workspace(cfg, top)
     work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     check(_lib.lib().urf_log_probs(cfg, logits.data_ptr(), at, n, top, log_prob.data_ptr() if n else None, entropy.data_ptr(),
@@ -235,8 +243,8 @@ def distill(logits, teacher_index, teacher_value, *, temperature=1.0, tail=False
     who = "distill"
     device, R, V, cfg = _rows_config(who, logits, _inverse(who, temperature))
     K, index, value = _teacher(who, teacher_index, teacher_value, R, device)
-    loss, lse = torch.empty(R, dtype=torch.float32, device=device), torch.empty(R, dtype=torch.float32, device=device)
-    log_tail = torch.empty(R, dtype=torch.float32, device=device) if tail else None
+    loss, lse = _floats(R, device), _floats(R, device)
+    log_tail = _floats(R, device) if tail else None
     check(_lib.lib().urf_distill(cfg, logits.data_ptr(), index, value, K, 1 if tail else 0, loss.data_ptr(), lse.data_ptr(),
                                  log_tail.data_ptr() if tail else None, _stream(device)), "urf_distill")
     return Distill(loss, lse, log_tail)
