@@ -624,7 +624,8 @@ int urf_attn_workspace(const urf_attn_config *cfg, int backward, size_t *bytes);
 /* o = softmax(scale q k^T) v per head, lse[b][head][row] = log of the row's sum of exponentials (f32, contiguous).
  * d_q_lens / d_k_lens: device ints, rows / keys in use per sequence (NULL = all; values are clamped to the tensors).  What lies
  * behind them is never used, whatever it holds; o is 0 and lse -infinity in rows behind q_lens and in rows that see no key.  (A
- * NaN or infinity among the keys in use of a causal call may reach rows before it too: a probability of 0 times it is NaN.)
+ * NaN or infinity among the keys in use of a causal call may reach rows before it too: a probability of 0 times it is NaN.)  A row
+ * in use with a NaN or a score of +infinity has NaN in o and lse, and NaN gradients of its own and of the keys it sees.
  * Scores, maxima, sums and accumulators are fp32; 16-bit types round the probabilities once, for the second product. */
 int urf_attn_forward(const urf_attn_config *cfg, const urf_attn_tensor *q, const urf_attn_tensor *k, const urf_attn_tensor *v,
                      const int *d_q_lens, const int *d_k_lens, const urf_attn_tensor *o, float *d_lse, void *d_work,

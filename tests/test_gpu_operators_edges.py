@@ -1,0 +1,64 @@
+"""Values at the edges of the operators' ranges on the GPU (-m gpu): NaN, infinities and scores that overflow among the rows and keys
+in use, small and large gradients in f16, scales outside of 32 bits, what torch records that these calls do not."""
+import math
+
+import pytest
+import torch
+
+import operators_reference as R
+from test_gpu_operators import DTYPES, INF, cuda, lens, normal, run_attention
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def O(U):
+    assert U._lib.lib().urf_device_count() >= 1, "GPU tests need an MI355X"
+    return U.operators
+
+
+# batch, rows, keys, query heads, key heads, head size: the forward kernel's three forms (128 rows a workgroup, 32, ranges of keys)
+FORMS = {"wide": (33, 1000, 70, 8, 8, 64), "narrow": (2, 150, 200, 4, 2, 64), "ranges": (2, 1, 3000, 4, 2, 128), "ranges of rows": (1, 300, 2500, 2, 1, 72)}
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("what", ["nan query", "nan key", "infinite score"])
+def test_attention_of_values_that_are_not_finite(O, dtype, form, what):
+    """A row in use with a NaN or a score of +infinity has no distribution: o, lse and dq are NaN there, and so are dk and dv of the
+    keys that it sees.  Other heads and sequences are what they are without it, and so are the head's other rows where a query is bad."""
+    B, Lq, Lk, Hq, Hk, D = FORMS[form]
+    G, h, row, key = Hq // Hk, 1, Lq - 1, Lk // 2 + 1
+    hk = h // G
+    q, do = normal((B, Lq, Hq, D), dtype, 1), normal((B, Lq, Hq, D), dtype, 2)
+    k, v = normal((B, Lk, Hk, D), dtype, 3), normal((B, Lk, Hk, D), dtype, 4)
+    clean = {n: t.cpu() for n, t in run_attention(O, cuda(q), cuda(k), cuda(v), cuda(do)).items()}
+    bound = {n: w[1] for n, w in R.attention(q[:1], k[:1], v[:1], False, None, None, None, do[:1]).items()}
+    head = torch.zeros((B, Lq, Hq), dtype=torch.bool)          # rows that share keys with the bad one
+    head[0, :, hk * G:hk * G + G] = True
+    bad = torch.zeros_like(head)
+    bad[0, row, h] = True
+    if what == "nan query":
+        q[0, row, h, D - 3] = torch.nan
+    elif what == "nan key":
+        k[0, key, hk, 5] = torch.nan
+        bad = head
+    elif dtype == torch.float16:             # products of f16 values stay below fp32's largest: an infinity among the inputs
+        q[0, row, h, 0] = INF
+        k[0, :, hk, 0] = 0.5 + k[0, :, hk, 0].abs()
+    else:                                    # finite inputs whose product overflows, for one key alone
+        q[0, row, h], k[0, key, hk] = 2.0 ** 66, 2.0 ** 66
+    got = {n: t.cpu() for n, t in run_attention(O, cuda(q), cuda(k), cuda(v), cuda(do)).items()}
+    for t in (got, clean):
+        t["lse"] = t["lse"].transpose(1, 2)
+    bound["lse"] = bound["lse"].transpose(1, 2)
+    for n in ("o", "lse", "dq"):
+        assert bool(got[n][bad].isnan().all()), n
+        assert torch.equal(got[n][~head], clean[n][~head]), n
+        if what == "nan query":              # (the running maximum moves for a wave's rows together: not the same bits)
+            rest = (head & ~bad)[0]
+            assert bool(((got[n][0][rest].double() - clean[n][0][rest].double()).abs() <= 2 * bound[n][0][rest]).all()), n
+    keys = torch.zeros((B, Lk, Hk), dtype=torch.bool)
+    keys[0, :, hk] = True
+    for n in ("dk", "dv"):
+        assert bool(got[n][keys].isnan().all()) and torch.equal(got[n][~keys], clean[n][~keys]), n

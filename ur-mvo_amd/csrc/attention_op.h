@@ -225,6 +225,11 @@ __device__ __forceinline__ int clamp_len(const int *lens, int b, int most) {
   return lens ? min(max(lens[b], 0), most) : most;      // lengths come from device memory: never trusted beyond the tensor
 }
 
+// A row's lse and what its accumulators are divided by, from its maximum (log2 units) and sum.  The sum is 0 for a row that saw no key
+// and no other; a NaN, which a NaN or an infinite score leaves in it, goes into both.
+__device__ __forceinline__ float row_lse(float m, float l) { return l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2; }
+__device__ __forceinline__ float row_inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
 // ------------------------------------------------------------------ forward
 // workgroups of four waves per CU that the registers are kept for (fp32 rows of 128: twice the registers of everything)
 template <typename T, int DP> constexpr int kBlocksPerCu = sizeof(T) == 2 || DP <= 64 ? 2 : 1;
@@ -393,17 +398,17 @@ __global__ void __launch_bounds__(256, (kBlocksPerCu<T, DP>)) attn_forward_kerne
       for (int e = 0; e < kOwn; e += 4) store4<float>(a.part_o + prow * DP + d0 + e, ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
       if (wave == 0 && half == 0) { a.part_ml[prow * 2] = m; a.part_ml[prow * 2 + 1] = l; }
     } else {
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const float inv = row_inverse(l);
       T *orow = (T *)a.o.p + (long long)b * a.o.b + (long long)i * a.o.r + (long long)(hk * a.G + g) * a.o.h;
 #pragma unroll
       for (int e = 0; e < kOwn; e += 4)
         if (d0 + e < a.D) store4<T>(orow + d0 + e, ov[e] * inv, ov[e + 1] * inv, ov[e + 2] * inv, ov[e + 3] * inv);
-      if (wave == 0 && half == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+      if (wave == 0 && half == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = row_lse(m, l);
     }
   } else if (inside) {
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = row_inverse(l);
     store_rows<T, DP>((T *)a.o.p + (long long)b * a.o.b + (long long)i * a.o.r + (long long)(hk * a.G + g) * a.o.h, acc, inv, a.D, half);
-    if (half == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+    if (half == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = row_lse(m, l);
   }
 }
 
@@ -432,12 +437,12 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
     for (int e = 0; e < kN; ++e)
       if (lane + 64 * e < DP) o[e] += a.part_o[p * DP + lane + 64 * e] * f;
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  const float inv = row_inverse(l);
   T *orow = (T *)a.o.p + (long long)b * a.o.b + (long long)i * a.o.r + (long long)(hk * a.G + g) * a.o.h;
 #pragma unroll
   for (int e = 0; e < kN; ++e)
     if (lane + 64 * e < a.D) orow[lane + 64 * e] = (T)(o[e] * inv);
-  if (lane == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  if (lane == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = row_lse(m, l);
 }
 
 // ------------------------------------------------------------------ backward
