@@ -62,3 +62,23 @@ def test_attention_of_values_that_are_not_finite(O, dtype, form, what):
     keys[0, :, hk] = True
     for n in ("dk", "dv"):
         assert bool(got[n][keys].isnan().all()) and torch.equal(got[n][~keys], clean[n][~keys]), n
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_rows_that_see_nothing_beside_keys_that_are_not_finite(O, dtype, form, causal):
+    """o and dq of rows behind the end, and of causal rows before the first key, are 0 and lse is -infinity whatever the keys in use hold"""
+    B, Lq, Lk, Hq, Hk, D = FORMS[form]
+    nq = [Lq // 2 if b % 2 else max(1, Lq - 3) for b in range(B)]
+    nk = [min(Lk, max(1, nq[b] - 1 - b % 3)) if causal else Lk for b in range(B)]
+    q, do = normal((B, Lq, Hq, D), dtype, 1), normal((B, Lq, Hq, D), dtype, 2)
+    k, v = normal((B, Lk, Hk, D), dtype, 3), normal((B, Lk, Hk, D), dtype, 4)
+    k[:, :, :, 3], v[:, 0], v[:, 1:] = torch.nan, torch.nan, INF
+    got = run_attention(O, cuda(q), cuda(k), cuda(v), cuda(do), causal, None, cuda(lens(nq)), cuda(lens(nk)))
+    blind = torch.stack([(torch.arange(Lq) >= nq[b]) | ((torch.arange(Lq) < nq[b] - nk[b]) if causal else False) for b in range(B)])
+    assert bool(blind.any())
+    blind = blind.cuda()
+    assert bool((got["o"][blind] == 0).all()) and bool((got["dq"][blind] == 0).all())
+    assert bool((got["lse"].transpose(1, 2)[blind] == -INF).all())
+    assert bool(got["lse"].transpose(1, 2)[~blind].isnan().all()) and bool(got["o"][~blind].isnan().all())

@@ -207,14 +207,16 @@ template <typename T> __device__ __forceinline__ void store4(T *p, float a, floa
   *(T4 *)p = T4{(T)a, (T)b, (T)c, (T)d};
 }
 
-// a lane's column of a transposed accumulator (row `p` of the output): four consecutive elements at a time
-template <typename T, int DP> __device__ __forceinline__ void store_rows(T *p, const f32x16 *acc, float f, int D, int half) {
+// a lane's column of a transposed accumulator (row `p` of the output): four consecutive elements at a time; 0 where nothing was `seen`,
+// whatever the others' keys left there (0 times infinity)
+template <typename T, int DP> __device__ __forceinline__ void store_rows(T *p, const f32x16 *acc, float f, bool seen, int D, int half) {
+  auto of = [&](float x) { return seen ? x * f : 0.0f; };
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int d = 32 * dt + 2 * r + 4 * half;
-      if (d < D) store4<T>(p + d, acc[dt][r] * f, acc[dt][r + 1] * f, acc[dt][r + 2] * f, acc[dt][r + 3] * f);
+      if (d < D) store4<T>(p + d, of(acc[dt][r]), of(acc[dt][r + 1]), of(acc[dt][r + 2]), of(acc[dt][r + 3]));
     }
 }
 
@@ -401,13 +403,15 @@ __global__ void __launch_bounds__(256, (kBlocksPerCu<T, DP>)) attn_forward_kerne
       const float inv = row_inverse(l);
       T *orow = (T *)a.o.p + (long long)b * a.o.b + (long long)i * a.o.r + (long long)(hk * a.G + g) * a.o.h;
 #pragma unroll
+      for (int e = 0; e < kOwn; ++e) ov[e] = l == 0.0f ? 0.0f : ov[e] * inv;
+#pragma unroll
       for (int e = 0; e < kOwn; e += 4)
-        if (d0 + e < a.D) store4<T>(orow + d0 + e, ov[e] * inv, ov[e + 1] * inv, ov[e + 2] * inv, ov[e + 3] * inv);
+        if (d0 + e < a.D) store4<T>(orow + d0 + e, ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
       if (wave == 0 && half == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = row_lse(m, l);
     }
   } else if (inside) {
     const float inv = row_inverse(l);
-    store_rows<T, DP>((T *)a.o.p + (long long)b * a.o.b + (long long)i * a.o.r + (long long)(hk * a.G + g) * a.o.h, acc, inv, a.D, half);
+    store_rows<T, DP>((T *)a.o.p + (long long)b * a.o.b + (long long)i * a.o.r + (long long)(hk * a.G + g) * a.o.h, acc, inv, l != 0.0f, a.D, half);
     if (half == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = row_lse(m, l);
   }
 }
@@ -441,7 +445,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
   T *orow = (T *)a.o.p + (long long)b * a.o.b + (long long)i * a.o.r + (long long)(hk * a.G + g) * a.o.h;
 #pragma unroll
   for (int e = 0; e < kN; ++e)
-    if (lane + 64 * e < a.D) orow[lane + 64 * e] = (T)(o[e] * inv);
+    if (lane + 64 * e < a.D) orow[lane + 64 * e] = (T)(l == 0.0f ? 0.0f : o[e] * inv);
   if (lane == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = row_lse(m, l);
 }
 
@@ -608,17 +612,14 @@ template <typename T, int DP> __device__ __forceinline__ void attn_backward_kv(c
     }
   }
   if (key >= a.Lk) return;
-  if (key >= nk) {                        // behind the sequence's end: its column held no key
-#pragma unroll
-    for (int dt = 0; dt < kDt; ++dt) dk[dt] = dv[dt] = f32x16{};
-  }
+  const bool used = key < nk;             // behind the sequence's end a column held no key
   if (a.kv_splits > 1) {
     const long long at = ((long long)split * a.B * a.Hk + group) * a.Lk + key, other = (long long)a.kv_splits * a.B * a.Hk * a.Lk * DP;
-    store_rows<float, DP>(a.part_kv + at * DP, dk, a.scale, DP, half);
-    store_rows<float, DP>(a.part_kv + other + at * DP, dv, 1.0f, DP, half);
+    store_rows<float, DP>(a.part_kv + at * DP, dk, a.scale, used, DP, half);
+    store_rows<float, DP>(a.part_kv + other + at * DP, dv, 1.0f, used, DP, half);
   } else {
-    store_rows<T, DP>((T *)a.dk.p + (long long)b * a.dk.b + (long long)key * a.dk.r + (long long)hk * a.dk.h, dk, a.scale, a.D, half);
-    store_rows<T, DP>((T *)a.dv.p + (long long)b * a.dv.b + (long long)key * a.dv.r + (long long)hk * a.dv.h, dv, 1.0f, a.D, half);
+    store_rows<T, DP>((T *)a.dk.p + (long long)b * a.dk.b + (long long)key * a.dk.r + (long long)hk * a.dk.h, dk, a.scale, used, a.D, half);
+    store_rows<T, DP>((T *)a.dv.p + (long long)b * a.dv.b + (long long)key * a.dv.r + (long long)hk * a.dv.h, dv, 1.0f, used, a.D, half);
   }
 }
 
@@ -718,9 +719,9 @@ template <typename T, int DP> __device__ __forceinline__ void attn_backward_q(co
   }
   if (!inside) return;
   if (a.q_splits > 1)
-    store_rows<float, DP>(a.part_q + (((long long)split * a.B * a.Hk + group) * ((long long)a.Lq * a.G) + row) * DP, dq, a.scale, DP, half);
+    store_rows<float, DP>(a.part_q + (((long long)split * a.B * a.Hk + group) * ((long long)a.Lq * a.G) + row) * DP, dq, a.scale, active, DP, half);
   else
-    store_rows<T, DP>((T *)a.dq.p + (long long)b * a.dq.b + (long long)i * a.dq.r + (long long)h * a.dq.h, dq, a.scale, a.D, half);
+    store_rows<T, DP>((T *)a.dq.p + (long long)b * a.dq.b + (long long)i * a.dq.r + (long long)h * a.dq.h, dq, a.scale, active, a.D, half);
 }
 
 // Both in one launch: the first workgroups make dk and dv, the others dq, so that neither leaves CUs idle at its end.  Seven products of
