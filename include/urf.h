@@ -612,7 +612,7 @@ typedef struct {
                                * batch * kv_heads * ceil32(q_len * q_heads / kv_heads) and batch * kv_heads * ceil32(k_len), and
                                * fewer than 2^27 batch * q_heads * q_len */
   int causal;                 /* non-zero: row i of a sequence sees key j iff j <= i + (its keys - its rows), the last row the last key */
-  float scale;                /* of q . k; 0 -> 1 / sqrt(head_dim) */
+  float scale;                /* of q . k, below 2^127; 0 -> 1 / sqrt(head_dim) */
   int device;
 } urf_attn_config;
 /* element (b, row, head, d) at data[b * batch_stride + row * row_stride + head * head_stride + d], strides in elements, any order
@@ -644,7 +644,7 @@ typedef struct {
   int dtype;                  /* URF_F32, URF_F16, URF_BF16: of the scores and their gradient; everything else is f32 */
   int rows, classes;          /* 0 .. 2^24 - 1 rows */
   long long row_stride;       /* elements between rows of the scores (any, also 0 or less than `classes`: they are only read) */
-  float scale;                /* the scores are multiplied by it first: 1 / temperature; positive */
+  float scale;                /* the scores are multiplied by it first: 1 / temperature; positive, below 2^127 */
   int device;
 } urf_rows_config;
 /* z = scale * logits of a row.  lse[row] = log sum exp z; entropy[row] of softmax(z), in nats; log_prob[row][n] = z[targets[row][n]]

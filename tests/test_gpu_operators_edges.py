@@ -82,3 +82,25 @@ def test_attention_rows_that_see_nothing_beside_keys_that_are_not_finite(O, dtyp
     assert bool((got["o"][blind] == 0).all()) and bool((got["dq"][blind] == 0).all())
     assert bool((got["lse"].transpose(1, 2)[blind] == -INF).all())
     assert bool(got["lse"].transpose(1, 2)[~blind].isnan().all()) and bool(got["o"][~blind].isnan().all())
+
+
+def test_scales_outside_of_32_bits_are_refused(O):
+    """a scale that 32 bits hold as 0 would be read as the default; one that they hold as infinity (or whose product with log2(e) they do) has no exponentials"""
+    q, z = torch.zeros((1, 4, 2, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((2, 50), device="cuda")
+    ix, val, f = torch.zeros((2, 3), dtype=torch.int32, device="cuda"), torch.zeros((2, 3), device="cuda"), torch.zeros(2, device="cuda")
+    o, lse = O.attention(q, q, q)
+    for s in (1e-46, 2.0 ** -150, 1e39, 3.3e38, 1e400, -1e-46, 0.0):
+        for call in (lambda: O.attention(q, q, q, scale=s), lambda: O.attention_backward(q, q, q, q, o, lse, scale=s), lambda: O.log_probs(z, scale=s),
+                     lambda: O.log_probs_backward(z, None, f, f, d_entropy=f, scale=s)):
+            with pytest.raises(ValueError):
+                call()
+    for t in (1e46, 1e-39, 0.0, -1.0, 5e-324, math.nan):
+        for call in (lambda: O.distill(z, ix, val, temperature=t), lambda: O.distill_backward(f, z, ix, val, f, temperature=t)):
+            with pytest.raises(ValueError):
+                call()
+
+
+def test_a_tiny_scale_is_not_the_default(O):
+    q, k, v = (normal((1, 40, 2, 64), torch.float32, s) for s in (1, 2, 3))
+    o, lse = O.attention(cuda(q), cuda(k), cuda(v), scale=1e-44)
+    R.check({"o": o, "lse": lse}, R.attention(q, k, v, False, 1e-44))

@@ -93,7 +93,7 @@ int check_config(const urf_attn_config *c, const char *who) {
   URF_CHECK(c->batch >= 1 && c->q_len >= 1 && c->k_len >= 0, "%s: batch %d, %d rows, %d keys", who, c->batch, c->q_len, c->k_len);
   URF_CHECK(c->kv_heads >= 1 && c->q_heads >= 1 && c->q_heads % c->kv_heads == 0, "%s: %d query heads over %d key heads", who, c->q_heads, c->kv_heads);
   URF_CHECK(c->head_dim >= 8 && c->head_dim <= 128 && c->head_dim % 8 == 0, "%s: head size %d (a multiple of 8 up to 128)", who, c->head_dim);
-  URF_CHECK(isfinite(c->scale) && c->scale >= 0.0f, "%s: scale %g", who, (double)c->scale);
+  URF_CHECK(c->scale >= 0.0f && c->scale < 0x1p127f, "%s: scale %g", who, (double)c->scale);      // (times log2(e) it is still finite)
   // row and key indices are 32-bit, element offsets 64-bit; a launch takes fewer than 2^24 workgroups of 256 threads
   const long long most = 1ll << 23, rows = (long long)c->q_len * (c->q_heads / c->kv_heads);
   const bool few = (long long)c->batch * c->q_heads < most;

@@ -829,7 +829,7 @@ int check_config(const urf_rows_config *c, const char *who) {
   URF_CHECK(dtype_bytes(c->dtype), "%s: element type %d (URF_F32, URF_F16 or URF_BF16)", who, c->dtype);
   // a workgroup per row, and a launch takes fewer than 2^24 of them (of 256 threads)
   URF_CHECK(c->rows >= 0 && c->rows < (1 << 24) && c->classes >= 1 && c->classes <= (1 << 30), "%s: %d rows of %d classes", who, c->rows, c->classes);
-  URF_CHECK(isfinite(c->scale) && c->scale > 0.0f, "%s: scale %g (positive)", who, (double)c->scale);
+  URF_CHECK(c->scale > 0.0f && c->scale < 0x1p127f, "%s: scale %g (positive)", who, (double)c->scale);      // (times log2(e) it is still finite)
   return 0;
 }
 

@@ -30,6 +30,13 @@ def _refuse(who, text):
     raise ValueError(f"{who}: {text}")
 
 
+def _scale(who, name, x):
+    """x, a factor that 32 bits hold neither as 0 (which the C ABI reads as a default) nor, times log2(e), as infinity"""
+    if not 2.0 ** -150 < x < 2.0 ** 127:
+        _refuse(who, f"{name} {x} (positive, in the range of 32 bits)")
+    return x
+
+
 def _scores(who, name, t, device):
     """what every floating input has to be"""
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
@@ -82,8 +89,8 @@ def _attn_config(who, q, k, v, causal, scale, q_lens, k_lens):
     (B, Lq, Hq, D), (Bk, Lk, Hk, Dk) = q.shape, k.shape
     if k.shape != v.shape or Bk != B or Dk != D:
         _refuse(who, f"shapes {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)} of q, k and v do not fit")
-    if scale is not None and not (math.isfinite(scale) and scale > 0):
-        _refuse(who, f"scale {scale}")
+    if scale is not None:
+        _scale(who, "scale", scale)
     lens = [None if t is None else _plain(who, name, t, torch.int32, (B,), device) for name, t in (("q_lens", q_lens), ("k_lens", k_lens))]
     cfg = _ATTN_CONFIG.pack(DTYPES[q.dtype], B, Hq, Hk, D, Lq, Lk, 1 if causal else 0, scale or 0.0, device.index)
     return device, cfg, views, lens
@@ -157,8 +164,7 @@ def _rows_config(who, logits, scale):
     (R, V), (sr, sv) = logits.shape, logits.stride()
     if V < 1 or (sv != 1 and V > 1):
         _refuse(who, "the rows of logits have to be contiguous and not empty")
-    if not (math.isfinite(scale) and scale > 0):
-        _refuse(who, f"scale {scale} (positive)")
+    _scale(who, "scale", scale)
     return device, R, V, _ROWS_CONFIG.pack(DTYPES[logits.dtype], R, V, sr, scale, device.index)
 
 
@@ -230,9 +236,9 @@ def _teacher(who, index, value, R, device):
 
 
 def _inverse(who, temperature):
-    if not (math.isfinite(temperature) and temperature > 0):
+    if not 0 < temperature < math.inf:
         _refuse(who, f"temperature {temperature}")
-    return 1.0 / temperature
+    return _scale(who, "1 / temperature", 1.0 / temperature)
 
 
 def distill(logits, teacher_index, teacher_value, *, temperature=1.0, tail=False):
