@@ -104,3 +104,24 @@ def test_a_tiny_scale_is_not_the_default(O):
     q, k, v = (normal((1, 40, 2, 64), torch.float32, s) for s in (1, 2, 3))
     o, lse = O.attention(cuda(q), cuda(k), cuda(v), scale=1e-44)
     R.check({"o": o, "lse": lse}, R.attention(q, k, v, False, 1e-44))
+
+
+def test_what_torch_would_record_is_refused(O):
+    """tangents of forward mode and traces would be cut silently"""
+    from torch.autograd import forward_ad
+    q = torch.zeros((1, 4, 2, 64), device="cuda")
+    z, f, t = torch.zeros((2, 50), device="cuda"), torch.zeros(2, device="cuda"), torch.zeros((2, 1), dtype=torch.int32, device="cuda")
+    with forward_ad.dual_level():
+        d, e, g = (forward_ad.make_dual(x, torch.ones_like(x)) for x in (q, z, f))
+        for call in (lambda: O.attention(d, q, q), lambda: O.attention(q, q, d), lambda: O.log_probs(e), lambda: O.distill(e, t, f[:, None]),
+                     lambda: O.distill(z, t, g[:, None]), lambda: O.distill_backward(g, z, t, f[:, None], f)):
+            with pytest.raises(ValueError):
+                call()
+        O.log_probs(z)                       # no tangent: as ever
+    for call in (lambda x: O.attention(x, x, x)[0], lambda x: O.log_probs(x[0, 0]).lse):
+        with pytest.raises(ValueError):
+            torch.jit.trace(call, q)
+    for call in (lambda: torch.func.jvp(lambda x: O.log_probs(x).lse, (z,), (z,)), lambda: torch.func.vmap(lambda x: O.log_probs(x).lse)(z[None]),
+                 lambda: torch.func.grad(lambda x: O.log_probs(x).lse.sum())(z)):
+        with pytest.raises((ValueError, RuntimeError)):
+            call()

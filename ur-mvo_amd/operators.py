@@ -2,8 +2,8 @@
 
 Every function enqueues its kernels on the current stream of its tensors' device and returns tensors allocated there, workspaces
 included, from torch's allocator: calls on several streams share nothing, and a call may be captured into a graph.  Forward and
-backward are separate calls, as in the C ABI; nothing here records for autograd (inputs that require a gradient are refused while
-it is enabled, rather than silently cut from the graph).
+backward are separate calls, as in the C ABI; nothing here records for autograd: inputs that require a gradient while it is enabled,
+inputs with a tangent of forward mode, and calls under torch.jit.trace are refused, rather than silently cut from what is recorded.
 """
 import collections
 import functools
@@ -11,6 +11,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check
@@ -37,15 +38,26 @@ def _scale(who, name, x):
     return x
 
 
+def _untraced(who):
+    if torch._C._get_tracing_state() is not None:
+        _refuse(who, "a trace would not record this call")
+
+
+def _unrecorded(who, name, t):
+    if t.requires_grad and torch.is_grad_enabled():
+        _refuse(who, f"{name} requires a gradient, which this call would not record: call it under torch.no_grad() or with detached "
+                     "tensors, and the backward call for the gradients")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        _refuse(who, f"{name} has a tangent, which this call would not carry on")
+
+
 def _scores(who, name, t, device):
     """what every floating input has to be"""
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
         _refuse(who, f"{name} has to be a tensor on the GPU")
     if t.dtype not in DTYPES:
         _refuse(who, f"{name} is {t.dtype} (float32, float16 or bfloat16)")
-    if t.requires_grad and torch.is_grad_enabled():
-        _refuse(who, f"{name} requires a gradient, which this call would not record: call it under torch.no_grad() or with detached "
-                     "tensors, and the backward call for the gradients")
+    _unrecorded(who, name, t)
     if device is not None and t.device != device:
         _refuse(who, f"{name} is on {t.device}, not on {device}")
     return t.device
@@ -55,8 +67,7 @@ def _plain(who, name, t, dtype, shape, device):
     """a contiguous tensor of the given type and shape; its address"""
     if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.shape == shape and t.is_contiguous()):
         _refuse(who, f"{name} has to be a contiguous {dtype} tensor {tuple(shape)} on {device}")
-    if t.requires_grad and torch.is_grad_enabled():
-        _refuse(who, f"{name} requires a gradient, which this call would not record")
+    _unrecorded(who, name, t)
     return t.data_ptr()
 
 
@@ -84,6 +95,7 @@ def _head_view(who, name, t, dtype, device):
 
 def _attn_config(who, q, k, v, causal, scale, q_lens, k_lens):
     """device, configuration, the views of q, k and v, the addresses of the lengths"""
+    _untraced(who)
     device = _scores(who, "q", q, None)
     views = [_head_view(who, name, t, q.dtype, device) for name, t in (("q", q), ("k", k), ("v", v))]
     (B, Lq, Hq, D), (Bk, Lk, Hk, Dk) = q.shape, k.shape
@@ -158,6 +170,7 @@ def attention_backward(do, q, k, v, o, lse, *, causal=False, scale=None, q_lens=
 # ------------------------------------------------------------------ rows of scores
 def _rows_config(who, logits, scale):
     """device, rows, classes, configuration"""
+    _untraced(who)
     device = _scores(who, "logits", logits, None)
     if logits.dim() != 2:
         _refuse(who, "logits has to be [rows, classes]")
