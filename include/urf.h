@@ -632,8 +632,8 @@ int urf_attn_forward(const urf_attn_config *cfg, const urf_attn_tensor *q, const
                      size_t work_bytes, void *stream);
 /* gradients of sum(o * d_o) with respect to q, k and v; o and d_lse are the forward call's, the probabilities are recomputed from
  * them.  Heads that share a key head are summed into its dk and dv.  Rows behind q_lens / k_lens and rows that see no key get 0, and
- * what they hold is not used.  16-bit types round the probabilities and the gradients of the scores once: of f16, d_o . v has to stay
- * below 65504 (a scaled loss). */
+ * what they hold is not used.  16-bit types round the probabilities and the gradients of the scores once (of f16, times powers of two
+ * that keep them in range, whatever the size of d_o). */
 int urf_attn_backward(const urf_attn_config *cfg, const urf_attn_tensor *q, const urf_attn_tensor *k, const urf_attn_tensor *v,
                       const urf_attn_tensor *o, const float *d_lse, const urf_attn_tensor *d_o, const int *d_q_lens,
                       const int *d_k_lens, const urf_attn_tensor *dq, const urf_attn_tensor *dk, const urf_attn_tensor *dv,

@@ -84,6 +84,53 @@ def test_attention_rows_that_see_nothing_beside_keys_that_are_not_finite(O, dtyp
     assert bool(got["lse"].transpose(1, 2)[~blind].isnan().all()) and bool(got["o"][~blind].isnan().all())
 
 
+# The probabilities (for dv) and the gradients of the scores (for dq and dk) are rounded to f16 once before the sum, and the sum once
+# more.  Terms and result are numbers of f16's full precision if the kernel keeps them in range, so that both roundings have the same
+# distribution relative to what they round; the terms' errors are independent and add up in squares: to at most the error of one
+# rounding of the result where the terms do not cancel (the keys and queries are random: |sum|^2 is sum |term|^2 on average).  Together
+# sqrt(2) times the error of one rounding at the end; delta's error (from the rounded o, whose entries are sqrt(e / keys) of v's) is
+# scale = 1 / sqrt(head size) of one rounding in dq, less in dk, and fp32's is far below.  2 leaves room for the draw.  (Rounded without their range in mind the terms are subnormal: 3 to 11 times.)
+SMALL = [(1, 1024, 8192, 1, 1, 64, False), (1, 256, 8192, 2, 1, 128, True), (16, 512, 4096, 8, 4, 64, False), (2, 1000, 1300, 2, 2, 40, True)]
+
+
+@pytest.mark.parametrize("shape", SMALL, ids=lambda s: "x".join(map(str, s[:6])) + ("c" if s[6] else ""))
+@pytest.mark.parametrize("size", [1e-4, 1e-3, 1e-2, 1.0, 30.0])
+def test_attention_f16_gradients_of_any_size(O, shape, size):
+    B, Lq, Lk, Hq, Hk, D, causal = shape
+    q, do = normal((B, Lq, Hq, D), torch.float16, 1), (normal((B, Lq, Hq, D), torch.float32, 2) * size).to(torch.float16)
+    k, v = normal((B, Lk, Hk, D), torch.float16, 3), normal((B, Lk, Hk, D), torch.float16, 4)
+    got = run_attention(O, cuda(q), cuda(k), cuda(v), cuda(do), causal)
+    b = B - 1                                # the definition of one sequence: 64 bits on the CPU
+    want = R.attention(*(t[b:b + 1] for t in (q, k, v)), causal, None, None, None, do[b:b + 1])
+    for n in ("dq", "dk", "dv"):
+        x = want[n][0]
+        once = float((x.to(torch.float16).double() - x).norm())
+        off = float((got[n][b:b + 1].cpu().double() - x).norm())
+        assert off <= 2 * once, (n, off / float(x.norm()), once / float(x.norm()))
+
+
+@pytest.mark.parametrize("shape", SMALL[:1] + SMALL[2:], ids=lambda s: "x".join(map(str, s[:6])) + ("c" if s[6] else ""))
+def test_attention_f16_products_beyond_its_largest_number(O, shape):
+    """do . v reaches some 10^6: the products before the sum need not fit f16, the gradients do.  Rows of very different sizes side by side."""
+    B, Lq, Lk, Hq, Hk, D, causal = shape
+    B = min(B, 2)
+    q, do = normal((B, Lq, Hq, D), torch.float16, 1) / 8, normal((B, Lq, Hq, D), torch.float32, 2)
+    k, v = normal((B, Lk, Hk, D), torch.float16, 3) / 8, normal((B, Lk, Hk, D), torch.float16, 4) * 64
+    do[:, ::2] *= 1e-3
+    do[:, 1::2] *= 2000
+    do = do.to(torch.float16)
+    got = run_attention(O, cuda(q), cuda(k), cuda(v), cuda(do), causal)
+    b = B - 1
+    want = R.attention(*(t[b:b + 1] for t in (q, k, v)), causal, None, None, None, do[b:b + 1])
+    assert float((do[b, :, 0].double() @ v[b, :, 0].double().T).abs().max()) > 2 * 65504
+    for n in ("dq", "dk", "dv"):
+        x = want[n][0]
+        assert float(x.abs().max()) < 65504
+        for part in ((x[:, ::2], got[n][b:b + 1, ::2]), (x[:, 1::2], got[n][b:b + 1, 1::2])) if n == "dq" else ((x, got[n][b:b + 1]),):
+            once = float((part[0].to(torch.float16).double() - part[0]).norm())
+            assert float((part[1].cpu().double() - part[0]).norm()) <= 2 * once, n
+
+
 def test_scales_outside_of_32_bits_are_refused(O):
     """a scale that 32 bits hold as 0 would be read as the default; one that they hold as infinity (or whose product with log2(e) they do) has no exponentials"""
     q, z = torch.zeros((1, 4, 2, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((2, 50), device="cuda")

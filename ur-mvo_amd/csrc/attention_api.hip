@@ -72,9 +72,12 @@ void backward_shape(const urf_attn_config &c, int *kv_splits, int *q_splits) {
     }
 }
 
-size_t delta_bytes(const urf_attn_config &c) { return ((size_t)c.batch * c.q_heads * c.q_len * sizeof(float) + 15) / 16 * 16; }
+size_t floats(size_t n) { return (n * sizeof(float) + 15) / 16 * 16; }
+size_t delta_bytes(const urf_attn_config &c) { return floats((size_t)c.batch * c.q_heads * c.q_len); }
+size_t norm_v_bytes(const urf_attn_config &c) { return floats((size_t)c.batch * c.kv_heads * c.k_len); }
 
-// delta, the parts of dk and dv, the parts of dq
+// delta, f16: the norms of do's and v's rows, the parts of dk and dv, the parts of dq
+size_t stat_bytes(const urf_attn_config &c) { return c.dtype == URF_F16 ? 2 * delta_bytes(c) + norm_v_bytes(c) : delta_bytes(c); }
 size_t part_kv_bytes(const urf_attn_config &c, int splits) {
   return splits > 1 ? 2 * (size_t)splits * c.batch * c.kv_heads * c.k_len * padded_dim(c) * sizeof(float) : 0;
 }
@@ -84,7 +87,7 @@ size_t part_q_bytes(const urf_attn_config &c, int splits) {
 size_t backward_bytes(const urf_attn_config &c) {
   int kv, q;
   backward_shape(c, &kv, &q);
-  return delta_bytes(c) + part_kv_bytes(c, kv) + part_q_bytes(c, q);
+  return stat_bytes(c) + part_kv_bytes(c, kv) + part_q_bytes(c, q);
 }
 
 int check_config(const urf_attn_config *c, const char *who) {
@@ -197,7 +200,9 @@ extern "C" int urf_attn_backward(const urf_attn_config *cfg, const urf_attn_tens
   a.lse = (float *)d_lse;
   a.delta = (float *)d_work;
   backward_shape(*cfg, &a.kv_splits, &a.q_splits);
-  a.part_kv = (float *)((char *)d_work + delta_bytes(*cfg));
+  a.norm_do = (float *)((char *)d_work + delta_bytes(*cfg));
+  a.norm_v = (float *)((char *)a.norm_do + delta_bytes(*cfg));
+  a.part_kv = (float *)((char *)d_work + stat_bytes(*cfg));
   a.part_q = (float *)((char *)a.part_kv + part_kv_bytes(*cfg, a.kv_splits));
   OnDevice on(cfg->device);
   URF_HIP(on.rc);

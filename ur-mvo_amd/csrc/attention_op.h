@@ -18,6 +18,9 @@
 #pragma once
 #include "operator_common.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace urf {
 
 struct AttnView { void *p; long long b, r, h; };   // base, strides in elements: batch, row, head
@@ -27,6 +30,7 @@ struct AttnArgs {
   const int *q_lens, *k_lens;    // rows in use per sequence (null = all)
   float *lse;                    // [B][Hq][Lq], natural logarithm
   float *delta;                  // [B][Hq][Lq] (backward)
+  float *norm_do, *norm_v;       // |do_i| [B][Hq][Lq], |v_j| [B][Hk][Lk] (backward, f16)
   float *part_o, *part_ml;       // forward over split keys: [split][B * Hk][Lq * G][DP] and (maximum, sum)
   float *part_kv, *part_q;       // backward in parts: dk then dv [split][B * Hk][Lk][DP]; dq [split][B * Hk][Lq * G][DP]
   int B, Hq, Hk, G, Lq, Lk, D;
@@ -450,17 +454,67 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 }
 
 // ------------------------------------------------------------------ backward
+// The range of f16 in the backward pass's second products.  Probabilities are about 1 / keys and gradients of any size, so that p and ds
+// as they are would be rounded among f16's subnormal numbers, in steps of 2^-24 (8192 keys, do ~ 1e-3: dq and dk off by 0.011 of their
+// norm, one rounding of the results 0.0009), and large ones beyond its largest.  p <= 1 is taken times 2^14, ds times a power of two that
+// brings its bound |do_i| |v_j| + |delta_i| (the largest among the rows and keys of a workgroup for dk, of a row for dq) to 2^14..2^15:
+// a subtraction becomes an fma, an exponent is shifted, and the results are multiplied by the inverse in fp32.  Terms down to 2^-29 of
+// the bound have all of f16's bits.  The norms are made beside delta.  (us, 16 x 4 heads of 1024 x 1024 x 64 / 2 x 16 heads of 4096 x 4096 x
+// 128, causal: 88 / 604, without any of it 82 / 588.  Following the largest term seen so far, as the forward pass does, needs no norms, but
+// its branch stands between the products: 92 / 735.)
+template <typename T> constexpr bool kScaled = std::is_same<T, _Float16>::value;
+constexpr int kProbShift = 14;
+template <typename T> constexpr float kDvScale = kScaled<T> ? 1.0f / (1 << kProbShift) : 1.0f;
+// the exponent of the power of two for ds below `bound`
+__device__ __forceinline__ int grad_shift(float bound) { return min(14 + 127 - (__float_as_int(bound) >> 23), 60); }
+__device__ __forceinline__ float finite_max(float m, float x) { return x < INFINITY ? fmaxf(m, x) : m; }       // (x >= 0 or NaN)
+// over the workgroup; `lds`: 16 bytes that nothing else uses until the caller's next barrier
+__device__ __forceinline__ float block_max(float m, float *lds) {
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+  lds_barrier();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
+  lds_barrier();
+  return fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+}
+
 // delta_i = do_i . o_i: L lanes per row, 16 bytes of each tensor at a time; 8 where that is a row of 64 16-bit elements, 16 otherwise.
 // Bound by memory: 2 x 4096 rows of 16 heads of 128, bf16, 67 MB each of o and do in 13 us (10.3 TB/s: what the forward pass wrote is in
 // the last-level cache).
 template <typename T, int L>
 __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a) {
   constexpr int kPer = 16 / (int)sizeof(T);
-  const unsigned u = blockIdx.x * (256 / L) + threadIdx.x / L, uh = u / a.Hq;      // row (b, i, h), (b, i)
+  constexpr bool kNorms = kScaled<T>;
+  constexpr unsigned kRows = 256 / L;
   const int c = threadIdx.x % L;
+  if constexpr (kNorms) {
+    const unsigned do_blocks = (a.B * a.Lq * a.Hq + kRows - 1) / kRows, v_rows = a.B * a.Lk * a.Hk;
+    if (blockIdx.x >= do_blocks) {                         // rows (b, j, h) of v
+      for (unsigned u = (blockIdx.x - do_blocks) * kRows + threadIdx.x / L; u < v_rows; u += (gridDim.x - do_blocks) * kRows) {
+        const unsigned uh = u / a.Hk;
+        const int h = u - uh * a.Hk, b = uh / a.Lk, j = uh - b * a.Lk;
+        float s = 0.0f;
+        if (j < clamp_len(a.k_lens, b, a.Lk)) {
+          const T *v = (const T *)a.v.p + (long long)b * a.v.b + (long long)j * a.v.r + (long long)h * a.v.h;
+          typedef T TV __attribute__((ext_vector_type(kPer)));
+          for (int e = c * kPer; e < a.D; e += L * kPer) {
+            const TV x = *(const TV *)(v + e);
+#pragma unroll
+            for (int n = 0; n < kPer; ++n) s = fmaf((float)x[n], (float)x[n], s);
+          }
+        }
+#pragma unroll
+        for (int x = L / 2; x >= 1; x >>= 1) s += __shfl_xor(s, x, L);
+        if (c == 0) a.norm_v[((long long)b * a.Hk + h) * a.Lk + j] = sqrtf(s);
+      }
+      return;
+    }
+  }
+  const unsigned u = blockIdx.x * kRows + threadIdx.x / L;
+  const unsigned uh = u / a.Hq;                            // row (b, i, h), (b, i)
   const bool inside = u < (unsigned)(a.B * a.Lq * a.Hq);
   const int h = u - uh * a.Hq, b = inside ? uh / a.Lq : 0, i = uh - b * a.Lq;
-  float s = 0.0f;
+  float s = 0.0f, ss = 0.0f;
   if (inside && i < clamp_len(a.q_lens, b, a.Lq)) {
     const T *o = (const T *)a.o.p + (long long)b * a.o.b + (long long)i * a.o.r + (long long)h * a.o.h;
     const T *d = (const T *)a.dout.p + (long long)b * a.dout.b + (long long)i * a.dout.r + (long long)h * a.dout.h;
@@ -468,12 +522,21 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a) {
     for (int e = c * kPer; e < a.D; e += L * kPer) {
       const TV x = *(const TV *)(o + e), y = *(const TV *)(d + e);
 #pragma unroll
-      for (int n = 0; n < kPer; ++n) s = fmaf((float)x[n], (float)y[n], s);
+      for (int n = 0; n < kPer; ++n) {
+        s = fmaf((float)x[n], (float)y[n], s);
+        if (kNorms) ss = fmaf((float)y[n], (float)y[n], ss);
+      }
     }
   }
 #pragma unroll
-  for (int x = L / 2; x >= 1; x >>= 1) s += __shfl_xor(s, x, L);
-  if (inside && c == 0) a.delta[((long long)b * a.Hq + h) * a.Lq + i] = s;
+  for (int x = L / 2; x >= 1; x >>= 1) {
+    s += __shfl_xor(s, x, L);
+    if (kNorms) ss += __shfl_xor(ss, x, L);
+  }
+  if (inside && c == 0) {
+    a.delta[((long long)b * a.Hq + h) * a.Lq + i] = s;
+    if (kNorms) a.norm_do[((long long)b * a.Hq + h) * a.Lq + i] = sqrtf(ss);
+  }
 }
 
 // Tiles of 64 rows (keys) where the registers allow it: half the barriers, and the second half's products run beside the first
@@ -515,7 +578,25 @@ template <typename T, int DP> __device__ __forceinline__ void attn_backward_kv(c
   f32x16 dk[kDt], dv[kDt];
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt) dk[dt] = dv[dt] = f32x16{};
+  float factor = 1.0f;                    // f16: of ds, beside the probabilities'
   if (begin < rows) {
+    if constexpr (kScaled<T>) {
+      float most_do = 0.0f, most_delta = 0.0f, most_v = 0.0f;
+      const int i0 = max(begin, low) / a.G, i1 = (rows + a.G - 1) / a.G;
+      for (int g = 0; g < a.G; ++g) {
+        const long long at = ((long long)b * a.Hq + hk * a.G + g) * a.Lq;
+        for (int i = i0 + tid; i < i1; i += 256) {
+          most_do = finite_max(most_do, a.norm_do[at + i]);
+          most_delta = finite_max(most_delta, fabsf(a.delta[at + i]));
+        }
+      }
+      if (tid < 128 && tile * 128 + tid < nk) most_v = finite_max(0.0f, a.norm_v[((long long)b * a.Hk + hk) * a.Lk + tile * 128 + tid]);
+      most_do = block_max(most_do, (float *)lds);
+      most_delta = block_max(most_delta, (float *)lds);
+      most_v = block_max(most_v, (float *)lds);
+      lds_barrier();
+      factor = ldexpf(1.0f, grad_shift(most_do * most_v + most_delta) - kProbShift);
+    }
     const T *krow = (const T *)a.k.p + (long long)b * a.k.b + (long long)key * a.k.r + (long long)hk * a.k.h;
     Frag k[kKc];
 #pragma unroll
@@ -544,7 +625,7 @@ template <typename T, int DP> __device__ __forceinline__ void attn_backward_kv(c
         stat_next = tid < kRows ? INFINITY : 0.0f;
         if (stat_row < rows && stat_row >= low) {
           const float x = stat[(long long)stat_g * a.Lq + stat_i];
-          stat_next = tid < kRows ? (x == -INFINITY ? INFINITY : x * kLog2e) : x;
+          stat_next = tid < kRows ? (x == -INFINITY ? INFINITY : x * kLog2e - (kScaled<T> ? kProbShift : 0)) : kScaled<T> ? x * factor : x;
         }
         stat_row -= kRows;
         stat_i -= kRows / a.G;
@@ -594,7 +675,7 @@ template <typename T, int DP> __device__ __forceinline__ void attn_backward_kv(c
           for (int e = 0; e < 4; ++e) {
             const int r = 4 * r4 + e;
             s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], a.scale2, -ls[e]));
-            dp[u][r] = s[u][r] * (dp[u][r] - de[e]);
+            dp[u][r] = s[u][r] * (kScaled<T> ? fmaf(dp[u][r], factor, -de[e]) : dp[u][r] - de[e]);
           }
         }
 #pragma unroll
@@ -613,13 +694,14 @@ template <typename T, int DP> __device__ __forceinline__ void attn_backward_kv(c
   }
   if (key >= a.Lk) return;
   const bool used = key < nk;             // behind the sequence's end a column held no key
+  const float of_dk = kScaled<T> ? a.scale * (kDvScale<T> / factor) : a.scale, of_dv = kDvScale<T>;
   if (a.kv_splits > 1) {
     const long long at = ((long long)split * a.B * a.Hk + group) * a.Lk + key, other = (long long)a.kv_splits * a.B * a.Hk * a.Lk * DP;
-    store_rows<float, DP>(a.part_kv + at * DP, dk, a.scale, used, DP, half);
-    store_rows<float, DP>(a.part_kv + other + at * DP, dv, 1.0f, used, DP, half);
+    store_rows<float, DP>(a.part_kv + at * DP, dk, of_dk, used, DP, half);
+    store_rows<float, DP>(a.part_kv + other + at * DP, dv, of_dv, used, DP, half);
   } else {
-    store_rows<T, DP>((T *)a.dk.p + (long long)b * a.dk.b + (long long)key * a.dk.r + (long long)hk * a.dk.h, dk, a.scale, used, a.D, half);
-    store_rows<T, DP>((T *)a.dv.p + (long long)b * a.dv.b + (long long)key * a.dv.r + (long long)hk * a.dv.h, dv, 1.0f, used, a.D, half);
+    store_rows<T, DP>((T *)a.dk.p + (long long)b * a.dk.b + (long long)key * a.dk.r + (long long)hk * a.dk.h, dk, of_dk, used, a.D, half);
+    store_rows<T, DP>((T *)a.dv.p + (long long)b * a.dv.b + (long long)key * a.dv.r + (long long)hk * a.dv.h, dv, of_dv, used, a.D, half);
   }
 }
 
@@ -662,6 +744,15 @@ template <typename T, int DP> __device__ __forceinline__ void attn_backward_q(co
   const long long at = ((long long)b * a.Hq + h) * a.Lq + i;
   // a row that sees nothing: probabilities 0
   const float lse = active ? a.lse[at] : -INFINITY, ls = lse == -INFINITY ? INFINITY : lse * kLog2e, de = active ? a.delta[at] : 0.0f;
+  float up = 0.0f;                        // f16: ds is taken times 2^up
+  if constexpr (kScaled<T>) {
+    float most_v = 0.0f;
+    const float *norm_v = a.norm_v + ((long long)b * a.Hk + hk) * a.Lk;
+    for (int j = begin + tid; j < block_end; j += 256) most_v = finite_max(most_v, norm_v[j]);
+    most_v = block_max(most_v, (float *)lds);
+    lds_barrier();
+    if (active) up = grad_shift(finite_max(0.0f, a.norm_do[at]) * most_v + finite_max(0.0f, fabsf(de)));
+  }
   f32x16 dq[kDt];
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt) dq[dt] = f32x16{};
@@ -703,7 +794,7 @@ template <typename T, int DP> __device__ __forceinline__ void attn_backward_q(co
 #pragma unroll
     for (int u = 0; u < kSub; ++u) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dp[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], a.scale2, -ls)) * (dp[u][r] - de);
+      for (int r = 0; r < 16; ++r) dp[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], a.scale2, up - ls)) * (dp[u][r] - de);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const Frag x = to_frag<T>(dp[u], t);
@@ -718,10 +809,11 @@ template <typename T, int DP> __device__ __forceinline__ void attn_backward_q(co
     }
   }
   if (!inside) return;
+  const float of_dq = kScaled<T> ? ldexpf(a.scale, -(int)up) : a.scale;
   if (a.q_splits > 1)
-    store_rows<float, DP>(a.part_q + (((long long)split * a.B * a.Hk + group) * ((long long)a.Lq * a.G) + row) * DP, dq, a.scale, active, DP, half);
+    store_rows<float, DP>(a.part_q + (((long long)split * a.B * a.Hk + group) * ((long long)a.Lq * a.G) + row) * DP, dq, of_dq, active, DP, half);
   else
-    store_rows<T, DP>((T *)a.dq.p + (long long)b * a.dq.b + (long long)i * a.dq.r + (long long)h * a.dq.h, dq, a.scale, active, a.D, half);
+    store_rows<T, DP>((T *)a.dq.p + (long long)b * a.dq.b + (long long)i * a.dq.r + (long long)h * a.dq.h, dq, of_dq, active, a.D, half);
 }
 
 // Both in one launch: the first workgroups make dk and dv, the others dq, so that neither leaves CUs idle at its end.  Seven products of
@@ -793,9 +885,10 @@ template <typename T, int DP> hipError_t attn_forward_dp(AttnArgs a, int narrow,
 }
 
 template <typename T, int DP> hipError_t attn_backward_dp(AttnArgs a, hipStream_t st) {
-  const long long rows = (long long)a.B * a.Lq * a.Hq;
+  const long long rows = (long long)a.B * a.Lq * a.Hq, v_rows = kScaled<T> ? (long long)a.B * a.Lk * a.Hk : 0;
   constexpr int kLanes = DP * sizeof(T) <= 128 ? 8 : 16, kPerBlock = 256 / kLanes;
-  hipLaunchKernelGGL((attn_delta_kernel<T, kLanes>), dim3((unsigned)((rows + kPerBlock - 1) / kPerBlock)), dim3(256), 0, st, a);
+  const long long v_blocks = std::min((v_rows + kPerBlock - 1) / kPerBlock, 1ll << 22);
+  hipLaunchKernelGGL((attn_delta_kernel<T, kLanes>), dim3((unsigned)((rows + kPerBlock - 1) / kPerBlock + v_blocks)), dim3(256), 0, st, a);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
   constexpr int kBytes = Tile<T, DP>::kBytes;
