@@ -131,6 +131,30 @@ def test_attention_f16_products_beyond_its_largest_number(O, shape):
             assert float((part[1].cpu().double() - part[0]).norm()) <= 2 * once, n
 
 
+@pytest.mark.parametrize("form", ["wide", "ranges"])
+def test_attention_f16_small_probabilities_add_up(O, form):
+    """One key takes 0.99 of a row, 300000 others 2^-25 of its probability each: together 0.009, whose values are 1 where the first one's is
+    0.  In f16's numbers next to 1 those that come behind it round to nothing.  Here they are taken times 2^9, 251 steps of f16's smallest: half a step is
+    0.002 of each, fp32's sums of n / 16 equal steps for o and the row's sum are off by 2^-24 per step at most, o is rounded once."""
+    n = 300000
+    B, Lq = (256, 64) if form == "wide" else (1, 8)
+    q = torch.zeros((B, Lq, 1, 64), dtype=torch.float16)
+    q[..., 0] = 8.0
+    k = torch.zeros((1, n, 1, 64), dtype=torch.float16)
+    k[0, n // 2, 0, 0] = 17.375                                 # score: 17.375, exp(-17.375) = 0.478 of 2^-24
+    v = torch.ones((1, n, 1, 64), dtype=torch.float16)
+    v[0, n // 2] = 0.0
+    share = math.exp(-17.375)
+    want = (n - 1) * share / (1 + (n - 1) * share)
+    o, lse = O.attention(cuda(q), cuda(k).expand(B, -1, -1, -1), cuda(v).expand(B, -1, -1, -1))
+    off = float((o.double() / want - 1).abs().max())
+    tol = 0.5 * 2.0 ** -24 / (share * 2.0 ** 9) + 2 * n / 16 * 2.0 ** -24 + R.unit(torch.float16)
+    assert off <= tol
+    # the row's sum takes in n / 64 tiles one after the other, each addition rounded by at most 2^-24 of the whole sum, which is 1 with the
+    # large key in it (not of the small keys' share): d(lse) = d(sum) / sum
+    assert float((lse.double() - (17.375 + math.log1p((n - 1) * share))).abs().max()) <= 2.0 ** -24 * (64 + 16 * 20 + n / 64)
+
+
 def test_scales_outside_of_32_bits_are_refused(O):
     """a scale that 32 bits hold as 0 would be read as the default; one that they hold as infinity (or whose product with log2(e) they do) has no exponentials"""
     q, z = torch.zeros((1, 4, 2, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((2, 50), device="cuda")

@@ -239,7 +239,10 @@ __device__ __forceinline__ float row_inverse(float l) { return l == 0.0f ? 0.0f 
 // ------------------------------------------------------------------ forward
 // workgroups of four waves per CU that the registers are kept for (fp32 rows of 128: twice the registers of everything)
 template <typename T, int DP> constexpr int kBlocksPerCu = sizeof(T) == 2 || DP <= 64 ? 2 : 1;
-constexpr float kSlack = 6.0f;      // log2: probabilities up to 64 before normalisation, in range of every type
+constexpr float kSlack = 6.0f;      // log2: probabilities may grow by 64 before the maximum moves
+// f16: probabilities start from 2^9, not from 1 (up to 2^15 with the slack): many small ones, which may be most of a row together, are
+// rounded to its subnormal numbers 2^9 times later (300000 keys of 2^-25 of the largest's probability: those behind it were lost altogether)
+template <typename T> constexpr float kLift = std::is_same<T, _Float16>::value ? 9.0f : 0.0f;
 // One workgroup: SPLIT = 0: 128 rows, 32 per wave, over tiles of 64 keys; SPLIT = 1: 32 rows, each of the four waves a quarter of
 // a 128-key tile, joined through LDS at the end (few rows: more workgroups, more loads in flight).  The key range may be cut in
 // `splits` parts, joined by attn_join_kernel.
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(256, (kBlocksPerCu<T, DP>)) attn_forward_kerne
   f32x16 acc[kDt];
 #pragma unroll
   for (int dt = 0; dt < kDt; ++dt) acc[dt] = f32x16{};
-  float m = -INFINITY, l = 0.0f;          // running maximum (log2 units) and this half wave's share of the sum
+  float m = -INFINITY, l = 0.0f;          // running maximum (log2 units; f16: 2^9 below it) and this half wave's share of the sum
   Stage<T, DP, kKeys> ks, vs;
   ks.start(kh, a.k.r, 0, 1, begin, a.D, tid);
   vs.start(vh, a.v.r, 0, 1, begin, a.D, tid);
@@ -335,8 +338,8 @@ __global__ void __launch_bounds__(256, (kBlocksPerCu<T, DP>)) attn_forward_kerne
     // The running maximum only has to keep the exponentials in range: it moves when some row of the wave has grown by more than
     // 2^kSlack, so that the accumulators are rescaled once or twice per row, not once per tile, and the half waves' maxima are
     // brought together only then.
-    if (__any(top * a.scale2 > m + kSlack)) {
-      const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * a.scale2), alpha = mn == -INFINITY ? 1.0f : exp2f(m - mn);
+    if (__any(top * a.scale2 > m + (kSlack + kLift<T>))) {
+      const float mn = fmaxf(m, fmaf(fmaxf(top, __shfl_xor(top, 32, 64)), a.scale2, -kLift<T>)), alpha = mn == -INFINITY ? 1.0f : exp2f(m - mn);
       m = mn;
       l *= alpha;
 #pragma unroll
