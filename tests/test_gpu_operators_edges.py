@@ -196,3 +196,18 @@ def test_what_torch_would_record_is_refused(O):
                  lambda: torch.func.grad(lambda x: O.log_probs(x).lse.sum())(z)):
         with pytest.raises((ValueError, RuntimeError)):
             call()
+
+
+def test_tensors_whose_memory_is_not_their_values_are_refused(O):
+    """torch puts a negation off (the memory holds the opposite), and a tensor of zeros may have no memory at all"""
+    q, z, f = (normal(s, torch.float32, 1).cuda() for s in ((1, 4, 2, 64), (2, 50), (2,)))
+    t, ix = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros((2, 3), dtype=torch.int32, device="cuda")
+    o, lse = O.attention(q, q, q)
+    none = torch._efficientzerotensor
+    for call in (lambda: O.attention(torch._neg_view(q), q, q), lambda: O.attention_backward(torch._neg_view(q), q, q, q, o, lse),
+                 lambda: O.attention_backward(q, q, q, q, o, torch._neg_view(lse)), lambda: O.log_probs(torch._neg_view(z)),
+                 lambda: O.distill_backward(torch._neg_view(f), z, ix, torch.zeros((2, 3), device="cuda"), f),
+                 lambda: O.attention(q, q, q, k_lens=none((1,), dtype=torch.int32, device="cuda")),
+                 lambda: O.log_probs(z, none((2,), dtype=torch.int32, device="cuda")), lambda: O.log_probs(none((2, 50), device="cuda"))):
+        with pytest.raises((ValueError, RuntimeError)):      # (the second: where the C ABI finds the null pointer)
+            call()

@@ -43,12 +43,15 @@ def _untraced(who):
         _refuse(who, "a trace would not record this call")
 
 
-def _unrecorded(who, name, t):
+def _given(who, name, t):
+    """what the kernels would not see of a tensor"""
     if t.requires_grad and torch.is_grad_enabled():
         _refuse(who, f"{name} requires a gradient, which this call would not record: call it under torch.no_grad() or with detached "
                      "tensors, and the backward call for the gradients")
     if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
         _refuse(who, f"{name} has a tangent, which this call would not carry on")
+    if t.is_neg():
+        _refuse(who, f"{name} is a negation that was put off: materialise it first (clone())")
 
 
 def _scores(who, name, t, device):
@@ -57,7 +60,7 @@ def _scores(who, name, t, device):
         _refuse(who, f"{name} has to be a tensor on the GPU")
     if t.dtype not in DTYPES:
         _refuse(who, f"{name} is {t.dtype} (float32, float16 or bfloat16)")
-    _unrecorded(who, name, t)
+    _given(who, name, t)
     if device is not None and t.device != device:
         _refuse(who, f"{name} is on {t.device}, not on {device}")
     return t.device
@@ -67,8 +70,11 @@ def _plain(who, name, t, dtype, shape, device):
     """a contiguous tensor of the given type and shape; its address"""
     if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.shape == shape and t.is_contiguous()):
         _refuse(who, f"{name} has to be a contiguous {dtype} tensor {tuple(shape)} on {device}")
-    _unrecorded(who, name, t)
-    return t.data_ptr()
+    _given(who, name, t)
+    p = t.data_ptr()
+    if not p and t.numel():
+        _refuse(who, f"{name} has no memory")
+    return p
 
 
 def _stream(device):
