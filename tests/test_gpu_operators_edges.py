@@ -211,3 +211,15 @@ def test_tensors_whose_memory_is_not_their_values_are_refused(O):
                  lambda: O.log_probs(z, none((2,), dtype=torch.int32, device="cuda")), lambda: O.log_probs(none((2, 50), device="cuda"))):
         with pytest.raises((ValueError, RuntimeError)):      # (the second: where the C ABI finds the null pointer)
             call()
+
+
+def test_sizes_beyond_32_bits_are_refused(O):
+    """broadcast views reach them without the memory"""
+    q, k, z = torch.zeros((1, 4, 2, 64), device="cuda"), torch.zeros((1, 1, 2, 64), device="cuda"), torch.zeros((1, 5), device="cuda")
+    f, ix = torch.zeros(1, device="cuda").expand(1 << 31), torch.zeros((1, 1), dtype=torch.int32, device="cuda").expand(1 << 31, 1)
+    long, many = k.expand(1, 1 << 31, 2, 64), z.expand(1 << 31, 5)
+    for call in (lambda: O.attention(q, long, long), lambda: O.attention(q[:, :1].expand(1 << 32, 1, 2, 64), k.expand(1 << 32, 1, 2, 64), k.expand(1 << 32, 1, 2, 64)),
+                 lambda: O.log_probs(many), lambda: O.log_probs(z[:, :1].expand(1, 1 << 31)), lambda: O.distill(many, ix, f[:, None]),
+                 lambda: O.log_probs_backward(many, None, f, f, d_entropy=f)):
+        with pytest.raises(ValueError):
+            call()

@@ -38,6 +38,13 @@ def _scale(who, name, x):
     return x
 
 
+def _config(who, layout, *values):
+    try:
+        return layout.pack(*values)
+    except struct.error:
+        _refuse(who, f"sizes beyond 32 bits: {values}")
+
+
 def _untraced(who):
     if torch._C._get_tracing_state() is not None:
         _refuse(who, "a trace would not record this call")
@@ -110,7 +117,7 @@ def _attn_config(who, q, k, v, causal, scale, q_lens, k_lens):
     if scale is not None:
         _scale(who, "scale", scale)
     lens = [None if t is None else _plain(who, name, t, torch.int32, (B,), device) for name, t in (("q_lens", q_lens), ("k_lens", k_lens))]
-    cfg = _ATTN_CONFIG.pack(DTYPES[q.dtype], B, Hq, Hk, D, Lq, Lk, 1 if causal else 0, scale or 0.0, device.index)
+    cfg = _config(who, _ATTN_CONFIG, DTYPES[q.dtype], B, Hq, Hk, D, Lq, Lk, 1 if causal else 0, scale or 0.0, device.index)
     return device, cfg, views, lens
 
 
@@ -184,7 +191,7 @@ def _rows_config(who, logits, scale):
     if V < 1 or (sv != 1 and V > 1):
         _refuse(who, "the rows of logits have to be contiguous and not empty")
     _scale(who, "scale", scale)
-    return device, R, V, _ROWS_CONFIG.pack(DTYPES[logits.dtype], R, V, sr, scale, device.index)
+    return device, R, V, _config(who, _ROWS_CONFIG, DTYPES[logits.dtype], R, V, sr, scale, device.index)
 
 
 @functools.lru_cache(maxsize=1024)
