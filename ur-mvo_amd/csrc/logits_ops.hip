@@ -833,8 +833,15 @@ int check_config(const urf_rows_config *c, const char *who) {
   return 0;
 }
 
+// rows that far apart are still within 64 bits of bytes
+bool stride_fits(long long stride, int rows) {
+  const long long most = (1ll << 59) / (rows > 1 ? rows : 1);
+  return rows <= 1 || (stride > -most && stride < most);
+}
+
 int check_rows(const urf_rows_config *c, const void *logits, const char *who) {
   if (check_config(c, who)) return -2;
+  URF_CHECK(stride_fits(c->row_stride, c->rows), "%s: rows %lld elements apart", who, c->row_stride);
   URF_CHECK(c->rows == 0 || logits, "%s: logits is null", who);
   URF_CHECK(((uintptr_t)logits & (dtype_bytes(c->dtype) - 1)) == 0, "%s: logits is not aligned to its elements", who);
   return 0;
@@ -845,6 +852,7 @@ int check_grad(const urf_rows_config *c, const void *logits, const void *d, long
   URF_CHECK(c->rows == 0 || d, "%s: d_logits is null", who);
   const long long b = dtype_bytes(c->dtype);
   URF_CHECK(((uintptr_t)d & (b - 1)) == 0, "%s: d_logits is not aligned to its elements", who);
+  URF_CHECK(stride_fits(stride, c->rows), "%s: rows of d_logits %lld elements apart", who, stride);
   URF_CHECK(c->rows <= 1 || stride >= c->classes, "%s: the rows of d_logits overlap (stride %lld, %d classes)", who, stride, c->classes);
   if (c->rows == 0) return 0;
   const long long in = c->row_stride * (c->rows - 1), n = c->classes;
