@@ -1,0 +1,28 @@
+"""tools/isa_barrier_audit.py on what the library is made of: every source whose kernels have a barrier, written out or through
+lds_barrier() of operator_common.h, compiled with the flags it is shipped with."""
+import importlib.util
+import os
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "ur-mvo_amd", "csrc")
+
+
+@pytest.fixture(scope="module")
+def A():
+    spec = importlib.util.spec_from_file_location("isa_barrier_audit", os.path.join(ROOT, "tools", "isa_barrier_audit.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    return m
+
+
+@pytest.mark.parametrize("op", ["s_load_dword s0, s[2:3], 0x0", "s_buffer_load_dwordx2 s[0:1], s[4:7], 0x0", "s_memtime s[0:1]", "s_memrealtime s[0:1]"])
+def test_scalar_memory_returns_out_of_order(A, op):
+    """a counted wait says nothing about an LDS write once a scalar memory operation is in flight beside it"""
+    def hits(body):
+        return A.audit_text("kern:\n" + body + "\n\ts_endpgm\n.Lfunc_end0:\n")
+    assert len(hits(f"\tds_write_b32 v0, v1\n\t{op}\n\ts_waitcnt lgkmcnt(1)\n\ts_barrier")) == 1
+    assert hits(f"\tds_write_b32 v0, v1\n\t{op}\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier") == []
+    for other in ("s_add_u32 s0, s1, s2", "s_setprio 1", "s_cmp_lg_u32 s0, 0", "s_and_saveexec_b64 s[0:1], vcc", "s_mov_b32 m0, s0"):
+        assert hits(f"\tds_write_b32 v0, v1\n\tds_read_b32 v2, v0\n\t{other}\n\ts_waitcnt lgkmcnt(1)\n\ts_barrier") == [], other

@@ -24,6 +24,8 @@ import tempfile
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CAP = 32
 DS_WRITE = re.compile(r"^ds_(write|add|sub|min|max|and|or|xor|inc|dec|mskor|cmpst|wrxchg|swizzle_never|append|consume|bpermute_never)")
+# scalar memory and cache operations of any kind, by the words in their names: they share the counter with LDS and return out of order
+SCALAR_MEMORY = re.compile(r"^s_(\w+_)?(load|memtime|memrealtime|atc|scratch|dcache|atomic|store)")
 BRANCH = re.compile(r"^(s_branch|s_cbranch_\w+|s_setpc_b64|s_endpgm)\b")
 
 
@@ -89,7 +91,7 @@ def transfer(state, t, hits, ln):
         if DS_WRITE.match(op):
             return (True, 0, False)
         return (pend, min(young + 1, CAP), smem) if pend else state
-    if op.startswith("s_load") or op.startswith("s_buffer_load") or op in ("s_memtime", "s_memrealtime", "s_dcache_inv", "s_dcache_wb") or op.startswith("s_atc") or op.startswith("s_scratch") or op.startswith("s_store"):
+    if SCALAR_MEMORY.match(op):
         return (pend, young, True) if pend else state
     if op.startswith("flat_"):
         return (pend, young, True) if pend else state
