@@ -26,3 +26,19 @@ def test_scalar_memory_returns_out_of_order(A, op):
     assert hits(f"\tds_write_b32 v0, v1\n\t{op}\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier") == []
     for other in ("s_add_u32 s0, s1, s2", "s_setprio 1", "s_cmp_lg_u32 s0, 0", "s_and_saveexec_b64 s[0:1], vcc", "s_mov_b32 m0, s0"):
         assert hits(f"\tds_write_b32 v0, v1\n\tds_read_b32 v2, v0\n\t{other}\n\ts_waitcnt lgkmcnt(1)\n\ts_barrier") == [], other
+
+
+def _make(name):
+    """a variable of the Makefile"""
+    for line in open(os.path.join(CSRC, "Makefile")):
+        if line.startswith(name + " :="):
+            return line.split(":=")[1].split()
+    raise KeyError(name)
+
+
+@pytest.mark.parametrize("source", [s for s in _make("OPERATORS") if s != "attention_api.hip"])
+def test_no_barrier_of_the_operators_is_reached_with_an_lds_write_in_flight(A, source):
+    """their barriers are all lds_barrier()'s, in headers: the sources' own text need not name one"""
+    text = A.compile_to_asm(os.path.join(CSRC, source), _make("NO_PACKED_FP32"))
+    assert "s_barrier" in text and A.audit_text(text) == []
+    assert not any(op in text for op in ("v_pk_add_f32", "v_pk_mul_f32", "v_pk_fma_f32"))
