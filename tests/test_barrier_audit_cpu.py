@@ -42,3 +42,12 @@ def test_no_barrier_of_the_operators_is_reached_with_an_lds_write_in_flight(A, s
     text = A.compile_to_asm(os.path.join(CSRC, source), _make("NO_PACKED_FP32"))
     assert "s_barrier" in text and A.audit_text(text) == []
     assert not any(op in text for op in ("v_pk_add_f32", "v_pk_mul_f32", "v_pk_fma_f32"))
+
+
+@pytest.mark.parametrize("source", ["sg_kernels.hip", "attn_h2.hip"])
+def test_no_kernel_is_built_with_packed_fp32_instructions(A, source):
+    """the sources whose code invites them (pairs of floats), with the flags every source is compiled with"""
+    flags = _make("NO_PACKED_FP32")
+    assert "$(NO_PACKED_FP32)" in _make("CXXFLAGS")
+    text = A.compile_to_asm(os.path.join(CSRC, source), flags)
+    assert not any(op in text for op in ("v_pk_add_f32", "v_pk_mul_f32", "v_pk_fma_f32"))

@@ -161,7 +161,7 @@ def compile_to_asm(src, extra=()):
     tmp = tempfile.NamedTemporaryFile(suffix=".s", delete=False)
     tmp.close()
     cmd = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-ffp-contract=off", "-fPIC", "-Wno-pass-failed",
-           "-S", "--cuda-device-only", "-o", tmp.name, src, *extra]
+           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-S", "--cuda-device-only", "-o", tmp.name, src, *extra]
     subprocess.check_call(cmd, stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
     text = open(tmp.name).read()
     os.unlink(tmp.name)

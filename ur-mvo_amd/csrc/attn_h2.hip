@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(64 * NW) attn_h2_il_kernel(const _Float16 *qkh
     const int kt = 2 * kp + (e >> 2), r = e & 3;
     if (u == 0) {
       const f32x2 sv = {s[t][kt][r], s[t][kt][r + 1]};
-      xd[q] = sv - f32x2{mn[t], mn[t]};            // v_pk_add_f32: the same two differences
+      xd[q] = sv - f32x2{mn[t], mn[t]};
     }
     if (u == 1) xp0[q] = __builtin_amdgcn_exp2f(xd[q][0]);
     if (u == 2) xp1[q] = __builtin_amdgcn_exp2f(xd[q][1]);

@@ -82,10 +82,9 @@ __device__ __forceinline__ float exp_c_nonpos(float x) {
   return x < -87.33654f ? 0.0f : v;
 }
 
-// Two softmax arguments at a time on the packed fp32 pipe (v_pk_mul_f32 / v_pk_fma_f32 / v_pk_add_f32: one instruction, two IEEE
-// operations per lane): the same operations on each element as exp_c_nonpos, hence the same bits -- 19 instructions per pair of
-// elements instead of 32.  The exact attention kernel spends 40 % of its time in this polynomial (fp32 VALU work does not hide under
-// the fp32 MFMAs on gfx950: EXPERIMENTS.md section 8, round 5).
+// Two softmax arguments at a time: the same operations on each element as exp_c_nonpos, hence the same bits, two independent chains
+// beside each other.  The exact attention kernel spends 40 % of its time in this polynomial (fp32 VALU work does not hide under the fp32
+// matrix instructions on gfx950).
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2 exp_c_nonpos2(f32x2 x) {
   auto fma2 = [](f32x2 a, f32x2 b, f32x2 c) { return __builtin_elementwise_fma(a, b, c); };
