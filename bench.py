@@ -71,28 +71,43 @@ def sg_attn_gflop(n0, n1):
 
 
 
-def kernel_source_sha():
-    """sha256 over the HIP sources of the library: a PMC summary is only quoted for the kernels it was taken on"""
+# no kernel of the measured path lives there: diagnostics, and the operators on caller-owned tensors
+OFF_THE_PATH = {"probes.hip", "attention_api.hip", "attention_f32.hip", "attention_f16.hip", "attention_bf16.hip", "attention_op.h",
+                "logits_ops.hip", "operator_common.h"}
+
+
+def kernel_source_sha(csrc=os.path.join(ROOT, "ur-mvo_amd", "csrc")):
+    """sha256 over the HIP sources of the path and the flags they are compiled with: a PMC summary is only quoted for the kernels it was
+    taken on"""
     h = hashlib.sha256()
-    for f in sorted(glob.glob(os.path.join(ROOT, "ur-mvo_amd", "csrc", "*.hip")) + glob.glob(os.path.join(ROOT, "ur-mvo_amd", "csrc", "*.h"))):
-        if os.path.basename(f) != "probes.hip":          # diagnostics only: no kernel of the path lives there
+    for f in sorted(glob.glob(os.path.join(csrc, "*.hip")) + glob.glob(os.path.join(csrc, "*.h"))):
+        if os.path.basename(f) not in OFF_THE_PATH:
             h.update(open(f, "rb").read())
+    for line in open(os.path.join(csrc, "Makefile")):
+        if line.split(" ")[0] in ("CXXFLAGS", "NO_PACKED_FP32"):
+            h.update(line.encode())
     return h.hexdigest()[:16]
+
+
+def _summary(name):
+    """the committed summary profiles/*`name`.json that was taken on the kernel sources of this tree, its file name; (None, why) else"""
+    files = sorted(glob.glob(os.path.join(ROOT, "profiles", f"*{name}.json")))
+    for f in reversed(files):
+        d = json.load(open(f))
+        if d.get("source_sha") == kernel_source_sha():
+            return d, os.path.basename(f)
+    return None, f"{len(files)} committed profiles/*{name}.json, none taken on these kernel sources (sha {kernel_source_sha()})"
 
 
 def pmc_traffic(kernel_label, resolution, prec):
     """HBM-side bytes per step of a kernel family, from the committed summary of the two rocprofv3 --pmc passes
     (FETCH_SIZE, WRITE_SIZE; tools/pmc_summary.py) of this same command.  bench.py cannot collect counters about
-    itself: the summary is the newest profiles/r*_pmc_hbm*.json for this resolution whose `source_sha` equals the
+    itself: the summary is the profiles/*pmc_hbm*.json for this resolution whose `source_sha` equals the
     sha of the kernel sources in this tree -- a summary taken on other kernels is refused (traffic = null)."""
     tag = ("" if resolution == "640x480" else "_" + resolution) + {0: "_exact", 1: "_fast", 2: "_guarded", 3: ""}[prec]
-    files = sorted(glob.glob(os.path.join(ROOT, "profiles", f"r*_pmc_hbm{tag}.json")))
-    if not files:
-        return None, "no committed PMC summary for this resolution"
-    d = json.load(open(files[-1]))
-    if d.get("source_sha") != kernel_source_sha():
-        return None, (f"{os.path.basename(files[-1])} was taken on other kernel sources (sha {d.get('source_sha')} != "
-                      f"{kernel_source_sha()}): refused")
+    d, file = _summary("pmc_hbm" + tag)
+    if d is None:
+        return None, file
     fam = ("conv_mfma_kernel<9,pool,fuse1a>" if "conv_mfma_kernel<9" in kernel_label else "linear_exact" if "gemm128" in kernel_label
            else "attn_kernel" if "(attn_kernel)" in kernel_label
            else "h2gemm" if "h2gemm" in kernel_label else "attn_h2_kernel" if "attn_h2" in kernel_label
@@ -102,11 +117,11 @@ def pmc_traffic(kernel_label, resolution, prec):
            else "sinkhorn_half_kernel" if "inkhorn" in kernel_label else "h2conv_kernel<pool,fuse1a>")
     k = d["kernels"].get(fam)
     if not k:
-        return None, f"{os.path.basename(files[-1])} has no {fam}"
+        return None, f"{file} has no {fam}"
     calls = d["superpoint_calls"] if (fam.startswith("h2conv") or fam.startswith("conv_mfma")) else d["matcher_calls"]
     return int(k["bytes_total"] / calls), (f"bytes per step = (2 x FETCH_SIZE + WRITE_SIZE) x 1024 summed over the "
                                            f"{k['launches'] // calls} {fam} launches of a step; L2-miss traffic incl. "
-                                           f"Infinity-Cache hits; {os.path.basename(files[-1])}")
+                                           f"Infinity-Cache hits; {file}")
 
 
 def pmc_mfma_busy(kernel_label, resolution, prec):
@@ -114,21 +129,18 @@ def pmc_mfma_busy(kernel_label, resolution, prec):
     GRBM_GUI_ACTIVE serialises the dispatches), from the committed summary (tools/pmc_mfma_summary.py) taken on THESE kernel
     sources; None otherwise.  Counter evidence beside the computed `mfma_issue_frac`, not a replacement for it."""
     tag = ("" if resolution == "640x480" else "_" + resolution) + {0: "_exact", 1: "_fast", 2: "_guarded", 3: ""}[prec]
-    files = sorted(glob.glob(os.path.join(ROOT, "profiles", f"r*_pmc_mfma{tag}.json")))
-    if not files:
-        return None, "no committed matrix-pipe PMC summary for this resolution and mode"
-    d = json.load(open(files[-1]))
-    if d.get("source_sha") != kernel_source_sha():
-        return None, f"{os.path.basename(files[-1])} was taken on other kernel sources: refused"
+    d, file = _summary("pmc_mfma" + tag)
+    if d is None:
+        return None, file
     fam = ("conv_mfma_kernel<9,pool,fuse1a>" if "conv_mfma_kernel<9" in kernel_label else "linear_exact" if "gemm128" in kernel_label
            else "attn_kernel" if "(attn_kernel)" in kernel_label
            else "h2gemm" if "h2gemm" in kernel_label else "attn_h2_kernel" if "attn_h2" in kernel_label
            else "h2conv_kernel<pool,fuse1a>" if "h2conv" in kernel_label else None)
     k = d["kernels"].get(fam) if fam else None
     if not k:
-        return None, f"{os.path.basename(files[-1])} has no matrix-core kernel for {kernel_label}"
+        return None, f"{file} has no matrix-core kernel for {kernel_label}"
     return k["mfma_busy_frac"], (f"SQ_VALU_MFMA_BUSY_CYCLES / (GRBM_GUI_ACTIVE per XCD x 1024 SIMDs) over the {k['launches']} {fam} launches of "
-                                 f"{os.path.basename(files[-1])} (each kernel alone on the chip)")
+                                 f"{file} (each kernel alone on the chip)")
 
 
 def stream_run(U, spb, sgb, dev, device_index, prec, Hh, Ww, batch, steps, repeats, warmup=5, keep=False):

@@ -12,23 +12,14 @@ the memory side of L2, i.e. Infinity-Cache hits are included: this is L2-miss tr
 bound on HBM bytes.
 """
 import collections
-import glob
-import hashlib
 import json
 import os
 import sqlite3
 import sys
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-
-
-def kernel_source_sha():
-    """must equal bench.kernel_source_sha(): bench.py refuses a summary taken on other kernel sources"""
-    h = hashlib.sha256()
-    for f in sorted(glob.glob(os.path.join(ROOT, "ur-mvo_amd", "csrc", "*.hip")) + glob.glob(os.path.join(ROOT, "ur-mvo_amd", "csrc", "*.h"))):
-        if os.path.basename(f) != "probes.hip":          # diagnostics only: no kernel of the path lives there
-            h.update(open(f, "rb").read())
-    return h.hexdigest()[:16]
+sys.path.insert(0, ROOT)
+from bench import kernel_source_sha  # noqa: E402  (bench.py quotes a summary for these sources only)
 
 
 def per_kernel(db):
