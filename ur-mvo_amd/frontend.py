@@ -301,9 +301,10 @@ class SuperGlue(_PM):
         top_log_prob [n0, top])."""
         n = getattr(self, "_n0", 0)
         if targets is not None:
-            targets = np.ascontiguousarray(targets, np.int32)
-            if targets.shape != (n,):
-                raise ValueError(f"match_log_probs: targets has to be [{n}], one per keypoint of image 0")
+            targets = np.asarray(targets)
+            if targets.shape != (n,) or targets.dtype.kind not in "iu":
+                raise ValueError(f"match_log_probs: targets has to be [{n}] integers, one per keypoint of image 0")
+            targets = np.ascontiguousarray(np.clip(targets, -1, np.iinfo(np.int32).max).astype(np.int32))
         lp = None if targets is None else np.zeros(n, np.float32)
         entropy, index, value = np.zeros(n, np.float32), np.zeros((n, max(top, 0)), np.int32), np.zeros((n, max(top, 0)), np.float32)
         check(_lib.lib().urf_sg_match_log_probs(self._h, _p(targets), top, _p(lp), _p(entropy), _p(index), _p(value)),
