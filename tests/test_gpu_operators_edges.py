@@ -155,6 +155,19 @@ def test_attention_f16_small_probabilities_add_up(O, form):
     assert float((lse.double() - (17.375 + math.log1p((n - 1) * share))).abs().max()) <= 2.0 ** -24 * (64 + 16 * 20 + n / 64)
 
 
+@pytest.mark.parametrize("form", [*FORMS.values(), (40, 100, 4, 4, 2, 64)], ids=[*FORMS, "few keys"])
+def test_attention_lse_of_16_bit_inputs_has_32(O, form):
+    """The same numbers as f16, bf16 and fp32 give the same scores and sums, all in 32 bits: one lse is as good as the other.  (Products of
+    16-bit numbers are exact, the order of sums differs: twice the fp32 call's error and a rounding of lse.)"""
+    B, Lq, Lk, Hq, Hk, D = form
+    q, k, v = (normal(s, torch.bfloat16, i).float().to(torch.float16) for i, s in enumerate([(B, Lq, Hq, D), (B, Lk, Hk, D), (B, Lk, Hk, D)]))
+    want = R.attention(q[-1:].float(), k[-1:].float(), v[-1:].float())["lse"][0]
+    off = {t: float((O.attention(cuda(q.to(t)), cuda(k.to(t)), cuda(v.to(t)))[1][-1:].cpu().double() - want).norm() / want.norm()) for t in DTYPES}
+    assert off[torch.float32] < 1e-6
+    for t in (torch.float16, torch.bfloat16):
+        assert off[t] <= 2 * off[torch.float32] + 2.0 ** -24, off
+
+
 def test_scales_outside_of_32_bits_are_refused(O):
     """a scale that 32 bits hold as 0 would be read as the default; one that they hold as infinity (or whose product with log2(e) they do) has no exponentials"""
     q, z = torch.zeros((1, 4, 2, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((2, 50), device="cuda")

@@ -231,18 +231,20 @@ __device__ __forceinline__ int clamp_len(const int *lens, int b, int most) {
   return lens ? min(max(lens[b], 0), most) : most;      // lengths come from device memory: never trusted beyond the tensor
 }
 
-// A row's lse and what its accumulators are divided by, from its maximum (log2 units) and sum.  The sum is 0 for a row that saw no key
-// and no other; a NaN, which a NaN or an infinite score leaves in it, goes into both.
-__device__ __forceinline__ float row_lse(float m, float l) { return l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2; }
-__device__ __forceinline__ float row_inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
-
 // ------------------------------------------------------------------ forward
 // workgroups of four waves per CU that the registers are kept for (fp32 rows of 128: twice the registers of everything)
 template <typename T, int DP> constexpr int kBlocksPerCu = sizeof(T) == 2 || DP <= 64 ? 2 : 1;
 constexpr float kSlack = 6.0f;      // log2: probabilities may grow by 64 before the maximum moves
 // f16: probabilities start from 2^9, not from 1 (up to 2^15 with the slack): many small ones, which may be most of a row together, are
 // rounded to its subnormal numbers 2^9 times later (300000 keys of 2^-25 of the largest's probability: those behind it were lost altogether)
-template <typename T> constexpr float kLift = std::is_same<T, _Float16>::value ? 9.0f : 0.0f;
+template <typename T> constexpr int kLift = std::is_same<T, _Float16>::value ? 9 : 0;
+// A row's lse and what its accumulators are divided by, from its maximum (log2 units, less kLift) and sum.  The sum is 0 for a row that saw
+// no key and no other; a NaN, which a NaN or an infinite score leaves in it, goes into both.  (The logarithm is taken of the sum
+// without the lift: near 9 its rounding would be most of the lse's error.)
+template <typename T> __device__ __forceinline__ float row_lse(float m, float l) {
+  return l == 0.0f ? -INFINITY : ((m + kLift<T>) + log2f(l * (1.0f / (1 << kLift<T>)))) * kLn2;
+}
+__device__ __forceinline__ float row_inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 // One workgroup: SPLIT = 0: 128 rows, 32 per wave, over tiles of 64 keys; SPLIT = 1: 32 rows, each of the four waves a quarter of
 // a 128-key tile, joined through LDS at the end (few rows: more workgroups, more loads in flight).  The key range may be cut in
 // `splits` parts, joined by attn_join_kernel.
@@ -414,12 +416,12 @@ __global__ void __launch_bounds__(256, (kBlocksPerCu<T, DP>)) attn_forward_kerne
 #pragma unroll
       for (int e = 0; e < kOwn; e += 4)
         if (d0 + e < a.D) store4<T>(orow + d0 + e, ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
-      if (wave == 0 && half == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = row_lse(m, l);
+      if (wave == 0 && half == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = row_lse<T>(m, l);
     }
   } else if (inside) {
     const float inv = row_inverse(l);
     store_rows<T, DP>((T *)a.o.p + (long long)b * a.o.b + (long long)i * a.o.r + (long long)(hk * a.G + g) * a.o.h, acc, inv, l != 0.0f, a.D, half);
-    if (half == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = row_lse(m, l);
+    if (half == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = row_lse<T>(m, l);
   }
 }
 
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 #pragma unroll
   for (int e = 0; e < kN; ++e)
     if (lane + 64 * e < a.D) orow[lane + 64 * e] = (T)(l == 0.0f ? 0.0f : o[e] * inv);
-  if (lane == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = row_lse(m, l);
+  if (lane == 0) a.lse[((long long)b * a.Hq + hk * a.G + g) * a.Lq + i] = row_lse<T>(m, l);
 }
 
 // ------------------------------------------------------------------ backward
