@@ -168,6 +168,36 @@ def test_attention_lse_of_16_bit_inputs_has_32(O, form):
         assert off[t] <= 2 * off[torch.float32] + 2.0 ** -24, off
 
 
+# Two roundings, of the terms (as above) and of the result, are sqrt(2) of one.  delta has to add little to that: from the rounded o it is off
+# by u |o|, which with n keys is sqrt(e / n) of what it is subtracted from, so that rows of 65 keys and more stay below sqrt(2 + 0.06), and
+# rows of fewer need a better one.  The terms' share is a sum of squares over few terms where there are few rows and keys: an error e is
+# uniform, e^2 has 0.8 of its mean squared as variance (second moment 1.8), and the terms' own sizes, products of a normal number and a
+# softmax weight, have a fourth moment of about 8 times the squared second: a relative standard deviation of sqrt(1.8 * 8 / terms), of
+# which three are allowed (16 for 14.4).  In dq the terms cancel a little: the keys a row prefers lie towards q, by 2 scale q among the terms
+# (weighted by p^2) and by scale q around their mean, so that sum |term|^2 is (1 + 4 / D) / (1 + 1 / D) = 1.05 of |sum|^2 for queries of
+# unit entries and 1.2 for those twice as long, which weigh more.  0.06 and, between the two, 0.14 make 2.2.
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=str)
+@pytest.mark.parametrize("keys", [2, 3, 15, 30, 64, 65, 90, 300])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attention_gradients_of_rows_with_few_keys(O, dtype, keys, causal, ragged):
+    """16-bit dq and dk are no worse where rows see a handful of keys; rows of the first tile, of later ones, of shared heads"""
+    B, Lq, Hq, Hk, D = 16, min(keys, 150) if causal else 150, 8, 4, 64
+    nk = [max(2, keys - b % 4 * keys // 5) for b in range(B)] if ragged else None
+    nq = [Lq - b % 3 for b in range(B)] if ragged and Lq > 3 else None
+    q, do = normal((B, Lq, Hq, D), dtype, 1), normal((B, Lq, Hq, D), dtype, 2)
+    k, v = normal((B, keys, Hk, D), dtype, 3), normal((B, keys, Hk, D), dtype, 4)
+    got = run_attention(O, cuda(q), cuda(k), cuda(v), cuda(do), causal, None, cuda(lens(nq)), cuda(lens(nk)))
+    want = R.attention(q, k, v, causal, None, nq, nk, do)
+    terms = sum(Hq * (min(max(0, i + 1 + c - a), c) if causal else c) for a, c in zip(nq or [Lq] * B, nk or [keys] * B) for i in range(a))
+    for n in ("dq", "dk", "dv"):
+        x = want[n][0]
+        once = float((x.to(dtype).double() - x).norm())
+        off = float((got[n].cpu().double() - x).norm())
+        assert off <= math.sqrt(2.2 + 3 * math.sqrt(16 / terms)) * once, (n, off / once)
+    R.check(got, want)
+
+
 def test_scales_outside_of_32_bits_are_refused(O):
     """a scale that 32 bits hold as 0 would be read as the default; one that they hold as infinity (or whose product with log2(e) they do) has no exponentials"""
     q, z = torch.zeros((1, 4, 2, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((2, 50), device="cuda")

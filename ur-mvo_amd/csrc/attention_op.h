@@ -38,6 +38,7 @@ struct AttnArgs {
   int splits;                    // forward: key ranges
   int tiles;                     // its row tiles per (sequence, key head)
   int kv_tiles, kv_splits, q_tiles, q_splits;   // backward: tiles of 128 keys / rows, and ranges of the other side
+  int few_tiles;                 // backward: tiles of 128 rows per (sequence, key head) that may hold rows of few keys
   float scale, scale2;           // scale, scale * log2(e)
 };
 
@@ -483,19 +484,80 @@ __device__ __forceinline__ float block_max(float m, float *lds) {
   return fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
 }
 
-// delta_i = do_i . o_i: L lanes per row, 16 bytes of each tensor at a time; 8 where that is a row of 64 16-bit elements, 16 otherwise.
+// Rows that see up to 64 keys, 16-bit types: delta_i = sum_j p_ij (do_i . v_j) in fp32.  o was rounded, and where few keys share a row that
+// error is as large as the gradients' own rounding (4 keys: dq and dk off by 2.05 of what one rounding costs, 15: 1.74, 30: 1.59; two
+// roundings, of ds and of the result, are 1.41).  With more keys o's entries are small beside v's, and do . o is as good.
+constexpr int kFewKeys = 64;
+// the keys of row i of nq, if these are few, or 0
+__device__ __forceinline__ int few_keys(int i, int nq, int nk, int causal) {
+  const int seen = i >= nq ? 0 : causal ? min(nk, max(0, i + 1 + nk - nq)) : nk;
+  return seen <= kFewKeys ? seen : 0;
+}
+template <typename T, int DP> __device__ __forceinline__ void attn_few_keys(const AttnArgs &a, int id, char *lds) {
+  typedef Tile<T, DP> TL;
+  typedef typename Elem<T>::Frag Frag;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5, col = lane & 31;
+  const unsigned row_base = TL::row_base(col, half);
+  const int group = id / a.few_tiles, tile = id - group * a.few_tiles, b = group / a.Hk, hk = group % a.Hk;
+  const int nq = clamp_len(a.q_lens, b, a.Lq), nk = clamp_len(a.k_lens, b, a.Lk);
+  const int i_first = max(tile * 128 / a.G, a.causal ? nq - nk : 0), i_last = min(nq, (min((tile + 1) * 128, a.Lq * a.G) - 1) / a.G + 1) - 1;
+  if (i_first > i_last || few_keys(i_first, nq, nk, a.causal) == 0) return;        // the first row that sees a key sees the fewest
+  const int end = a.causal ? min(min(nk, kFewKeys), i_last + 1 + nk - nq) : nk;
+  const int row = tile * 128 + 32 * wave + col, i = row / a.G, g = row - i * a.G, h = hk * a.G + g, few = few_keys(i, nq, nk, a.causal);
+  const T *qrow = (const T *)a.q.p + (long long)b * a.q.b + (long long)i * a.q.r + (long long)h * a.q.h;
+  const T *drow = (const T *)a.dout.p + (long long)b * a.dout.b + (long long)i * a.dout.r + (long long)h * a.dout.h;
+  constexpr int kTile = kFewKeys * TL::kBytes;
+  {
+    Stage<T, DP, kFewKeys> x;
+    x.start((const T *)a.k.p + (long long)b * a.k.b + (long long)hk * a.k.h, a.k.r, 0, 1, 0, a.D, tid);
+    x.load(end);
+    x.store(lds, tid);
+    x.start((const T *)a.v.p + (long long)b * a.v.b + (long long)hk * a.v.h, a.v.r, 0, 1, 0, a.D, tid);
+    x.load(end);
+    x.store(lds + kTile, tid);
+  }
+  const long long at = ((long long)b * a.Hq + h) * a.Lq + i;
+  const float lse = few ? a.lse[at] : -INFINITY, ls = lse == -INFINITY ? INFINITY : lse * kLog2e;
+  lds_barrier();
+  float delta = 0.0f;
+#pragma unroll
+  for (int u = 0; u < kFewKeys / 32; ++u) {
+    f32x16 s = {}, dp = {};
+#pragma unroll
+    for (int kc = 0; kc < DP / 16; ++kc) {
+      s = Elem<T>::mma(TL::row(lds, row_base, 32 * u, kc), load_frag<T>(qrow, few, kc, half, a.D), s);
+      dp = Elem<T>::mma(TL::row(lds + kTile, row_base, 32 * u, kc), load_frag<T>(drow, few, kc, half, a.D), dp);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (32 * u + 4 * half + 8 * (r >> 2) + (r & 3) < few) delta = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -ls)), dp[r], delta);
+  }
+  delta += __shfl_xor(delta, 32, 64);
+  if (few && half == 0) a.delta[at] = delta;
+}
+
+// delta_i = do_i . o_i of the other rows: L lanes per row, 16 bytes of each tensor at a time; 8 where that is a row of 64 16-bit elements, 16
+// otherwise.  FEW: the first workgroups do the rows of few keys; 0 where none can have few.
 // Bound by memory: 2 x 4096 rows of 16 heads of 128, bf16, 67 MB each of o and do in 13 us (10.3 TB/s: what the forward pass wrote is in
 // the last-level cache).
-template <typename T, int L>
-__global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a) {
+template <typename T, int DP, int L, bool FEW>
+__global__ void __launch_bounds__(256, FEW ? 4 : 0) attn_delta_kernel(AttnArgs a) {
+  extern __shared__ __align__(16) char lds[];
+  unsigned block = blockIdx.x;
+  if constexpr (FEW) {
+    const unsigned few_blocks = a.few_tiles * a.B * a.Hk;
+    if (block < few_blocks) return attn_few_keys<T, DP>(a, block, lds);
+    block -= few_blocks;
+  }
   constexpr int kPer = 16 / (int)sizeof(T);
   constexpr bool kNorms = kScaled<T>;
   constexpr unsigned kRows = 256 / L;
   const int c = threadIdx.x % L;
   if constexpr (kNorms) {
     const unsigned do_blocks = (a.B * a.Lq * a.Hq + kRows - 1) / kRows, v_rows = a.B * a.Lk * a.Hk;
-    if (blockIdx.x >= do_blocks) {                         // rows (b, j, h) of v
-      for (unsigned u = (blockIdx.x - do_blocks) * kRows + threadIdx.x / L; u < v_rows; u += (gridDim.x - do_blocks) * kRows) {
+    if (block >= do_blocks) {                              // rows (b, j, h) of v
+      const unsigned v_blocks = gridDim.x - (blockIdx.x - block) - do_blocks;
+      for (unsigned u = (block - do_blocks) * kRows + threadIdx.x / L; u < v_rows; u += v_blocks * kRows) {
         const unsigned uh = u / a.Hk;
         const int h = u - uh * a.Hk, b = uh / a.Lk, j = uh - b * a.Lk;
         float s = 0.0f;
@@ -515,7 +577,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a) {
       return;
     }
   }
-  const unsigned u = blockIdx.x * kRows + threadIdx.x / L;
+  const unsigned u = block * kRows + threadIdx.x / L;
   const unsigned uh = u / a.Hq;                            // row (b, i, h), (b, i)
   const bool inside = u < (unsigned)(a.B * a.Lq * a.Hq);
   const int h = u - uh * a.Hq, b = inside ? uh / a.Lq : 0, i = uh - b * a.Lq;
@@ -539,7 +601,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnArgs a) {
     if (kNorms) ss += __shfl_xor(ss, x, L);
   }
   if (inside && c == 0) {
-    a.delta[((long long)b * a.Hq + h) * a.Lq + i] = s;
+    if (!FEW || !few_keys(i, clamp_len(a.q_lens, b, a.Lq), clamp_len(a.k_lens, b, a.Lk), a.causal)) a.delta[((long long)b * a.Hq + h) * a.Lq + i] = s;
     if (kNorms) a.norm_do[((long long)b * a.Hq + h) * a.Lq + i] = sqrtf(ss);
   }
 }
@@ -893,10 +955,20 @@ template <typename T, int DP> hipError_t attn_backward_dp(AttnArgs a, hipStream_
   const long long rows = (long long)a.B * a.Lq * a.Hq, v_rows = kScaled<T> ? (long long)a.B * a.Lk * a.Hk : 0;
   constexpr int kLanes = DP * sizeof(T) <= 128 ? 8 : 16, kPerBlock = 256 / kLanes;
   const long long v_blocks = std::min((v_rows + kPerBlock - 1) / kPerBlock, 1ll << 22);
-  hipLaunchKernelGGL((attn_delta_kernel<T, kLanes>), dim3((unsigned)((rows + kPerBlock - 1) / kPerBlock + v_blocks)), dim3(256), 0, st, a);
+  constexpr int kBytes = Tile<T, DP>::kBytes;
+  // rows of few keys: none unless the keys are few, a length that only the device knows may be, or a causal call begins with few
+  const long long begin = (long long)a.Lk - a.Lq + 1;      // causal, all in use: the keys of row 0
+  const bool unknown = a.k_lens || (a.causal && a.q_lens);
+  const long long few_rows = sizeof(T) == 4 || a.Lk == 0 ? 0 : unknown || a.Lk <= kFewKeys ? a.Lq
+                           : a.causal && begin <= kFewKeys ? std::min<long long>(a.Lq, kFewKeys + 1 - begin) : 0;
+  a.few_tiles = (int)((few_rows * a.G + 127) / 128);
+  const unsigned delta_grid = (unsigned)((long long)a.few_tiles * a.B * a.Hk + (rows + kPerBlock - 1) / kPerBlock + v_blocks);
+  if constexpr (sizeof(T) == 2) {
+    if (a.few_tiles) hipLaunchKernelGGL((attn_delta_kernel<T, DP, kLanes, true>), dim3(delta_grid), dim3(256), 2 * kFewKeys * kBytes, st, a);
+  }
+  if (!a.few_tiles) hipLaunchKernelGGL((attn_delta_kernel<T, DP, kLanes, false>), dim3(delta_grid), dim3(256), 0, st, a);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
-  constexpr int kBytes = Tile<T, DP>::kBytes;
   static DeviceOnce once;
   const int lds = 128 * kBytes + 4 * 32 * kBackwardSub<T, DP> * kBytes + 1024;
   rc = allow_lds(once, (const void *)attn_backward_kernel<T, DP>, lds);
