@@ -198,6 +198,42 @@ def test_attention_gradients_of_rows_with_few_keys(O, dtype, keys, causal, ragge
     R.check(got, want)
 
 
+@pytest.mark.parametrize("rows,classes,pad", [(9000, 1025, 3), (5000, 2048, 0), (6, 1500, 1), (300, 777, 0), (5000, 300, 0), (4100, 1025, 0)])
+@pytest.mark.parametrize("tail", [None, False, True], ids=["log_probs", "distill", "distill with the rest"])
+def test_fp32_gradients_are_not_off_by_the_rounding_of_lse(O, rows, classes, pad, tail):
+    """lse is about 20: rounded to 32 bits it is off by up to 16 times 2^-24, and a probability by as much of itself.  What the kernels may
+    lose, per probability p = exp(x), in units of 2^-24: two roundings of x (|x| each), one of the exponential (2), the sum's (5 after
+    some 26 additions of random errors) and the products' (2), each 0.58 of that in the mean: at most 2 + |x|; of what is listed,
+    one.  Student and teacher nearly agree."""
+    g = torch.Generator().manual_seed(rows)
+    teacher = torch.randn((rows, classes + pad), generator=g)[:, :classes] * 2 + 10
+    z = (teacher + 0.2 * torch.randn((rows, classes), generator=g)).contiguous()
+    zc = torch.zeros((rows, classes + pad), device="cuda")[:, :classes].copy_(cuda(z))
+    x = z.double() - torch.logsumexp(z.double(), 1, keepdim=True)
+    p = x.exp()
+    if tail is None:
+        w, at = torch.rand(rows, generator=g), torch.randint(0, classes, (rows, 1), generator=g, dtype=torch.int32)
+        r = O.log_probs(zc, cuda(at))
+        got = O.log_probs_backward(zc, cuda(at), r.lse, r.entropy, d_log_prob=cuda(w[:, None].contiguous()))
+        want = torch.zeros_like(p).scatter_add_(1, at.long(), torch.ones((rows, 1), dtype=torch.float64)) - p
+        # what is subtracted is 1: the gradient of the target itself is 1 - p, rounded
+        room = (2 + x.abs()) * p + want.abs()
+        want, room = want * w[:, None].double(), room * w[:, None].double()
+    else:
+        t = O.log_probs(cuda(teacher.contiguous()), top=20)
+        index, value = t.top_index, t.top_log_prob
+        if not tail:
+            value = cuda(teacher).gather(1, index.long())
+        w = torch.rand(rows, generator=g)
+        r = O.distill(zc, index, value, tail=tail)
+        got = O.distill_backward(cuda(w), zc, index, value, r.lse, r.log_tail, tail=tail)
+        want = R.distill(z, index.cpu(), value.cpu(), 1.0, tail, w)["d_logits"][0]
+        share = torch.zeros_like(p).scatter_add_(1, index.cpu().long(), torch.softmax(value.double().cpu(), 1))
+        room = ((2 + x.abs()) * p + 2 * share) * w[:, None].double()
+    off = float((got.cpu().double() - want).norm())
+    assert off <= 2.0 ** -24 * float(room.norm()), off / (2.0 ** -24 * float(room.norm()))
+
+
 def test_scales_outside_of_32_bits_are_refused(O):
     """a scale that 32 bits hold as 0 would be read as the default; one that they hold as infinity (or whose product with log2(e) they do) has no exponentials"""
     q, z = torch.zeros((1, 4, 2, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((2, 50), device="cuda")

@@ -29,7 +29,8 @@ static_assert(URF_TOP_MAX == 64, "one listed candidate per lane");
 constexpr int kUnroll = 4;               // 16-byte loads in flight per lane
 constexpr double kLog2eDouble = 1.4426950408889634;
 constexpr int kMostParts = 32;           // of a row
-constexpr int kShort = 8 * URF_TOP_MAX;  // classes of a row that the listed candidates may be a large part of
+constexpr int kShort = 2048;             // classes of an fp32 row whose gradient is normalised by the row's own sum (exact_lse)
+constexpr int kKept = kShort / 256;      // vectors of it per lane of a wave
 constexpr float kNothing = -0x1p100f;    // a row whose largest scaled score is below it allows nothing (masks of -inf or the lowest value)
 constexpr float kFloor = -1.0e4f;        // 2^kFloor is 0: a masked score (-inf) adds 0 * kFloor to A, not 0 * inf
 
@@ -569,9 +570,31 @@ __device__ __forceinline__ void set_shift(float &hi, float &lo, double shift) {
   lo = (float)(shift - (double)hi);
 }
 
-// STREAM: written past the caches (a template: the compiler joins two stores that differ in this only)
-template <typename T, bool ENTROPY, bool TAIL, bool STREAM>
-__device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float scale, const GradRow &g, int part, int parts, int lane) {
+// a short row, read once for its sum and its gradient: its vectors, and the score that a lane takes before or behind them
+template <typename T> struct Kept {
+  typename Row<T>::Vec v[kKept];
+  float extra;
+};
+template <typename T> __device__ __forceinline__ Kept<T> keep_row(const T *z, int V, int lane) {
+  typedef Row<T> RW;
+  constexpr int kPer = RW::kPer;
+  const int head = RW::template head<64>(z, V), tail = (V - head) % kPer, at = lane >= head + tail ? -1 : lane < head ? lane : V - tail + lane - head;
+  Kept<T> k;
+#pragma unroll
+  for (int s = 0; s < kKept; ++s) {
+    const int first = (s * 64 + lane) * kPer;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) k.v[s][e] = (T)-INFINITY;
+    if (first + kPer <= V - head) k.v[s] = *(const typename RW::Vec *)(z + head + first);
+  }
+  k.extra = at >= 0 ? (float)z[at] : -INFINITY;
+  return k;
+}
+
+// STREAM: written past the caches (a template: the compiler joins two stores that differ in this only).  KEEP: the row is in `kept`, 1: its
+// scores, 2: its probabilities, which coef and lcoef are of
+template <typename T, bool ENTROPY, bool TAIL, bool STREAM, int KEEP>
+__device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float scale, const GradRow &g, int part, int parts, int lane, const Kept<T> &kept) {
   typedef Row<T> RW;
   constexpr int kPer = RW::kPer, kStep = 64 * kPer;
   auto exponent = [&](float f, float shift, float slo) {
@@ -579,6 +602,7 @@ __device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float scale,
     return (sizeof(T) == 4 ? d - slo : d) * kLog2e;
   };
   auto grad = [&](float f) {
+    if (KEEP == 2) return f * g.coef;
     const float x = exponent(f, g.shift, g.slo), p = __builtin_amdgcn_exp2f(x);
     if (ENTROPY) return p * fmaf(-g.h, fmaxf(x, kFloor) + g.ent2, g.coef);
     return p * g.coef;
@@ -590,7 +614,7 @@ __device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float scale,
         const int at = __shfl(g.mine, (int)__ffsll((long long)h) - 1, 64) - first;
 #pragma unroll
         for (int e = 0; e < n; ++e)
-          if (e == at) d[e] = g.lcoef * __builtin_amdgcn_exp2f(exponent(f[e], g.lshift, g.lslo));
+          if (e == at) d[e] = g.lcoef * (KEEP == 2 ? f[e] : __builtin_amdgcn_exp2f(exponent(f[e], g.lshift, g.lslo)));
       }
     for (u64 h = hits; h; h &= h - 1) {                    // what each mention adds, in the list's order
       const int src = (int)__ffsll((long long)h) - 1, at = __shfl(g.mine, src, 64) - first;
@@ -609,12 +633,13 @@ __device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float scale,
   const bool loose = (uintptr_t)dz & 15;
   const int steps = (V / kPer + 63) / 64;
   const int b0 = (int)((long long)steps * part / parts), b1 = (int)((long long)steps * (part + 1) / parts);
-  for (int b = b0; b < b1; b += kUnroll) {
+  auto steps_from = [&](int b) __attribute__((always_inline)) {
     float f[kUnroll][kPer];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int first = (b + u) * kStep + lane * kPer;
-      if (b + u < b1 && first + kPer <= V) RW::load(z + first, f[u]);
+      if constexpr (KEEP) RW::spread(kept.v[b + u], f[u]);
+      else if (b + u < b1 && first + kPer <= V) RW::load(z + first, f[u]);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
@@ -634,10 +659,17 @@ __device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float scale,
           else *(typename RW::Vec *)(dz + first) = o;
         }
       }
+  };
+  if constexpr (KEEP) {
+#pragma unroll
+    for (int b = 0; b < kKept; b += kUnroll)
+      if (b < b1) steps_from(b);
+  } else {
+    for (int b = b0; b < b1; b += kUnroll) steps_from(b);
   }
   if (part == 0 && head + tail) {
     const int at = lane >= head + tail ? -1 : lane < head ? lane : all - tail + lane - head;
-    const float f[1] = {at >= 0 ? (float)row[at] : -INFINITY};
+    const float f[1] = {KEEP ? kept.extra : at >= 0 ? (float)row[at] : -INFINITY};
     float d[1] = {grad(f[0])};
     const u64 hits = __ballot(g.mine >= 0 && (g.mine < head || g.mine >= all - tail));
     if (hits) listed(f, d, 1, at, hits);
@@ -646,9 +678,11 @@ __device__ __forceinline__ void grad_pass(const T *z, T *dz, int V, float scale,
 }
 
 // A row's lse from the one that was rounded to 32 bits.  Where probability and what is subtracted from it are close, that rounding is
-// all that would be left of a gradient (rows of five classes, all of them listed, fp32: 1.7e-6 of its norm, 3e-7 so).  The sum of
-// the probabilities says how far it is off; rows that the listed candidates may be a large part of are short and summed again (8192 rows
-// of 200: 5.8 -> 6.8 us; up to 4096 classes it would cost 8192 rows of 4000 43 -> 58).  16-bit gradients are rounded coarser than that.
+// all that would be left of a gradient (fp32: rows of five classes, all of them listed: 1.7e-6 of its norm, 3e-7 so; 1585 classes, 20
+// listed, student near its teacher: 1.6e-6, 3.8e-7).  The sum of the probabilities says how far it is off.  A wave that has its row to
+// itself reads it once for both (us for 8200 rows of 1025, distillation / log probabilities: 17.7 / 14.5; without the sum 15.5 / 13.3, read
+// twice 19.0 / 16.5); where a few rows are spread over waves each reads all of it.  Longer rows keep the rounded lse (their gradients are
+// off by up to 8e-7).  16-bit gradients are rounded coarser than that.
 template <typename T> __device__ __forceinline__ double exact_lse(const T *z, int V, float scale, float lse, int lane) {
   if constexpr (sizeof(T) == 4) {
     if (V <= kShort) {
@@ -665,13 +699,32 @@ template <typename T> __device__ __forceinline__ double exact_lse(const T *z, in
   }
   return lse;
 }
+// of a kept row: the sum of its probabilities by the rounded lse, which replace the scores if asked to (PROBS)
+template <typename T, bool PROBS> __device__ __forceinline__ float kept_sum(Kept<T> &k, int V, float scale, float lse) {
+  float sum = 0.0f;
+  auto p_of = [&](float f) {
+    const float p = __builtin_amdgcn_exp2f(fmaf(f, scale, -lse) * kLog2e);
+    sum += p;
+    return PROBS ? p : f;
+  };
+#pragma unroll
+  for (int s = 0; s < kKept; ++s)
+    if (256 * s < V)                                       // (the same for all lanes)
+#pragma unroll
+      for (int e = 0; e < Row<T>::kPer; ++e) k.v[s][e] = p_of(k.v[s][e]);
+  k.extra = p_of(k.extra);
+  return row_sum<64>(sum);
+}
 
-template <typename T, bool ENTROPY, bool STREAM>
+template <typename T, bool ENTROPY, bool STREAM, bool KEEP>
 __global__ void __launch_bounds__(256) log_probs_backward_kernel(RowsArgs a) {
   const int lane = threadIdx.x & 63;
   const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int r = a.R - 1 - (int)(w / a.per_row), part = (int)(w % a.per_row);      // the last rows, read last by the forward pass, first
   if (r < 0) return;
+  const T *z = (const T *)a.z + (long long)r * a.stride;
+  Kept<T> kept;
+  if constexpr (KEEP) kept = keep_row(z, a.V, lane);
   const float lse = a.lse[r];
   const bool empty = lse == -INFINITY;                    // no score to choose from: constant outputs, no gradient
   GradRow g = {};
@@ -683,28 +736,47 @@ __global__ void __launch_bounds__(256) log_probs_backward_kernel(RowsArgs a) {
     else own = a.g1[(long long)r * a.N + lane];
   }
   g.add = own * a.scale;
-  set_shift(g.shift, g.slo, empty ? 0.0 : exact_lse((const T *)a.z + (long long)r * a.stride, a.V, a.scale, lse, lane));
+  double exact = empty ? 0.0 : lse;
+  if constexpr (KEEP) exact += empty ? 0.0f : logf(kept_sum<T, false>(kept, a.V, a.scale, lse));
+  else if (!empty) exact = exact_lse(z, a.V, a.scale, lse, lane);
+  set_shift(g.shift, g.slo, exact);
   g.coef = empty ? 0.0f : -row_sum<64>(own) * a.scale;
   if (ENTROPY && !empty) {
     g.h = a.g2[r] * a.scale * kLn2;
     g.ent2 = a.entropy[r] * kLog2e;
   }
-  grad_pass<T, ENTROPY, false, STREAM>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.scale, g, part, a.per_row, lane);
+  grad_pass<T, ENTROPY, false, STREAM, KEEP ? 1 : 0>(z, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.scale, g, part, a.per_row, lane, kept);
 }
 
-template <typename T, bool TAIL, bool STREAM>
+template <typename T, bool TAIL, bool STREAM, bool KEEP>
 __global__ void __launch_bounds__(256) distill_backward_kernel(RowsArgs a) {
   const int lane = threadIdx.x & 63;
   const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int r = a.R - 1 - (int)(w / a.per_row), part = (int)(w % a.per_row);      // the last rows, read last by the forward pass, first
   if (r < 0) return;
+  const T *z = (const T *)a.z + (long long)r * a.stride;
+  Kept<T> kept;
+  if constexpr (KEEP) kept = keep_row(z, a.V, lane);
   const Teacher t = teacher_of<TAIL, 64>(a, r, lane);
   const double gs = (double)a.g1[r] * a.scale;
   const bool empty = a.lse[r] == -INFINITY;
-  const double lse = empty ? 0.0 : exact_lse((const T *)a.z + (long long)r * a.stride, a.V, a.scale, a.lse[r], lane);
   GradRow g = {};
   g.mine = empty ? -1 : t.index;
   g.add = (float)(-gs * t.p);
+  T *dz = (T *)a.dz + (long long)r * a.dz_stride;
+  double lse = empty ? 0.0 : a.lse[r];
+  if constexpr (KEEP) {
+    const float tail = TAIL ? a.log_tail[r] : 0.0f, sum = empty ? 1.0f : kept_sum<T, true>(kept, a.V, a.scale, (float)lse);
+    // the probabilities are at hand unless the unlisted ones are too small next to the listed
+    if (!empty && !(tail < -40.0f)) {
+      g.lcoef = (float)(gs * t.mass / sum);
+      g.coef = TAIL ? (float)(gs * (t.mass - t.rest * expf(-tail)) / sum) : g.lcoef;
+      return grad_pass<T, false, TAIL, STREAM, 2>(z, dz, a.V, a.scale, g, part, a.per_row, lane, kept);
+    }
+    lse += logf(sum);
+  } else if (!empty) {
+    lse = exact_lse(z, a.V, a.scale, a.lse[r], lane);
+  }
   set_shift(g.shift, g.slo, lse);
   g.coef = empty ? 0.0f : (float)(gs * t.mass);
   if (TAIL) {
@@ -719,7 +791,7 @@ __global__ void __launch_bounds__(256) distill_backward_kernel(RowsArgs a) {
       g.coef = (float)(gs * (t.mass * expf(tail) - t.rest));
     }
   }
-  grad_pass<T, false, TAIL, STREAM>((const T *)a.z + (long long)r * a.stride, (T *)a.dz + (long long)r * a.dz_stride, a.V, a.scale, g, part, a.per_row, lane);
+  grad_pass<T, false, TAIL, STREAM, 0>(z, dz, a.V, a.scale, g, part, a.per_row, lane, kept);
 }
 
 // ------------------------------------------------------------------ launches
@@ -766,6 +838,9 @@ inline bool two_rows(int R, int V, int lists, int bytes) {
   return R >= 2048 && size <= 6144 && 2 * size <= 3ll * R && lists <= 32;
 }
 
+// fp32 gradients: short rows that a wave has to itself are kept in its registers
+inline bool keeps(const RowsArgs &a) { return a.V <= kShort && a.per_row == 1; }
+
 template <typename T> hipError_t launch_log_probs(const RowsArgs &a, hipStream_t st) {
   if (a.parts) {
     auto part = a.K ? log_probs_part_kernel<T, true> : log_probs_part_kernel<T, false>;
@@ -801,8 +876,12 @@ template <typename T> hipError_t launch_log_probs_backward(RowsArgs a, hipStream
   a.per_row = grad_waves(a.R, a.V, sizeof(T));
   const bool far = streams(a, sizeof(T));
   const dim3 grid((unsigned)(((long long)a.R * a.per_row + 3) / 4));
-  auto kernel = a.g2 ? (far ? log_probs_backward_kernel<T, true, true> : log_probs_backward_kernel<T, true, false>)
-                     : (far ? log_probs_backward_kernel<T, false, true> : log_probs_backward_kernel<T, false, false>);
+  auto kernel = a.g2 ? (far ? log_probs_backward_kernel<T, true, true, false> : log_probs_backward_kernel<T, true, false, false>)
+                     : (far ? log_probs_backward_kernel<T, false, true, false> : log_probs_backward_kernel<T, false, false, false>);
+  if constexpr (sizeof(T) == 4)
+    if (keeps(a))
+      kernel = a.g2 ? (far ? log_probs_backward_kernel<T, true, true, true> : log_probs_backward_kernel<T, true, false, true>)
+                    : (far ? log_probs_backward_kernel<T, false, true, true> : log_probs_backward_kernel<T, false, false, true>);
   hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
@@ -810,8 +889,12 @@ template <typename T> hipError_t launch_distill_backward(RowsArgs a, bool tail, 
   a.per_row = grad_waves(a.R, a.V, sizeof(T));
   const bool far = streams(a, sizeof(T));
   const dim3 grid((unsigned)(((long long)a.R * a.per_row + 3) / 4));
-  auto kernel = tail ? (far ? distill_backward_kernel<T, true, true> : distill_backward_kernel<T, true, false>)
-                     : (far ? distill_backward_kernel<T, false, true> : distill_backward_kernel<T, false, false>);
+  auto kernel = tail ? (far ? distill_backward_kernel<T, true, true, false> : distill_backward_kernel<T, true, false, false>)
+                     : (far ? distill_backward_kernel<T, false, true, false> : distill_backward_kernel<T, false, false, false>);
+  if constexpr (sizeof(T) == 4)
+    if (keeps(a))
+      kernel = tail ? (far ? distill_backward_kernel<T, true, true, true> : distill_backward_kernel<T, true, false, true>)
+                    : (far ? distill_backward_kernel<T, false, true, true> : distill_backward_kernel<T, false, false, true>);
   hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
