@@ -234,6 +234,21 @@ def test_fp32_gradients_are_not_off_by_the_rounding_of_lse(O, rows, classes, pad
     assert off <= 2.0 ** -24 * float(room.norm()), off / (2.0 ** -24 * float(room.norm()))
 
 
+@pytest.mark.parametrize("dtype", DTYPES[1:], ids=str)
+def test_attention_rows_of_one_key_have_no_gradient(O, dtype):
+    """p = 1 whatever the score: dq and dk are 0, and not what rounding leaves of do . v - delta"""
+    for B, Lq, Lk, Hq, Hk, D, causal, nk in ((5, 200, 1, 4, 2, 64, False, None), (3, 30, 9, 4, 1, 96, False, [1, 9, 1]), (2, 700, 700, 2, 2, 128, True, None)):
+        q, do = normal((B, Lq, Hq, D), dtype, 1), normal((B, Lq, Hq, D), dtype, 2)
+        k, v = normal((B, Lk, Hk, D), dtype, 3), normal((B, Lk, Hk, D), dtype, 4)
+        got = run_attention(O, cuda(q), cuda(k), cuda(v), cuda(do), causal, None, None, cuda(lens(nk)))
+        R.check(got, R.attention(q, k, v, causal, None, None, nk, do))
+        for b in range(B):
+            if causal:
+                assert bool((got["dq"][b, 0] == 0).all())
+            elif nk is None or nk[b] == 1:
+                assert bool((got["dq"][b] == 0).all()) and bool((got["dk"][b] == 0).all())
+
+
 def test_scales_outside_of_32_bits_are_refused(O):
     """a scale that 32 bits hold as 0 would be read as the default; one that they hold as infinity (or whose product with log2(e) they do) has no exponentials"""
     q, z = torch.zeros((1, 4, 2, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((2, 50), device="cuda")

@@ -530,7 +530,8 @@ template <typename T, int DP> __device__ __forceinline__ void attn_few_keys(cons
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r)
-      if (32 * u + 4 * half + 8 * (r >> 2) + (r & 3) < few) delta = fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -ls)), dp[r], delta);
+      if (32 * u + 4 * half + 8 * (r >> 2) + (r & 3) < few)
+        delta = few == 1 ? dp[r] : fmaf(__builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -ls)), dp[r], delta);      // (one key: no gradient, not its rounding's)
   }
   delta += __shfl_xor(delta, 32, 64);
   if (few && half == 0) a.delta[at] = delta;
