@@ -67,7 +67,8 @@ def _scores(who, name, t, device):
         _refuse(who, f"{name} has to be a tensor on the GPU")
     if t.dtype not in DTYPES:
         _refuse(who, f"{name} is {t.dtype} (float32, float16 or bfloat16)")
-    _given(who, name, t)
+    if t.requires_grad or t.is_neg() or forward_ad._current_level >= 0:
+        _given(who, name, t)
     if device is not None and t.device != device:
         _refuse(who, f"{name} is on {t.device}, not on {device}")
     return t.device
@@ -77,7 +78,8 @@ def _plain(who, name, t, dtype, shape, device):
     """a contiguous tensor of the given type and shape; its address"""
     if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.shape == shape and t.is_contiguous()):
         _refuse(who, f"{name} has to be a contiguous {dtype} tensor {tuple(shape)} on {device}")
-    _given(who, name, t)
+    if t.requires_grad or t.is_neg() or forward_ad._current_level >= 0:
+        _given(who, name, t)
     p = t.data_ptr()
     if not p and t.numel():
         _refuse(who, f"{name} has no memory")
