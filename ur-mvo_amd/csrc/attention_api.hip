@@ -84,11 +84,7 @@ size_t part_kv_bytes(const urf_attn_config &c, int splits) {
 size_t part_q_bytes(const urf_attn_config &c, int splits) {
   return splits > 1 ? (size_t)splits * c.batch * c.q_heads * c.q_len * padded_dim(c) * sizeof(float) : 0;
 }
-size_t backward_bytes(const urf_attn_config &c) {
-  int kv, q;
-  backward_shape(c, &kv, &q);
-  return stat_bytes(c) + part_kv_bytes(c, kv) + part_q_bytes(c, q);
-}
+size_t backward_bytes(const urf_attn_config &c, int kv, int q) { return stat_bytes(c) + part_kv_bytes(c, kv) + part_q_bytes(c, q); }
 
 int check_config(const urf_attn_config *c, const char *who) {
   URF_CHECK(c, "%s: null configuration", who);
@@ -148,7 +144,9 @@ AttnArgs args_of(const urf_attn_config *c, const urf_attn_tensor *q, const urf_a
 extern "C" int urf_attn_workspace(const urf_attn_config *cfg, int backward, size_t *bytes) {
   if (check_config(cfg, "urf_attn_workspace")) return -2;
   URF_CHECK(bytes, "urf_attn_workspace: null pointer");
-  *bytes = backward ? backward_bytes(*cfg) : forward_bytes(*cfg);
+  int kv = 1, q = 1;
+  if (backward) backward_shape(*cfg, &kv, &q);
+  *bytes = backward ? backward_bytes(*cfg, kv, q) : forward_bytes(*cfg);
   return 0;
 }
 
@@ -193,13 +191,15 @@ extern "C" int urf_attn_backward(const urf_attn_config *cfg, const urf_attn_tens
     for (int y = 0; y < 5; ++y) URF_CHECK(!out[x] || out[x] != in[y], "%s: an output may not be an input", who);
     for (int y = 0; y < x; ++y) URF_CHECK(!out[x] || out[x] != out[y], "%s: two outputs share a base", who);
   }
-  const size_t need = backward_bytes(*cfg);
+  int kv_splits, q_splits;
+  backward_shape(*cfg, &kv_splits, &q_splits);
+  const size_t need = backward_bytes(*cfg, kv_splits, q_splits);
   URF_CHECK(d_work && work_bytes >= need && ((uintptr_t)d_work & 15) == 0, "%s: workspace of %zu bytes, %zu needed", who, work_bytes, need);
   AttnArgs a = args_of(cfg, q, k, v, d_q_lens, d_k_lens);
   a.o = view(o); a.dout = view(d_o); a.dq = view(dq); a.dk = view(dk); a.dv = view(dv);
   a.lse = (float *)d_lse;
   a.delta = (float *)d_work;
-  backward_shape(*cfg, &a.kv_splits, &a.q_splits);
+  a.kv_splits = kv_splits; a.q_splits = q_splits;
   a.norm_do = (float *)((char *)d_work + delta_bytes(*cfg));
   a.norm_v = (float *)((char *)a.norm_do + delta_bytes(*cfg));
   a.part_kv = (float *)((char *)d_work + stat_bytes(*cfg));
