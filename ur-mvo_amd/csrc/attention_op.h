@@ -539,8 +539,8 @@ template <typename T, int DP> __device__ __forceinline__ void attn_few_keys(cons
 
 // delta_i = do_i . o_i of the other rows: L lanes per row, 16 bytes of each tensor at a time; 8 where that is a row of 64 16-bit elements, 16
 // otherwise.  FEW: the first workgroups do the rows of few keys; 0 where none can have few.
-// Bound by memory: 2 x 4096 rows of 16 heads of 128, bf16, 67 MB each of o and do in 13 us (10.3 TB/s: what the forward pass wrote is in
-// the last-level cache).
+// Bound by memory: 2 x 4096 rows of 16 heads of 128, bf16, 67 MB each of o and do in 13 us, 15.8 with the rows of few keys (10.3 and 8.5
+// TB/s: what the forward pass wrote is in the last-level cache).
 template <typename T, int DP, int L, bool FEW>
 __global__ void __launch_bounds__(256, FEW ? 4 : 0) attn_delta_kernel(AttnArgs a) {
   extern __shared__ __align__(16) char lds[];
