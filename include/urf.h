@@ -659,7 +659,8 @@ int urf_log_probs(const urf_rows_config *cfg, const void *logits, const int *d_t
 int urf_log_probs_workspace(const urf_rows_config *cfg, int top, size_t *bytes);
 /* d_logits (rows of d_logits_stride elements) = the gradient of sum(log_prob * d_log_prob) + sum(entropy * d_entropy), from the
  * forward call's lse and entropy; d_entropy may be NULL.  A candidate that is a target twice gets both.  Rows that allow
- * nothing get 0. */
+ * nothing get 0.  Probabilities are relative to lse, whose rounding to 32 bits is one of 2^-24 |lse| in them (fp32 rows of up to 2048
+ * classes are normalised again, within 2^30 of 0). */
 int urf_log_probs_backward(const urf_rows_config *cfg, const void *logits, const int *d_targets, int n_targets, const float *d_lse,
                            const float *d_entropy, const float *d_d_log_prob, const float *d_d_entropy, void *d_logits,
                            long long d_logits_stride, void *stream);
